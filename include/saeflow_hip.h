@@ -26,7 +26,7 @@
 extern "C" {
 #endif
 
-#define SF_ABI_VERSION 4
+#define SF_ABI_VERSION 5
 
 /* The library is built with hidden symbol visibility; exactly these entry points are exported. */
 #ifndef SF_API
@@ -390,6 +390,49 @@ SF_API int sf_column_sums(const void* A, int64_t M, int64_t D, int64_t sa, int d
  * W_enc db_enc. */
 SF_API int sf_matvec(const void* W, int64_t R, int64_t C, int64_t swr, int64_t swc, int w_dt, const float* v,
               float sign, int accumulate, float* out, float* workspace, int64_t workspace_floats, void* stream);
+
+/*
+ * Rows in 8 bits (no reference counterpart): e4m3 codes with one power-of-two scale for each block of
+ * 128 elements along a row. Row r of a store of R rows over K elements: codes q + r * sq (sq bytes
+ * apart, a multiple of 16 and at least K rounded up to 128; 16-B aligned; zeros behind K) and scale
+ * bytes scale + r * ss (ss a multiple of 4 and at least ceil(K / 128) rounded up to 4; 4-B aligned).
+ * Element k is code * 2^(byte[k / 128] - 127).
+ *
+ * sf_quantize_rows: row (row0 + m) % R of the store from x[m] - shift, m < M <= R.
+ *   x [M, K] of x_dt, any strides; shift [K] contiguous of shift_dt, or NULL; the difference is formed
+ *   in fp32. Per block the scale is the smallest 2^e, e >= -127, with max |element| <= 448 * 2^e over
+ *   the finite elements; codes round to nearest even; NaN and infinities become NaN. The bytes up to
+ *   the padded ends of a row are zeroed.
+ * sf_dequantize_rows: out[m] = row + shift, in fp32, rounded to out_dt; the row is rows[m] (int64 ids on
+ *   the device; one outside [0, R) gives zeros), or (row0 + m) % R with rows NULL (then M <= R).
+ *   out [M, K], rows som elements apart.
+ */
+SF_API int sf_quantize_rows(const void* x, int64_t sxm, int64_t sxk, int x_dt, const void* shift, int shift_dt,
+                            int64_t M, int64_t K, void* q, int64_t sq, void* scale, int64_t ss, int64_t row0,
+                            int64_t R, void* stream);
+SF_API int sf_dequantize_rows(const void* q, int64_t sq, const void* scale, int64_t ss, int64_t R,
+                              const int64_t* rows, int64_t row0, const void* shift, int shift_dt, int64_t M,
+                              int64_t K, void* out, int64_t som, int out_dt, void* stream);
+
+/*
+ * sf_encode on 8-bit rows: out = act(x w^T + b_enc), x [M, K] and w [N, K] (a row a feature) as such
+ * rows, fp32 sums. b_enc [N] or NULL, thr [N], activations, row_nnz and rounding as in sf_encode;
+ * out [M, N], rows som elements apart.
+ *   sf_encode_fp8_rows  x as 8-bit rows (of an activation cache).
+ *   sf_encode_fp8       x [M, K] of x_dt with any strides, quantised as sf_quantize_rows does with
+ *                       shift b_dec (or NULL) into the workspace: caller-owned, 16-B aligned, at least
+ *                       sf_encode_fp8_workspace_size(M, K) bytes. Calls in flight at the same time must
+ *                       not share a workspace.
+ */
+SF_API int sf_encode_fp8_rows(const void* xq, int64_t sxq, const void* xs, int64_t sxs, const void* wq, int64_t swq,
+                              const void* ws, int64_t sws, const void* b_enc, int benc_dt, const void* thr, int thr_dt,
+                              void* out, int64_t som, int out_dt, int32_t* row_nnz, int64_t M, int64_t N, int64_t K,
+                              int act, void* stream);
+SF_API int sf_encode_fp8_workspace_size(int64_t M, int64_t K, int64_t* bytes);
+SF_API int sf_encode_fp8(const void* x, int64_t sxm, int64_t sxk, int x_dt, const void* b_dec, int bdec_dt,
+                         const void* wq, int64_t swq, const void* ws, int64_t sws, const void* b_enc, int benc_dt,
+                         const void* thr, int thr_dt, void* out, int64_t som, int out_dt, int32_t* row_nnz, int64_t M,
+                         int64_t N, int64_t K, int act, void* workspace, int64_t workspace_bytes, void* stream);
 
 #ifdef __cplusplus
 }

@@ -15,7 +15,7 @@ from pathlib import Path
 import torch
 
 LIB_PATH = Path(__file__).resolve().parent / "libsaeflow_hip.so"
-ABI_VERSION = 4
+ABI_VERSION = 5
 
 SF_OK, SF_EINVAL, SF_EHIP, SF_EUNSUPPORTED = 0, 1, 2, 3
 ACT = {"relu": 0, "jumprelu": 1, "none": 2}
@@ -65,6 +65,13 @@ SIGNATURES = {
     "sf_transpose": (_I32, [_P, _I64, _I64, _I64, _I32, _P, _P, _P]),
     "sf_column_sums": (_I32, [_P, _I64, _I64, _I64, _I32, ctypes.c_float, _I32, _P, _P, _I64, _P]),
     "sf_matvec": (_I32, [_P, _I64, _I64, _I64, _I64, _I32, _P, ctypes.c_float, _I32, _P, _P, _I64, _P]),
+    "sf_quantize_rows": (_I32, [_P, _I64, _I64, _I32, _P, _I32, _I64, _I64, _P, _I64, _P, _I64, _I64, _I64, _P]),
+    "sf_dequantize_rows": (_I32, [_P, _I64, _P, _I64, _I64, _P, _I64, _P, _I32, _I64, _I64, _P, _I64, _I32, _P]),
+    "sf_encode_fp8_rows": (_I32, [_P, _I64, _P, _I64, _P, _I64, _P, _I64, _P, _I32, _P, _I32, _P, _I64, _I32, _P, _I64,
+                                  _I64, _I64, _I32, _P]),
+    "sf_encode_fp8_workspace_size": (_I32, [_I64, _I64, _P]),
+    "sf_encode_fp8": (_I32, [_P, _I64, _I64, _I32, _P, _I32, _P, _I64, _P, _I64, _P, _I32, _P, _I32, _P, _I64, _I32, _P,
+                             _I64, _I64, _I64, _I32, _P, _I64, _P]),
 }
 
 _lib = None
@@ -148,4 +155,12 @@ def encode_workspace_bytes(M, K, w_code):
     """sf_encode_workspace_size, a function of its arguments alone."""
     nbytes = ctypes.c_int64()
     check(load().sf_encode_workspace_size(M, K, w_code, ctypes.byref(nbytes)))
+    return nbytes.value
+
+
+@functools.lru_cache(maxsize=256)
+def fp8_workspace_bytes(M, K):
+    """sf_encode_fp8_workspace_size, a function of its arguments alone."""
+    nbytes = ctypes.c_int64()
+    check(load().sf_encode_fp8_workspace_size(M, K, ctypes.byref(nbytes)))
     return nbytes.value

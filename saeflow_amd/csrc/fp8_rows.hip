@@ -1,0 +1,314 @@
+// 8-bit rows written and read back (format: fp8.h). Both are one pass over the data, bound by HBM.
+#include <algorithm>
+
+#include "fp8.h"
+
+namespace sff8 {
+
+// How the source lies: rows contiguous and 16-B aligned, or anything (element by element).
+enum Src { SRC_ROWS = 0, SRC_ANY = 1 };
+
+// Sixteen lanes take one block of 128, eight elements each: the maximum is four rotations within a
+// DPP row, each lane's eight codes are one 8-B store and the sixteen of a block one cache line.
+// Blocks are numbered row by row over [0, total), total < 2^31, so the row is a 32-bit division.
+template <int DT, int SRC>
+__global__ __launch_bounds__(256) void quantize_kernel(const void* x, int64_t sxm, int64_t sxk, const void* shift,
+                                                       int shift_dt, int shift_vec, int64_t K, uint32_t nb,
+                                                       uint32_t total, uint8_t* q, int64_t sq, uint8_t* scale,
+                                                       int64_t ss, int64_t row0, int64_t R, int pad) {
+  const uint32_t lane16 = threadIdx.x & 15;
+  for (uint32_t b = blockIdx.x * 16 + (threadIdx.x >> 4); b < total; b += gridDim.x * 16) {
+    const uint32_t m = b / nb, kb = b - m * nb;
+    const int64_t k0 = (int64_t)kb * BLOCK + lane16 * 8;
+    float v[8];
+    if (SRC == SRC_ROWS && k0 + 8 <= K) {
+      load8<DT>(x, (int64_t)m * sxm + k0, v);
+      if (shift_vec) {  // shift of x's type, 16-B aligned
+        float c[8];
+        load8<DT>(shift, k0, c);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] -= c[e];
+      } else if (shift) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] -= load_as_f32(shift, shift_dt, k0 + e);
+      }
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        v[e] = 0.f;
+        if (k0 + e < K) {
+          v[e] = load_as_f32(x, DT, (int64_t)m * sxm + (k0 + e) * sxk);
+          if (shift) v[e] -= load_as_f32(shift, shift_dt, k0 + e);
+        }
+      }
+    }
+    uint32_t top = 0;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) top = max(top, finite_bits(v[e]));
+    const uint32_t byte = scale_byte(max16(top));
+    const float inv = inverse_of(byte);
+    float u[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) u[e] = scaled(v[e], inv);
+    int64_t r = row0 + m;
+    if (r >= R) r -= R;
+    *(u32x2*)(q + r * sq + k0) = u32x2{pack4(u[0], u[1], u[2], u[3]), pack4(u[4], u[5], u[6], u[7])};
+    if (lane16 == 0) scale[r * ss + kb] = (uint8_t)byte;
+    if (lane16 > 0 && lane16 <= (uint32_t)pad && kb + 1 == nb) scale[r * ss + kb + lane16] = 0;
+  }
+}
+
+// Columns contiguous (x[m, k] at m + k * sxk, a dictionary's W_enc^T): a workgroup takes 64 rows x one
+// block of 128, read as 128 row pieces of 64 elements (128 B of bf16) into LDS, and every four lanes
+// write one row's 128 codes, a whole cache line. LDS piece k lies at k * 64 E + (k / 32) * 16 E: the
+// four lanes of a row read pieces 32 apart, 16 rows at once, which fills the 64 banks exactly.
+template <int DT>
+__global__ __launch_bounds__(256) void quantize_columns_kernel(const void* x, int64_t sxk, int vec, const void* shift,
+                                                               int shift_dt, int64_t M, int64_t K, int64_t nb,
+                                                               uint8_t* q, int64_t sq, uint8_t* scale, int64_t ss,
+                                                               int64_t row0, int64_t R, int pad) {
+  constexpr int E = DT == SF_F32 ? 4 : 2, EPC = 16 / E, CPR = 64 / EPC, PER = 128 * CPR / 256;
+  __shared__ __attribute__((aligned(16))) char st[128 * 64 * E + 4 * 16 * E];
+  const int t = threadIdx.x;
+  const int64_t m0 = (int64_t)blockIdx.x * 64, kb = blockIdx.y, k0 = kb * BLOCK;
+  if (vec && m0 + 64 <= M) {
+    u32x4 v[PER];
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      const int k = (i * 256 + t) / CPR, c = t % CPR;
+      v[i] = u32x4{0, 0, 0, 0};
+      if (k0 + k < K) v[i] = *(const u32x4*)((const char*)x + ((k0 + k) * sxk + m0) * E + c * 16);
+    }
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      const int k = (i * 256 + t) / CPR, c = t % CPR;
+      *(u32x4*)(st + k * 64 * E + (k >> 5) * 16 * E + c * 16) = v[i];
+    }
+  } else {
+    for (int i = t; i < 128 * 64; i += 256) {
+      const int k = i >> 6, m = i & 63;
+      const uint32_t bits = k0 + k < K && m0 + m < M ? load_bits(x, DT, (k0 + k) * sxk + m0 + m) : 0u;
+      char* dst = st + k * 64 * E + (k >> 5) * 16 * E + m * E;
+      if constexpr (E == 4) *(uint32_t*)dst = bits;
+      else *(u16*)dst = (u16)bits;
+    }
+  }
+  __syncthreads();
+  const int m = t >> 2, kq = t & 3;
+  float v[32];
+  uint32_t top = 0;
+#pragma unroll
+  for (int i = 0; i < 32; ++i) {
+    const int k = kq * 32 + i;
+    v[i] = load_as_f32(st + k * 64 * E + kq * 16 * E, DT, m);
+    if (shift && k0 + k < K) v[i] -= load_as_f32(shift, shift_dt, k0 + k);
+    top = max(top, finite_bits(v[i]));
+  }
+  const uint32_t byte = scale_byte(max4(top));
+  const float inv = inverse_of(byte);
+  if (m0 + m >= M) return;
+  int64_t r = row0 + m0 + m;
+  if (r >= R) r -= R;
+  uint32_t w[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i)
+    w[i] = pack4(scaled(v[4 * i], inv), scaled(v[4 * i + 1], inv), scaled(v[4 * i + 2], inv), scaled(v[4 * i + 3], inv));
+  char* dst = (char*)q + r * sq + k0 + kq * 32;
+  *(u32x4*)dst = u32x4{w[0], w[1], w[2], w[3]};
+  *(u32x4*)(dst + 16) = u32x4{w[4], w[5], w[6], w[7]};
+  if (kq == 0) scale[r * ss + kb] = (uint8_t)byte;
+  if (kq > 0 && kq <= pad && kb + 1 == nb) scale[r * ss + kb + kq] = 0;
+}
+
+// Eight codes a lane, sixteen lanes a block, as quantize_kernel. Row m of the result is row
+// (row0 + m) % R of the store, or rows[m]; an id outside [0, R) gives zeros.
+template <int ODT>
+__global__ __launch_bounds__(256) void dequantize_kernel(const uint8_t* q, int64_t sq, const uint8_t* scale, int64_t ss,
+                                                         int64_t R, const int64_t* rows, int64_t row0,
+                                                         const void* shift, int shift_dt, int shift_vec, int64_t K,
+                                                         uint32_t nb, uint32_t total, void* out, int64_t som, int vec) {
+  const uint32_t lane16 = threadIdx.x & 15;
+  for (uint32_t b = blockIdx.x * 16 + (threadIdx.x >> 4); b < total; b += gridDim.x * 16) {
+    const uint32_t m = b / nb, kb = b - m * nb;
+    const int64_t k0 = (int64_t)kb * BLOCK + lane16 * 8;
+    if (k0 >= K) continue;
+    int64_t r;
+    if (rows) {
+      r = rows[m];
+    } else {
+      r = row0 + m;
+      if (r >= R) r -= R;
+    }
+    float v[8];
+    if (r >= 0 && r < R) {
+      const u32x2 c = *(const u32x2*)(q + r * sq + k0);
+      const float f = scale_of(scale[r * ss + kb]);
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const f32x2 lo = __builtin_amdgcn_cvt_pk_f32_fp8((int)c[i], false);
+        const f32x2 hi = __builtin_amdgcn_cvt_pk_f32_fp8((int)c[i], true);
+        v[4 * i] = lo[0] * f;
+        v[4 * i + 1] = lo[1] * f;
+        v[4 * i + 2] = hi[0] * f;
+        v[4 * i + 3] = hi[1] * f;
+      }
+      if (shift_vec && k0 + 8 <= K) {
+        float s[8];
+        load8<ODT>(shift, k0, s);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] += s[e];
+      } else if (shift) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+          if (k0 + e < K) v[e] += load_as_f32(shift, shift_dt, k0 + e);
+      }
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[e] = 0.f;
+    }
+    if (vec && k0 + 8 <= K) {
+      if constexpr (ODT == SF_F32) {
+        float* dst = (float*)out + m * som + k0;
+        *(float4*)dst = float4{v[0], v[1], v[2], v[3]};
+        *(float4*)(dst + 4) = float4{v[4], v[5], v[6], v[7]};
+      } else {
+        u32x4 o;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[e] = f32_to_bits(v[2 * e], ODT) | f32_to_bits(v[2 * e + 1], ODT) << 16;
+        *(u32x4*)((u16*)out + m * som + k0) = o;
+      }
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        if (k0 + e < K) {
+          if constexpr (ODT == SF_F32) ((float*)out)[m * som + k0 + e] = v[e];
+          else ((u16*)out)[m * som + k0 + e] = (u16)f32_to_bits(v[e], ODT);
+        }
+    }
+  }
+}
+
+namespace {
+
+constexpr int64_t MOST_BLOCKS = 1ll << 30;  // of one launch (32-bit block numbers)
+
+bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
+
+// Workgroups of 16 blocks each: enough to fill the chip several times over, then a grid stride.
+unsigned grid_of(int64_t total) { return (unsigned)std::min<int64_t>((total + 15) / 16, 1 << 16); }
+
+int check_store(const void* q, int64_t sq, const void* scale, int64_t ss, int64_t R, int64_t K) {
+  SF_REQUIRE(q && scale, "codes and scales must not be NULL");
+  SF_REQUIRE(aligned16(q) && sq % 16 == 0, "rows of codes must be 16-B aligned");
+  SF_REQUIRE(((uintptr_t)scale & 3) == 0 && ss % 4 == 0, "rows of scales must be 4-B aligned");
+  SF_REQUIRE(sq >= code_bytes(K), "rows of codes hold %lld bytes, %lld are needed for %lld elements", (long long)sq,
+             (long long)code_bytes(K), (long long)K);
+  SF_REQUIRE(ss >= scale_bytes(K), "rows of scales hold %lld bytes, %lld are needed for %lld elements", (long long)ss,
+             (long long)scale_bytes(K), (long long)K);
+  SF_REQUIRE(R >= 0, "negative number of rows");
+  return SF_OK;
+}
+
+template <int DT>
+int quantize_typed(const void* x, int64_t sxm, int64_t sxk, const void* shift, int shift_dt, int64_t M, int64_t K,
+                   void* q, int64_t sq, void* scale, int64_t ss, int64_t row0, int64_t R, hipStream_t s) {
+  constexpr int E = DT == SF_F32 ? 4 : 2;
+  const int64_t nb = blocks_of(K);
+  const int pad = (int)(scale_bytes(K) - nb);
+  if (sxm == 1 && sxk != 1 && M >= 16 && nb < 65536) {
+    // 65536 * 64 rows a launch at most
+    const int vec = aligned16(x) && sxk * E % 16 == 0;
+    for (int64_t m = 0; m < M; m += 64 << 16) {
+      const int64_t n = std::min<int64_t>(M - m, 64 << 16);
+      const int64_t at = (row0 + m) % R;
+      hipLaunchKernelGGL((quantize_columns_kernel<DT>), dim3((unsigned)((n + 63) / 64), (unsigned)nb), dim3(256), 0, s,
+                         (const char*)x + m * E, sxk, vec, shift, shift_dt, n, K, nb, (uint8_t*)q, sq, (uint8_t*)scale,
+                         ss, at, R, pad);
+      SF_LAUNCH_CHECK("quantize_columns");
+    }
+    return SF_OK;
+  }
+  const bool rows = sxk == 1 && aligned16(x) && sxm * E % 16 == 0;
+  const int svec = shift && shift_dt == DT && aligned16(shift);
+  const int64_t step = std::max<int64_t>(1, MOST_BLOCKS / nb);
+  for (int64_t m = 0; m < M; m += step) {
+    const int64_t n = std::min(M - m, step);
+    const int64_t at = (row0 + m) % R;
+    const dim3 grid(grid_of(n * nb)), block(256);
+    const char* xm = (const char*)x + m * sxm * E;
+    if (rows)
+      hipLaunchKernelGGL((quantize_kernel<DT, SRC_ROWS>), grid, block, 0, s, xm, sxm, sxk, shift, shift_dt, svec, K,
+                         (uint32_t)nb, (uint32_t)(n * nb), (uint8_t*)q, sq, (uint8_t*)scale, ss, at, R, pad);
+    else
+      hipLaunchKernelGGL((quantize_kernel<DT, SRC_ANY>), grid, block, 0, s, xm, sxm, sxk, shift, shift_dt, svec, K,
+                         (uint32_t)nb, (uint32_t)(n * nb), (uint8_t*)q, sq, (uint8_t*)scale, ss, at, R, pad);
+    SF_LAUNCH_CHECK("quantize");
+  }
+  return SF_OK;
+}
+
+}  // namespace
+
+int launch_quantize(const void* x, int64_t sxm, int64_t sxk, int x_dt, const void* shift, int shift_dt, int64_t M,
+                    int64_t K, void* q, int64_t sq, void* scale, int64_t ss, int64_t row0, int64_t R, hipStream_t s) {
+  switch (x_dt) {
+    case SF_F32: return quantize_typed<SF_F32>(x, sxm, sxk, shift, shift_dt, M, K, q, sq, scale, ss, row0, R, s);
+    case SF_BF16: return quantize_typed<SF_BF16>(x, sxm, sxk, shift, shift_dt, M, K, q, sq, scale, ss, row0, R, s);
+    default: return quantize_typed<SF_F16>(x, sxm, sxk, shift, shift_dt, M, K, q, sq, scale, ss, row0, R, s);
+  }
+}
+
+}  // namespace sff8
+
+extern "C" int sf_quantize_rows(const void* x, int64_t sxm, int64_t sxk, int x_dt, const void* shift, int shift_dt,
+                                int64_t M, int64_t K, void* q, int64_t sq, void* scale, int64_t ss, int64_t row0,
+                                int64_t R, void* stream) {
+  using namespace sff8;
+  sf_clear_error();
+  SF_REQUIRE(sf_valid_dtype(x_dt) && (!shift || sf_valid_dtype(shift_dt)), "unsupported dtype code");
+  SF_REQUIRE(M >= 0 && K >= 1 && K <= (1 << 24), "bad shape [%lld, %lld]", (long long)M, (long long)K);
+  if (M == 0) return SF_OK;
+  SF_REQUIRE(x, "x must not be NULL");
+  if (const int rc = check_store(q, sq, scale, ss, R, K)) return rc;
+  SF_REQUIRE(M <= R, "%lld rows do not fit %lld", (long long)M, (long long)R);
+  SF_REQUIRE(row0 >= 0 && row0 < R, "first row %lld outside [0, %lld)", (long long)row0, (long long)R);
+  return launch_quantize(x, sxm, sxk, x_dt, shift, shift_dt, M, K, q, sq, scale, ss, row0, R, (hipStream_t)stream);
+}
+
+extern "C" int sf_dequantize_rows(const void* q, int64_t sq, const void* scale, int64_t ss, int64_t R,
+                                  const int64_t* rows, int64_t row0, const void* shift, int shift_dt, int64_t M,
+                                  int64_t K, void* out, int64_t som, int out_dt, void* stream) {
+  using namespace sff8;
+  sf_clear_error();
+  SF_REQUIRE(sf_valid_dtype(out_dt) && (!shift || sf_valid_dtype(shift_dt)), "unsupported dtype code");
+  SF_REQUIRE(M >= 0 && K >= 1 && K <= (1 << 24), "bad shape [%lld, %lld]", (long long)M, (long long)K);
+  if (M == 0) return SF_OK;
+  if (const int rc = check_store(q, sq, scale, ss, R, K)) return rc;
+  SF_REQUIRE(out, "out must not be NULL");
+  SF_REQUIRE(som >= K || M == 1, "rows of the result overlap");
+  if (!rows) {
+    SF_REQUIRE(M <= R, "%lld rows asked for of %lld", (long long)M, (long long)R);
+    SF_REQUIRE(row0 >= 0 && row0 < R, "first row %lld outside [0, %lld)", (long long)row0, (long long)R);
+  }
+  const int64_t nb = blocks_of(K), step = std::max<int64_t>(1, MOST_BLOCKS / nb);
+  const int E = sf_dtype_size(out_dt);
+  const int vec = aligned16(out) && som * E % 16 == 0;
+  const int svec = shift && shift_dt == out_dt && aligned16(shift);
+  for (int64_t m = 0; m < M; m += step) {
+    const int64_t n = std::min(M - m, step);
+    const int64_t at = rows ? 0 : (row0 + m) % R;
+    const int64_t* ids = rows ? rows + m : nullptr;
+    const dim3 grid(grid_of(n * nb)), block(256);
+    void* o = (char*)out + m * som * E;
+    const hipStream_t s = (hipStream_t)stream;
+    auto go = [&](auto kernel) {
+      hipLaunchKernelGGL(kernel, grid, block, 0, s, (const uint8_t*)q, sq, (const uint8_t*)scale, ss, R, ids, at, shift,
+                         shift_dt, svec, K, (uint32_t)nb, (uint32_t)(n * nb), o, som, vec);
+    };
+    if (out_dt == SF_F32) go(dequantize_kernel<SF_F32>);
+    else if (out_dt == SF_BF16) go(dequantize_kernel<SF_BF16>);
+    else go(dequantize_kernel<SF_F16>);
+    SF_LAUNCH_CHECK("dequantize");
+  }
+  return SF_OK;
+}

@@ -1,0 +1,203 @@
+"""Rows in 8 bits on gfx950: written, read back, and multiplied (C ABI, include/saeflow_hip.h).
+
+The reference has no counterpart. A row is held as e4m3 codes with one power-of-two scale for each
+block of 128 elements (the last block may be short): element = code * 2^(byte - 127), the byte's 2^e
+the smallest, e >= -127, that brings the block's largest finite magnitude to 448 or less. Codes round
+to nearest even, so an element keeps four significant bits down to 2^-6 of its scale and an absolute
+2^-10 of it below; NaN and infinities become NaN. 16-bit rows take half the memory, fp32 a quarter.
+"""
+
+import torch
+
+from .. import _lib
+from .encode import _vector
+
+BLOCK = 128
+ACTIVATIONS = {"none": _lib.ACT["none"], "relu": _lib.ACT["relu"], "jumprelu": _lib.ACT["jumprelu"]}
+
+
+def _up(n, m):
+    return -(-n // m) * m
+
+
+class Fp8Rows:
+    """R rows of d elements in 8 bits: `q` [R, d rounded up to 128] float8_e4m3fn, zeros behind d, and
+    `scale` [R, ceil(d / 128) rounded up to 4] uint8. Slicing rows gives a view."""
+
+    __slots__ = ("q", "scale", "d")
+
+    def __init__(self, q, scale, d):
+        if q.dtype != torch.float8_e4m3fn or scale.dtype != torch.uint8:
+            raise ValueError(f"8-bit rows are float8_e4m3fn codes and uint8 scales, got {q.dtype} and {scale.dtype}")
+        if d < 1 or q.dim() != 2 or scale.dim() != 2 or q.shape[0] != scale.shape[0]:
+            raise ValueError(f"bad shapes for rows of {d}: codes {tuple(q.shape)}, scales {tuple(scale.shape)}")
+        if q.shape[1] != _up(d, BLOCK) or scale.shape[1] != _up(_up(d, BLOCK) // BLOCK, 4):
+            raise ValueError(f"rows of {d} are padded to {_up(d, BLOCK)} codes and {_up(_up(d, BLOCK) // BLOCK, 4)} "
+                             f"scales, got {q.shape[1]} and {scale.shape[1]}")
+        if q.stride(1) != 1 or scale.stride(1) != 1:
+            raise ValueError("codes and scales must be contiguous along a row")
+        self.q, self.scale, self.d = q, scale, d
+
+    @classmethod
+    def empty(cls, rows, d, device="cuda"):
+        """Room for `rows` rows, uninitialised."""
+        kp = _up(d, BLOCK)
+        return cls(torch.empty(rows, kp, dtype=torch.float8_e4m3fn, device=device),
+                   torch.empty(rows, _up(kp // BLOCK, 4), dtype=torch.uint8, device=device), d)
+
+    @classmethod
+    def from_parts(cls, codes, scale):
+        """Rows from codes [R, d] (float8_e4m3fn) and scale bytes [R, ceil(d / 128)], padded as needed."""
+        if codes.dtype != torch.float8_e4m3fn or codes.dim() != 2:
+            raise ValueError(f"codes must be a float8_e4m3fn matrix, got {codes.dtype} {list(codes.shape)}")
+        R, d = codes.shape
+        kp, sp = _up(d, BLOCK), _up(_up(d, BLOCK) // BLOCK, 4)
+        if scale.shape != (R, kp // BLOCK):
+            raise ValueError(f"codes {tuple(codes.shape)} need scales of shape {(R, kp // BLOCK)}, got {tuple(scale.shape)}")
+        if kp != d or codes.stride(1) != 1:
+            codes = torch.nn.functional.pad(codes.view(torch.uint8), (0, kp - d)).view(torch.float8_e4m3fn)
+        return cls(codes, torch.nn.functional.pad(scale, (0, sp - kp // BLOCK)), d)
+
+    @property
+    def shape(self):
+        return torch.Size((self.q.shape[0], self.d))
+
+    @property
+    def device(self):
+        return self.q.device
+
+    @property
+    def nbytes(self):
+        return self.q.nbytes + self.scale.nbytes
+
+    def __len__(self):
+        return self.q.shape[0]
+
+    def __getitem__(self, rows):
+        if not isinstance(rows, slice):
+            raise TypeError("8-bit rows are sliced; dequantize_rows takes row ids")
+        return Fp8Rows(self.q[rows], self.scale[rows], self.d)
+
+    def to(self, device, non_blocking=False):
+        return Fp8Rows(self.q.to(device, non_blocking=non_blocking), self.scale.to(device, non_blocking=non_blocking), self.d)
+
+    def __repr__(self):
+        return f"Fp8Rows({len(self)} x {self.d}, {self.device})"
+
+
+def _shift(t, n, name):
+    return None if t is None else _vector(t, n, name)
+
+
+def quantize_rows(x, *, shift=None, out=None, row0=0):
+    """x [M, d] in fp32, bf16 or fp16 (any strides; a transposed matrix is read along its own rows) as
+    8-bit rows, minus `shift` [d] if given (the difference in fp32).
+
+    out: Fp8Rows to write into, rows (row0 + m) % len(out); a new Fp8Rows of M rows if None.
+    """
+    if x.dim() != 2:
+        raise ValueError(f"x must have two dimensions, got {list(x.shape)}")
+    M, d = x.shape
+    if d < 1:
+        raise ValueError("rows of no elements have no 8-bit form")
+    shift = _shift(shift, d, "shift")
+    if out is None:
+        if row0:
+            raise ValueError("row0 is a row of `out`, which is not given")
+        _lib.require_gpu(("x", x))
+        out = Fp8Rows.empty(M, d, x.device)
+    elif out.d != d:
+        raise ValueError(f"out holds rows of {out.d}, x has {d}")
+    dev = _lib.require_gpu(("x", x), ("shift", shift), ("out", out.q), ("out", out.scale))
+    if M == 0:
+        return out
+    with _lib.device(dev):
+        _lib.check(_lib.load().sf_quantize_rows(
+            x.data_ptr(), x.stride(0), x.stride(1), _lib.dtype_code(x, "x"), _lib.ptr(shift),
+            0 if shift is None else _lib.dtype_code(shift, "shift"), M, d, out.q.data_ptr(), out.q.stride(0),
+            out.scale.data_ptr(), out.scale.stride(0), row0, len(out), _lib.stream(dev)))
+    return out
+
+
+def dequantize_rows(rows8, rows=None, *, row0=0, count=None, shift=None, out_dtype=torch.bfloat16):
+    """Rows read back, plus `shift` [d] if given (the sum in fp32, then rounded to out_dtype): those with
+    the ids `rows` (int64, in any order; an id outside the store gives zeros), or `count` rows from row0 on,
+    going on at row 0 behind the last (all of them by default)."""
+    R, d = rows8.shape
+    if rows is not None:
+        if rows.dtype != torch.int64 or rows.dim() != 1:
+            raise ValueError(f"rows must be a one-dimensional int64 tensor, got {rows.dtype} {list(rows.shape)}")
+        if row0 or count is not None:
+            raise ValueError("rows are named by ids or by row0 and count, not by both")
+        rows = rows.contiguous()
+        M = rows.numel()
+    else:
+        M = R if count is None else count
+        if M < 0 or M > R:
+            raise ValueError(f"count must lie in [0, {R}], got {M}")
+    shift = _shift(shift, d, "shift")
+    dev = _lib.require_gpu(("rows8", rows8.q), ("rows8", rows8.scale), ("rows", rows), ("shift", shift))
+    out = torch.empty(M, d, dtype=out_dtype, device=dev)
+    code = _lib.dtype_code(out, "out_dtype")
+    if M == 0:
+        return out
+    with _lib.device(dev):
+        _lib.check(_lib.load().sf_dequantize_rows(
+            rows8.q.data_ptr(), rows8.q.stride(0), rows8.scale.data_ptr(), rows8.scale.stride(0), R, _lib.ptr(rows),
+            row0, _lib.ptr(shift), 0 if shift is None else _lib.dtype_code(shift, "shift"), M, d, out.data_ptr(), d,
+            code, _lib.stream(dev)))
+    return out
+
+
+def fused_encode_fp8(x, W, b_enc=None, threshold=None, activation="relu", *, b_dec=None, out_dtype=None, row_nnz=None):
+    """fused_encode on 8-bit rows: act(x W^T + b_enc) [M, d_sae] with fp32 sums on the 8-bit matrix cores.
+
+    x: Fp8Rows [M, d_in], or tokens [M, d_in] in fp32, bf16 or fp16, which are quantised on the way
+      (minus `b_dec` if given).
+    W: Fp8Rows [d_sae, d_in], a row a feature (quantize_rows(W_enc.T)).
+    activation: "relu", "none", or "jumprelu" with a per-feature `threshold` [d_sae].
+    out_dtype: x's own, bfloat16 for Fp8Rows. row_nnz: as in fused_encode.
+    """
+    if activation not in ACTIVATIONS:
+        raise ValueError(f"fused_encode_fp8 supports {list(ACTIVATIONS)}, got {activation!r}")
+    if activation == "jumprelu" and threshold is None:
+        raise ValueError("jumprelu needs a threshold")
+    held = isinstance(x, Fp8Rows)
+    if not isinstance(W, Fp8Rows):
+        raise ValueError("W must be Fp8Rows, a row a feature: quantize_rows(W_enc.T)")
+    if held and b_dec is not None:
+        raise ValueError("b_dec is subtracted before tokens are quantised; 8-bit rows are taken as they are")
+    if not held and x.dim() != 2:
+        raise ValueError(f"x must have two dimensions, got {list(x.shape)}")
+    (M, d), (N, d_w) = x.shape, W.shape
+    if d != d_w:
+        raise ValueError(f"x has d_in={d} but W has d_in={d_w}")
+    if out_dtype is None:
+        out_dtype = torch.bfloat16 if held else x.dtype
+    dev = _lib.require_gpu(("x", x.q if held else x), ("x", x.scale if held else None), ("W", W.q), ("W", W.scale),
+                           ("b_enc", b_enc), ("b_dec", b_dec), ("threshold", threshold), ("row_nnz", row_nnz))
+    b_enc, b_dec = _shift(b_enc, N, "b_enc"), _shift(b_dec, d, "b_dec")
+    threshold = _vector(threshold, N, "threshold") if activation == "jumprelu" else None
+    if row_nnz is not None:
+        if row_nnz.dtype != torch.int32 or row_nnz.dim() != 1 or row_nnz.numel() != M or not row_nnz.is_contiguous():
+            raise ValueError(f"row_nnz must be a contiguous int32 tensor of shape [{M}]")
+    out = torch.empty(M, N, dtype=out_dtype, device=dev)
+    code = _lib.dtype_code(out, "out_dtype")
+    if M == 0 or N == 0:
+        return out
+    lib = _lib.load()
+    tail = (W.q.data_ptr(), W.q.stride(0), W.scale.data_ptr(), W.scale.stride(0), _lib.ptr(b_enc),
+            0 if b_enc is None else _lib.dtype_code(b_enc, "b_enc"), _lib.ptr(threshold),
+            0 if threshold is None else _lib.dtype_code(threshold, "threshold"), out.data_ptr(), N, code,
+            _lib.ptr(row_nnz), M, N, d, ACTIVATIONS[activation])
+    with _lib.device(dev):
+        if held:
+            _lib.check(lib.sf_encode_fp8_rows(x.q.data_ptr(), x.q.stride(0), x.scale.data_ptr(), x.scale.stride(0),
+                                              *tail, _lib.stream(dev)))
+        else:
+            x_code = _lib.dtype_code(x, "x")
+            ws = torch.empty(_lib.fp8_workspace_bytes(M, d), dtype=torch.uint8, device=dev)
+            _lib.check(lib.sf_encode_fp8(x.data_ptr(), x.stride(0), x.stride(1), x_code, _lib.ptr(b_dec),
+                                         0 if b_dec is None else _lib.dtype_code(b_dec, "b_dec"), *tail, ws.data_ptr(),
+                                         ws.numel(), _lib.stream(dev)))
+    return out
