@@ -418,7 +418,8 @@ SF_API int sf_dequantize_rows(const void* q, int64_t sq, const void* scale, int6
  * sf_encode on 8-bit rows: out = act(x w^T + b_enc), x [M, K] and w [N, K] (a row a feature) as such
  * rows, fp32 sums. b_enc [N] or NULL, thr [N], activations, row_nnz and rounding as in sf_encode;
  * out [M, N], rows som elements apart.
- *   sf_encode_fp8_rows  x as 8-bit rows (of an activation cache).
+ *   sf_encode_fp8_rows  x as 8-bit rows (of an activation cache). workspace: caller-owned, 16-B
+ *                       aligned, at least sf_encode_fp8_workspace_size(0, K) bytes (tile counters).
  *   sf_encode_fp8       x [M, K] of x_dt with any strides, quantised as sf_quantize_rows does with
  *                       shift b_dec (or NULL) into the workspace: caller-owned, 16-B aligned, at least
  *                       sf_encode_fp8_workspace_size(M, K) bytes. Calls in flight at the same time must
@@ -427,7 +428,7 @@ SF_API int sf_dequantize_rows(const void* q, int64_t sq, const void* scale, int6
 SF_API int sf_encode_fp8_rows(const void* xq, int64_t sxq, const void* xs, int64_t sxs, const void* wq, int64_t swq,
                               const void* ws, int64_t sws, const void* b_enc, int benc_dt, const void* thr, int thr_dt,
                               void* out, int64_t som, int out_dt, int32_t* row_nnz, int64_t M, int64_t N, int64_t K,
-                              int act, void* stream);
+                              int act, void* workspace, int64_t workspace_bytes, void* stream);
 SF_API int sf_encode_fp8_workspace_size(int64_t M, int64_t K, int64_t* bytes);
 SF_API int sf_encode_fp8(const void* x, int64_t sxm, int64_t sxk, int x_dt, const void* b_dec, int bdec_dt,
                          const void* wq, int64_t swq, const void* ws, int64_t sws, const void* b_enc, int benc_dt,

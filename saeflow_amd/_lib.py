@@ -68,7 +68,7 @@ SIGNATURES = {
     "sf_quantize_rows": (_I32, [_P, _I64, _I64, _I32, _P, _I32, _I64, _I64, _P, _I64, _P, _I64, _I64, _I64, _P]),
     "sf_dequantize_rows": (_I32, [_P, _I64, _P, _I64, _I64, _P, _I64, _P, _I32, _I64, _I64, _P, _I64, _I32, _P]),
     "sf_encode_fp8_rows": (_I32, [_P, _I64, _P, _I64, _P, _I64, _P, _I64, _P, _I32, _P, _I32, _P, _I64, _I32, _P, _I64,
-                                  _I64, _I64, _I32, _P]),
+                                  _I64, _I64, _I32, _P, _I64, _P]),
     "sf_encode_fp8_workspace_size": (_I32, [_I64, _I64, _P]),
     "sf_encode_fp8": (_I32, [_P, _I64, _I64, _I32, _P, _I32, _P, _I64, _P, _I64, _P, _I32, _P, _I32, _P, _I64, _I32, _P,
                              _I64, _I64, _I64, _I32, _P, _I64, _P]),

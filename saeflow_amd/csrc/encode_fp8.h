@@ -259,4 +259,431 @@ __global__ __launch_bounds__(TL::NT, TL::ST * TL::NS > 81920 ? (TL::NW + 3) / 4 
   }
 }
 
+
+// dword of a scale row to LDS at wave_base + 4 * lane
+__device__ __forceinline__ void dma4(__amdgpu_buffer_rsrc_t r, char* wave_base, uint32_t voff, uint32_t soff) {
+  __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (lds_void*)wave_base, 4, (int)voff, (int)soff, 0, 0);
+}
+
+// Feature (within a block of 32) that row i of a W fragment holds. Lane half h of an MFMA result has the
+// rows 8 g + 4 h + r; with this order they are the consecutive features 16 h + 4 g + r, 32 B of a row.
+__device__ __forceinline__ int frag_feature(int i) { return (i & 4) * 4 + (i >> 3) * 4 + (i & 3); }
+
+// Three bf16 pieces of a fp32 value, whose sum it is (8 significant bits each; a lone first piece for
+// infinities and NaN), as two dwords.
+__device__ __forceinline__ sfenc::u32x2 pieces(float v) {
+  const float p0 = bf16_to_f32(f32_to_bf16(v));
+  const float r = v - p0;
+  const bool fine = r == r && fabsf(p0) < __builtin_inff();
+  const float p1 = bf16_to_f32(f32_to_bf16(r));
+  return sfenc::u32x2{f32_to_bf16(v) | (fine ? f32_to_bf16(r) << 16 : 0u), fine ? f32_to_bf16(r - p1) : 0u};
+}
+
+// 16 B of a result row, at any element's address
+typedef sfenc::u32x4 u32x4_any __attribute__((aligned(2)));
+
+// Epilogue of a wave's 128x128 tile of 16-bit results at token m0, feature n0, through 16 KiB of LDS, two
+// passes of 64 tokens; fragment rows in frag_feature order. PLAIN: relu or none and no counts, one
+// instruction an element (gfx950's v_maximum3_f32 keeps a NaN) before the conversion; otherwise as
+// sfenc::epilogue, with the thresholds s_t. RAGGED: the tile reaches past M or N.
+struct Out {
+  char* out;
+  int64_t som;
+  int32_t* row_nnz;
+  int64_t M, N;
+  int act;
+};
+template <int ODT, bool PLAIN, bool RAGGED>
+__device__ __forceinline__ void f8_epilogue(const Out& a, f32x16 (&acc)[4][4], int64_t m0, int64_t n0, int lane,
+                                            const float* s_t, char* reg) {
+  using namespace sfenc;
+  float lo = a.act == SF_ACT_NONE ? -__builtin_inff() : 0.f;
+  asm volatile("" : "+v"(lo));  // (opaque: else a maximum with 0 and a select)
+  const int h = lane >> 5, unit = lane & 15;
+  const int rows = RAGGED ? (int)max((int64_t)0, min((int64_t)128, a.M - m0)) : 128;
+  const int cols = RAGGED ? (int)max((int64_t)0, min((int64_t)128, a.N - n0)) : 128;
+  // (opaque, so that no multiples of it are formed ahead of the tile loop and spilled)
+  int64_t som = a.som;
+  asm volatile("" : "+s"(som));
+  char* dst = (char*)a.out + ((m0 + lane / 16) * som + n0 + unit * 8) * 2;
+#pragma unroll
+  for (int pass = 0; pass < 2; ++pass) {
+    int cnt[2] = {0, 0};
+#pragma unroll
+    for (int nb = 0; nb < 4; ++nb) {
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {  // eight consecutive features
+        const int cl = nb * 32 + h * 16 + half * 8;
+        float thv[8];
+        if constexpr (!PLAIN) {
+          const float4 ta = *(const float4*)(s_t + cl), tb = *(const float4*)(s_t + cl + 4);
+          thv[0] = ta.x; thv[1] = ta.y; thv[2] = ta.z; thv[3] = ta.w;
+          thv[4] = tb.x; thv[5] = tb.y; thv[6] = tb.z; thv[7] = tb.w;
+        }
+#pragma unroll
+        for (int mi = 0; mi < 2; ++mi) {
+          const int rl = mi * 32 + (lane & 31);
+          float o[8];
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            const float pre = acc[nb][pass * 2 + mi][half * 8 + e];
+            if constexpr (PLAIN) {
+              o[e] = __builtin_elementwise_maximum(pre, lo);
+            } else {
+              const bool keep = !(pre <= thv[e]);
+              o[e] = keep ? pre : 0.f;
+              cnt[mi] += keep && (!RAGGED || cl + e < cols) ? 1 : 0;
+            }
+          }
+          if constexpr (!PLAIN) asm volatile("" : "+v"(cnt[mi]));  // keep the count from sinking
+          *(sfenc::u32x4*)(reg + rl * 256 + (((cl >> 3) ^ (rl & 15)) << 4)) =
+              sfenc::u32x4{pack2<ODT>(o[0], o[1]), pack2<ODT>(o[2], o[3]), pack2<ODT>(o[4], o[5]), pack2<ODT>(o[6], o[7])};
+        }
+        __builtin_amdgcn_sched_barrier(0);  // (bounds what the compiler holds in registers at once)
+      }
+    }
+    if constexpr (!PLAIN) {
+      if (a.row_nnz) {
+#pragma unroll
+        for (int mi = 0; mi < 2; ++mi) {
+          const int c = cnt[mi] + __shfl_xor(cnt[mi], 32), r = (pass * 2 + mi) * 32 + lane;
+          if (lane < 32 && c > 0 && (!RAGGED || r < rows)) atomicAdd(a.row_nnz + m0 + r, c);
+        }
+      }
+    }
+    __builtin_amdgcn_wave_barrier();  // the staged rows are this wave's own (in-order LDS)
+#pragma unroll
+    for (int part = 0; part < 2; ++part) {
+      sfenc::u32x4 v[8];
+#pragma unroll
+      for (int it = 0; it < 8; ++it) {
+        const int rl = (part * 8 + it) * 4 + lane / 16;
+        v[it] = *(const sfenc::u32x4*)(reg + rl * 256 + ((unit ^ (rl & 15)) << 4));
+      }
+#pragma unroll
+      for (int it = 0; it < 8; ++it) {
+        const int rl = pass * 64 + (part * 8 + it) * 4;
+        if (!RAGGED || (rl + lane / 16 < rows && unit * 8 + 8 <= cols)) {
+          __builtin_nontemporal_store(v[it], (u32x4_any*)dst);
+        } else if (rl + lane / 16 < rows) {
+#pragma unroll
+          for (int e = 0; e < 8; ++e)
+            if (unit * 8 + e < cols) ((u16*)dst)[e] = (u16)(v[it][e >> 1] >> ((e & 1) * 16));
+        }
+        dst += 8 * som;
+      }
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    __builtin_amdgcn_wave_barrier();
+  }
+}
+
+// Persistent form for 256x256 tiles of 16-bit results: gemm_persist_kernel's walk of an XCD's tiles, its claims, its alternating stage buffers
+// and its epilogue, four waves of 128x128 (one per SIMD; eight waves of 128x64 would need the registers of
+// both halves' fragments twice), with a K loop of its own:
+//   Y(kt)      16 MFMAs on the first half (64 elements) of block kt, the second half's fragments read
+//              under the first of them. After 12 the wave has read all it needs of kt's buffer and
+//              meets the others: past that barrier block kt + 1 has landed and kt's buffer is free, so the
+//              DMAs of block kt + 2 go into it at once, a whole K-step before they are awaited.
+//   X(kt + 1)  16 MFMAs on the second half of kt, the first half of kt + 1 read under them.
+// The order of MFMAs, LDS reads and DMAs is pinned (a scheduling barrier after each MFMA): left to itself
+// the compiler puts all reads of a half before its first MFMA. An odd number of blocks is rounded
+// up; the one past the end reads zeros.
+template <int ODT, bool PLAIN>
+__global__ __launch_bounds__(256, 1) void gemm_f8_persist_kernel(F8Args a) {
+  using namespace sfenc;
+  constexpr int NW = 4, NB = 4, MB = 4, NMF = NB * MB;
+  constexpr int NST = 32;                 // the epilogue's stores per lane
+  constexpr int PER = 32 / NW;            // DMAs a wave issues per operand and K-step
+  // Y's schedule: two reads after each of the first YD MFMAs and one after the others, the barrier after
+  // MFMA YB, one DMA an MFMA from there on
+  constexpr int YD = 4, YB = 13;
+  __shared__ __attribute__((aligned(1024))) char lds0[STAGE];
+  __shared__ __attribute__((aligned(1024))) char lds1[STAGE];
+  __shared__ __attribute__((aligned(1024))) char s_sc[2][2048];  // dwords of four blocks: features, then tokens
+  __shared__ __attribute__((aligned(16))) float s_bias[2][BN];
+  __shared__ __attribute__((aligned(16))) float s_thr[2][BN];
+  __shared__ int s_claim;
+
+  // The arguments that only a tile's ends need, read again from the kernel's argument block there: held in
+  // scalar registers throughout, they spill into vector registers, and those into memory, whose loads then
+  // wait for the tile's stores.
+  auto cold = [] {
+    const __attribute__((address_space(4))) F8Args* p =
+        (const __attribute__((address_space(4))) F8Args*)__builtin_amdgcn_kernarg_segment_ptr();
+    asm volatile("" : "+s"(p));
+    return p;
+  };
+  // The thread's index, formed anew (and opaquely) where it is used, so that it and what derives from it
+  // take no registers in between.
+  const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  auto thread = [&] {
+    int zero = 0;
+    asm volatile("" : "+s"(zero));
+    return w * 64 + __builtin_amdgcn_mbcnt_hi(~0u, __builtin_amdgcn_mbcnt_lo(~0u, zero));
+  };
+  const int total = a.tiles_m * a.tiles_n;
+  const int b = blockIdx.x;
+  const int per = total / 8, rem = total % 8, xcd = b % 8, loc = b / 8;
+  const int first = xcd * per + min(xcd, rem), last = first + per + (xcd < rem ? 1 : 0);
+  const int step = gridDim.x / 8;  // workgroups per XCD: the fixed first tiles
+  int32_t* const ctr = a.tile_ctr + xcd * TILE_CTR_STRIDE;
+  int lid = first + loc;
+  if (lid >= last) return;  // the whole workgroup
+  const int KB = a.ksteps, KT = (KB + 1) & ~1;
+
+  // A tile. Its DMAs fill LDS rows (i * NW + w) * 8 + lane / 8; rows past M or N are the last valid one again
+  // (rm, rn).
+  struct Tile {
+    int64_t m0, n0;
+    int rm, rn;
+  };
+  auto open_tile = [&](int lid) {
+    const auto c = cold();
+    // runs of group_n feature panels, token panel by token panel (tile_of)
+    const int g = c->group_n, per_group = g * c->tiles_m;
+    const int first = lid / per_group * g, at = lid % per_group, gs = min(c->tiles_n - first, g);
+    Tile T;
+    T.m0 = (int64_t)(at / gs) * BM;
+    T.n0 = (int64_t)(first + at % gs) * BN;
+    T.rm = (int)min((int64_t)BM, c->M - T.m0) - 1;
+    T.rn = (int)min((int64_t)BN, c->N - T.n0) - 1;
+    return T;
+  };
+  // Bias and keep-threshold (as gemm_kernel forms it) of feature t of a tile: raw bits, loaded while the
+  // tile before ends, and their values in LDS, read past the tile's first barrier.
+  struct Raw {
+    uint32_t bias, thr;
+  };
+  auto load_raw = [&](const Tile& T, int t) {
+    const auto c = cold();
+    const int64_t n = T.n0 + min(t, T.rn);
+    Raw r;
+    r.bias = c->b_enc ? load_bits(c->b_enc, c->benc_dt, n) : 0u;
+    r.thr = !PLAIN && c->act == SF_ACT_JUMPRELU ? load_bits(c->thr, c->thr_dt, n) : 0u;
+    return r;
+  };
+  auto put_raw = [&](const Tile& T, const Raw& r, int slot, int t) {
+    const auto c = cold();
+    s_bias[slot][t] = bits_as_f32(r.bias, c->benc_dt);
+    if constexpr (!PLAIN) {
+      constexpr float h = ODT == SF_BF16 ? 0x1p-126f : 0x1p-25f;
+      float tv = c->act == SF_ACT_NONE ? __builtin_nanf("") : h;
+      if (t > T.rn) {
+        tv = __builtin_inff();
+      } else if (c->act == SF_ACT_JUMPRELU) {
+        const float th = bits_as_f32(r.thr, c->thr_dt);
+        tv = th != th ? __builtin_inff() : fmaxf(th, h);
+      }
+      s_thr[slot][t] = tv;
+    }
+  };
+  // A lane's offsets of its DMAs of a K-step, within the tile's rows.
+  struct Offsets {
+    uint32_t x[PER], w[PER];
+  };
+  auto offsets_of = [&](const Tile& T, int t) {
+    Offsets o;
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      const int row = ((t >> 3) & 31) + i * 32;
+      const uint32_t c = (((t & 7) ^ ((t >> 3) & 7) ^ (i & 1) * 4 ^ ((t >> 6) & 3)) & 7) * 16;  // swz(row)
+      o.x[i] = (uint32_t)(min(row, T.rm) & 255) * ((uint32_t)a.Kp & 0xffffffu) + c;
+      o.w[i] = (uint32_t)(min(row, T.rn) & 255) * ((uint32_t)a.swn & 0xffffffu) + c;
+    }
+    return o;
+  };
+  // DMAs [q0, q1) of a K-step's 2 PER, x' and W in turn
+  auto stage = [&](const Tile& T, const Offsets& o, int kt, char* buf, int q0, int q1) {
+    const __amdgpu_buffer_rsrc_t xr = rsrc(a.xw + T.m0 * a.Kp, kt < KB ? T.rm * a.Kp + (int64_t)KB * BLOCK : 0);
+    const __amdgpu_buffer_rsrc_t wr = rsrc(a.w + T.n0 * a.swn, kt < KB ? T.rn * a.swn + (int64_t)KB * BLOCK : 0);
+#pragma unroll
+    for (int q = 0; q < 2 * PER; ++q) {
+      if (q < q0 || q >= q1) continue;
+      const int i = q >> 1;
+      if (q & 1) dma16(wr, buf + (i * NW + w) * 1024, o.w[i], (uint32_t)(kt * BLOCK));
+      else dma16(xr, buf + TILE + (i * NW + w) * 1024, o.x[i], (uint32_t)(kt * BLOCK));
+    }
+  };
+  auto stage_scales = [&](const Tile& T, int g, int w, int t) {
+    dma4(rsrc(a.ws + T.n0 * a.sws, 256 * a.sws), s_sc[g & 1] + w * 256,
+         (uint32_t)(min(t, T.rn) & 255) * ((uint32_t)a.sws & 0xffffffu), (uint32_t)(g * 4));
+    dma4(rsrc(a.xs + T.m0 * a.sxs, 256 * a.sxs), s_sc[g & 1] + 1024 + w * 256,
+         (uint32_t)(min(t, T.rm) & 255) * ((uint32_t)a.sxs & 0xffffffu), (uint32_t)(g * 4));
+  };
+
+  Tile T = open_tile(lid);
+  {
+    const int t0 = thread();
+    const Raw r = load_raw(T, t0);
+    stage(T, offsets_of(T, t0), 0, lds0, 0, 2 * PER);
+    stage_scales(T, 0, w, t0);
+    put_raw(T, r, 0, t0);
+    wait_vmcnt0();
+  }
+
+  auto tile = [&](auto par_tag) -> bool {
+    constexpr int P = decltype(par_tag)::value;
+    char* const B0 = P ? lds1 : lds0;
+    char* const B1 = P ? lds0 : lds1;
+    int t = thread(), lane = t & 63;
+    const int wm = w >> 1, wn = w & 1;
+    // past this barrier block 0 and its scales have landed, and B1 is no longer staging space
+    wait_lgkmcnt0();
+    barrier_no_fence();
+    const Offsets off = offsets_of(T, t);
+    stage(T, off, 1, B1, 0, 2 * PER);
+    // The accumulators start at b_enc: one bf16 MFMA each, of the bias in three exact pieces with ones (a
+    // quarter of the time that writing 256 registers takes).
+    f32x16 acc[NB][MB];
+    {
+      uint32_t one2 = 0x3f803f80u, one1 = 0x3f80u, none = 0;  // (opaque: not kept across tiles)
+      asm volatile("" : "+v"(one2), "+v"(one1), "+v"(none));
+      const bf16x8 ones = __builtin_bit_cast(bf16x8, sfenc::u32x4{one2, one1, none, none});
+#pragma unroll
+      for (int nb = 0; nb < NB; ++nb) {
+        const sfenc::u32x2 p = pieces(lane < 32 ? s_bias[P][wn * 128 + nb * 32 + frag_feature(lane)] : 0.f);
+        const bf16x8 pb = __builtin_bit_cast(bf16x8, sfenc::u32x4{p[0], p[1], none, none});
+#pragma unroll
+        for (int mb = 0; mb < MB; ++mb) {
+          acc[nb][mb] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(pb, ones, f32x16{}, 0, 0, 0);
+          asm volatile("" : "+a"(acc[nb][mb]));  // (four MFMAs, not one and copies)
+        }
+      }
+    }
+    int claim = 0;
+    if (t == 0) claim = atomicAdd(ctr, 1);
+    if (t == 0) s_claim = claim;  // visible past the next barrier
+
+    struct Frag {
+      sfenc::u32x4 lo[8], hi[8];  // x' fragments 0 to 3, W fragments 4 to 7
+    };
+    // Where a lane reads: chunk 4 s + 2 j + lane / 32 of row r of block q of the wave's rows (r: lane % 32
+    // of x', frag_feature of it of W). swz of row 32 q + r is swz(r), with bit 2 flipped where q is odd, so s and q only decide bit 6 of the
+    // offset: four offsets per operand, which the compiler is kept from working out anew per read.
+    int at_x[2][2], at_w[2][2];
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      const int rx = lane & 31, rw = frag_feature(rx), c = 2 * j + (lane >> 5);
+#pragma unroll
+      for (int p = 0; p < 2; ++p) {
+        at_x[j][p] = TILE + (wm * 128 + rx) * ROWB + (((c ^ swz(rx)) << 4) ^ (p * 64));
+        at_w[j][p] = (wn * 128 + rw) * ROWB + (((c ^ swz(rw)) << 4) ^ (p * 64));
+        asm volatile("" : "+v"(at_x[j][p]), "+v"(at_w[j][p]));
+      }
+    }
+    // LDS read i of a half's 16, in the order in which the MFMAs want them
+    auto read = [&](Frag& f, const char* cur, int s, int i) {
+      constexpr int order[8] = {0, 4, 1, 2, 3, 5, 6, 7};
+      const int q = order[i >> 1], p = (s ^ q) & 1;
+      const char* at = cur + (q < 4 ? at_x : at_w)[i & 1][p] + (q & 3) * 32 * ROWB;
+      if (i & 1) f.hi[q] = *(const sfenc::u32x4*)at;
+      else f.lo[q] = *(const sfenc::u32x4*)at;
+    };
+    int sc[8], scn[8];  // scale bytes of the block in use and of the next
+    auto read_scales = [&](int (&v)[8], int kt) {
+      const char* sb = s_sc[(kt >> 2) & 1] + (kt & 3);
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        v[q] = *(const uint8_t*)(sb + (256 + wm * 128 + q * 32 + (lane & 31)) * 4);
+        v[4 + q] = *(const uint8_t*)(sb + (wn * 128 + q * 32 + frag_feature(lane & 31)) * 4);
+      }
+    };
+    auto mma = [&](const Frag& f, int i) {
+      const int nb = i >> 2, mb = i & 3;
+      mfma_f8(acc[nb][mb], join(f.lo[4 + nb], f.hi[4 + nb]), join(f.lo[mb], f.hi[mb]), sc[4 + nb], sc[mb]);
+      asm volatile("" : "+a"(acc[nb][mb]));  // keeps the MFMA in its place among the memory operations
+    };
+    Frag F0, F1;
+    // DMA: block kt + 2 goes into cur
+    auto phase_y = [&](auto dma_tag, char* cur, int kt) {
+      constexpr bool DMA = decltype(dma_tag)::value;
+#pragma unroll
+      for (int i = 0; i < NMF; ++i) {
+        mma(F0, i);
+        if (i < YD) {
+          read(F1, cur, 1, 2 * i);
+          read(F1, cur, 1, 2 * i + 1);
+        } else if (i < 16 - YD) {
+          read(F1, cur, 1, YD + i);
+        }
+        if (i == YB) {
+          wait_vm_lgkm0<0>();
+          barrier_no_fence();
+          read_scales(scn, kt + 1);
+        }
+        if (DMA && i > YB) stage(T, off, kt + 2, cur, i - YB - 1, i - YB);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+    };
+    auto phase_x = [&](auto dma_tag, const char* nxt, char* cur, int kt) {  // kt: the block just left (cur)
+      constexpr bool DMA = decltype(dma_tag)::value;
+#pragma unroll
+      for (int i = 0; i < NMF; ++i) {
+        mma(F1, i);
+        read(F0, nxt, 0, i);
+        if (DMA) stage(T, off, kt + 2, cur, 15 - YB + i, 16 - YB + i);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+      if (DMA && ((kt + 2) & 3) == 0) stage_scales(T, (kt + 2) >> 2, w, thread());
+#pragma unroll
+      for (int q = 0; q < 8; ++q) sc[q] = scn[q];
+    };
+    read_scales(sc, 0);
+#pragma unroll
+    for (int i = 0; i < 16; ++i) read(F0, B0, 0, i);
+    using Yes = std::true_type;
+    using No = std::false_type;
+    int end = KT;
+    asm volatile("" : "+s"(end));  // (opaque: whether there is a loop is not remembered across tiles)
+    for (int kt = 0; kt + 2 < end; kt += 2) {
+      phase_y(Yes{}, B0, kt);
+      phase_x(Yes{}, B1, B0, kt);
+      phase_y(Yes{}, B1, kt + 1);
+      phase_x(Yes{}, B0, B1, kt + 1);
+    }
+    phase_y(No{}, B0, KT - 2);
+    // (behind a barrier of this tile, even where it has two K-steps only: s_claim is this tile's)
+    const int nlid = first + step + s_claim;  // claims past the range fail: the loop ends
+    const bool more = nlid < last;
+    const Tile U = open_tile(more ? nlid : lid);
+    const Raw raw = load_raw(U, thread());
+    phase_x(No{}, B1, B0, KT - 2);
+    phase_y(No{}, B1, KT - 1);
+    // both buffers are free past the last barrier: the next tile's block 0 goes to B1 (its B0), the
+    // epilogue stages through B0
+    t = thread();
+    lane = t & 63;
+    put_raw(U, raw, 1 - P, t);
+    const int64_t mw = T.m0 + wm * 128, nw = T.n0 + wn * 128;
+    if (more) {
+      stage(U, offsets_of(U, t), 0, B1, 0, 2 * PER);
+      stage_scales(U, 0, w, t);
+    }
+    T = U;
+#pragma unroll
+    for (int i = 0; i < NMF; ++i) mma(F1, i);
+    const Out out = {(char*)cold()->out, cold()->som, cold()->row_nnz, cold()->M, cold()->N, cold()->act};
+    if (mw + 128 <= out.M && nw + 128 <= out.N) {
+      f8_epilogue<ODT, PLAIN, false>(out, acc, mw, nw, lane, s_thr[P] + wn * 128, B0 + w * 16384);
+      // vector-memory operations retire in issue order: at most the epilogue's NST stores outstanding
+      // means that the next tile's DMAs have landed
+      __builtin_amdgcn_s_waitcnt(0x0F70 | (NST & 15) | (((NST >> 4) & 3) << 14));
+    } else {
+      f8_epilogue<ODT, PLAIN, true>(out, acc, mw, nw, lane, s_thr[P] + wn * 128, B0 + w * 16384);
+      wait_vmcnt0();
+    }
+    return more;
+  };
+  for (;;) {
+    if (!tile(std::integral_constant<int, 0>{})) break;
+    if (!tile(std::integral_constant<int, 1>{})) break;
+  }
+}
+
+// The persistent kernels' tile counters, before each launch.
+__global__ void clear_counters_kernel(int32_t* ctr) {
+  if (threadIdx.x < 8) ctr[threadIdx.x * sfenc::TILE_CTR_STRIDE] = 0;
+}
+
 }  // namespace sff8

@@ -24,6 +24,29 @@ hipError_t launch_tile(F8Args& a, hipStream_t s) {
   return hipGetLastError();
 }
 
+// 256x256 tiles of 16-bit results: the persistent form, one workgroup per CU (at most one per
+// tile, whole XCD groups of eight). ctr: TILE_CTR_BYTES of the caller's workspace.
+hipError_t launch_persist(F8Args& a, void* ctr, hipStream_t s) {
+  a.tiles_m = (int)((a.M + BM - 1) / BM);
+  a.tiles_n = (int)((a.N + BN - 1) / BN);
+  a.group_n = std::min(a.group_n, a.tiles_n);
+  a.tile_ctr = (int32_t*)ctr;
+  const int cus = device_cus();
+  if (cus <= 0) return hipErrorInvalidDevice;
+  const int total = a.tiles_m * a.tiles_n;
+  const dim3 grid((unsigned)std::max(8, std::min(cus / 8 * 8, (total + 7) / 8 * 8))), block(256);
+  hipLaunchKernelGGL(clear_counters_kernel, dim3(1), dim3(64), 0, s, a.tile_ctr);
+  const bool plain = a.act != SF_ACT_JUMPRELU && !a.row_nnz;
+  if (a.out_dt == SF_F16) {
+    if (plain) hipLaunchKernelGGL((gemm_f8_persist_kernel<SF_F16, true>), grid, block, 0, s, a);
+    else hipLaunchKernelGGL((gemm_f8_persist_kernel<SF_F16, false>), grid, block, 0, s, a);
+  } else {
+    if (plain) hipLaunchKernelGGL((gemm_f8_persist_kernel<SF_BF16, true>), grid, block, 0, s, a);
+    else hipLaunchKernelGGL((gemm_f8_persist_kernel<SF_BF16, false>), grid, block, 0, s, a);
+  }
+  return hipGetLastError();
+}
+
 bool aligned(const void* p, uintptr_t n) { return ((uintptr_t)p & (n - 1)) == 0; }
 
 int check_rows(const char* fn, const char* what, const void* q, int64_t sq, const void* scale, int64_t ss, int64_t K) {
@@ -32,7 +55,7 @@ int check_rows(const char* fn, const char* what, const void* q, int64_t sq, cons
   SF_REQUIRE(aligned(scale, 4) && ss % 4 == 0, "%s: %s: rows of scales must be 4-B aligned", fn, what);
   SF_REQUIRE(sq >= code_bytes(K) && sq <= (1 << 22), "%s: %s: rows of codes %lld bytes apart, %lld to 4194304 wanted",
              fn, what, (long long)sq, (long long)code_bytes(K));
-  SF_REQUIRE(ss >= scale_bytes(K), "%s: %s: rows of scales %lld bytes apart, at least %lld wanted", fn, what,
+  SF_REQUIRE(ss >= scale_bytes(K) && ss <= (1 << 22), "%s: %s: rows of scales %lld bytes apart, %lld to 4194304 wanted", fn, what,
              (long long)ss, (long long)scale_bytes(K));
   return SF_OK;
 }
@@ -54,7 +77,7 @@ int check_call(const char* fn, const void* b_enc, int benc_dt, const void* thr, 
 
 int product(const char* fn, const void* xq, int64_t sxq, const void* xs, int64_t sxs, const void* wq, int64_t swq,
             const void* ws, int64_t sws, const void* b_enc, int benc_dt, const void* thr, int thr_dt, void* out,
-            int64_t som, int out_dt, int32_t* row_nnz, int64_t M, int64_t N, int64_t K, int act, hipStream_t s) {
+            int64_t som, int out_dt, int32_t* row_nnz, int64_t M, int64_t N, int64_t K, int act, void* ctr, hipStream_t s) {
   F8Args a = {};
   a.xw = (const char*)xq; a.Kp = sxq; a.xs = (const uint8_t*)xs; a.sxs = sxs;
   a.w = (const char*)wq; a.swn = swq; a.swk = 1; a.ws = (const uint8_t*)ws; a.sws = sws;
@@ -70,6 +93,7 @@ int product(const char* fn, const void* xq, int64_t sxq, const void* xs, int64_t
   SF_REQUIRE(tiles < (1ll << 22), "%s: too many tiles", fn);
   hipError_t e;
   if (M <= 32) e = launch_tile<F8x32, AUX_NT>(a, s);
+  else if (tiles >= 256 && out_dt != SF_F32) e = launch_persist(a, ctr, s);
   else if (tiles < 512) e = launch_tile<F8x128, 0>(a, s);
   else e = launch_tile<F8x256, 0>(a, s);
   if (e != hipSuccess) return sf_fail(SF_EHIP, "%s: kernel launch failed: %s", fn, hipGetErrorString(e));
@@ -82,16 +106,18 @@ int product(const char* fn, const void* xq, int64_t sxq, const void* xs, int64_t
 extern "C" int sf_encode_fp8_rows(const void* xq, int64_t sxq, const void* xs, int64_t sxs, const void* wq, int64_t swq,
                                   const void* ws, int64_t sws, const void* b_enc, int benc_dt, const void* thr,
                                   int thr_dt, void* out, int64_t som, int out_dt, int32_t* row_nnz, int64_t M, int64_t N,
-                                  int64_t K, int act, void* stream) {
+                                  int64_t K, int act, void* workspace, int64_t workspace_bytes, void* stream) {
   using namespace sff8;
   static const char* fn = "sf_encode_fp8_rows";
   sf_clear_error();
   if (const int rc = check_call(fn, b_enc, benc_dt, thr, thr_dt, out, som, out_dt, M, N, K, act)) return rc;
   if (M == 0 || N == 0) return SF_OK;
+  SF_REQUIRE(workspace && aligned(workspace, 16) && workspace_bytes >= TILE_CTR_BYTES,
+             "%s: needs a 16-B aligned workspace of %lld bytes", fn, (long long)TILE_CTR_BYTES);
   if (const int rc = check_rows(fn, "x", xq, sxq, xs, sxs, K)) return rc;
   if (const int rc = check_rows(fn, "w", wq, swq, ws, sws, K)) return rc;
   return product(fn, xq, sxq, xs, sxs, wq, swq, ws, sws, b_enc, benc_dt, thr, thr_dt, out, som, out_dt, row_nnz, M, N, K,
-                 act, (hipStream_t)stream);
+                 act, workspace, (hipStream_t)stream);
 }
 
 extern "C" int sf_encode_fp8_workspace_size(int64_t M, int64_t K, int64_t* bytes) {
@@ -100,7 +126,7 @@ extern "C" int sf_encode_fp8_workspace_size(int64_t M, int64_t K, int64_t* bytes
   SF_REQUIRE(bytes, "sf_encode_fp8_workspace_size: bytes must not be NULL");
   SF_REQUIRE(M >= 0 && M <= INT32_MAX && K >= 1 && K <= (1 << 22), "sf_encode_fp8_workspace_size: bad size (M=%lld K=%lld)",
              (long long)M, (long long)K);
-  *bytes = M * (code_bytes(K) + scale_bytes(K));
+  *bytes = (M * (code_bytes(K) + scale_bytes(K)) + 63) / 64 * 64 + TILE_CTR_BYTES;
   return SF_OK;
 }
 
@@ -117,13 +143,14 @@ extern "C" int sf_encode_fp8(const void* x, int64_t sxm, int64_t sxk, int x_dt, 
   if (M == 0 || N == 0) return SF_OK;
   SF_REQUIRE(x, "%s: x must not be NULL", fn);
   const int64_t sq = code_bytes(K), ss = scale_bytes(K);
-  SF_REQUIRE(workspace && aligned(workspace, 16) && workspace_bytes >= M * (sq + ss),
-             "%s: needs a 16-B aligned workspace of %lld bytes", fn, (long long)(M * (sq + ss)));
+  const int64_t ctr = (M * (sq + ss) + 63) / 64 * 64;
+  SF_REQUIRE(workspace && aligned(workspace, 16) && workspace_bytes >= ctr + TILE_CTR_BYTES,
+             "%s: needs a 16-B aligned workspace of %lld bytes", fn, (long long)(ctr + TILE_CTR_BYTES));
   if (const int rc = check_rows(fn, "w", wq, swq, ws, sws, K)) return rc;
   char* xs = (char*)workspace + M * sq;
   if (const int rc = launch_quantize(x, sxm, sxk, x_dt, b_dec, bdec_dt, M, K, workspace, sq, xs, ss, 0, M,
                                      (hipStream_t)stream))
     return rc;
   return product(fn, workspace, sq, xs, ss, wq, swq, ws, sws, b_enc, benc_dt, thr, thr_dt, out, som, out_dt, row_nnz, M,
-                 N, K, act, (hipStream_t)stream);
+                 N, K, act, (char*)workspace + ctr, (hipStream_t)stream);
 }

@@ -191,12 +191,12 @@ def fused_encode_fp8(x, W, b_enc=None, threshold=None, activation="relu", *, b_d
             0 if threshold is None else _lib.dtype_code(threshold, "threshold"), out.data_ptr(), N, code,
             _lib.ptr(row_nnz), M, N, d, ACTIVATIONS[activation])
     with _lib.device(dev):
+        ws = torch.empty(_lib.fp8_workspace_bytes(0 if held else M, d), dtype=torch.uint8, device=dev)
         if held:
             _lib.check(lib.sf_encode_fp8_rows(x.q.data_ptr(), x.q.stride(0), x.scale.data_ptr(), x.scale.stride(0),
-                                              *tail, _lib.stream(dev)))
+                                              *tail, ws.data_ptr(), ws.numel(), _lib.stream(dev)))
         else:
             x_code = _lib.dtype_code(x, "x")
-            ws = torch.empty(_lib.fp8_workspace_bytes(M, d), dtype=torch.uint8, device=dev)
             _lib.check(lib.sf_encode_fp8(x.data_ptr(), x.stride(0), x.stride(1), x_code, _lib.ptr(b_dec),
                                          0 if b_dec is None else _lib.dtype_code(b_dec, "b_dec"), *tail, ws.data_ptr(),
                                          ws.numel(), _lib.stream(dev)))
