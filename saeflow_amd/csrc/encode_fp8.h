@@ -29,6 +29,12 @@ struct F8Args : sfenc::GemmArgs {
   int64_t sxs;
   const uint8_t* ws;
   int64_t sws;
+  // The fused form's tokens: x [M, K] of x_dt minus shift, quantised by each workgroup for itself.
+  const void* x;
+  int64_t sxm, sxk;
+  int x_dt, x_rows;  // x_rows: rows contiguous and 16-B aligned
+  const void* shift;
+  int shift_dt, shift_vec;
 };
 
 constexpr int SG = 8;              // groups of four blocks whose scales LDS holds at a time
@@ -54,22 +60,120 @@ __device__ __forceinline__ i32x8 join(const sfenc::u32x4& lo, const sfenc::u32x4
   return __builtin_bit_cast(i32x8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
 }
 
+// Feature (within a block of 32) that row i of a W fragment holds. Lane half h of an MFMA result has the
+// rows 8 g + 4 h + r; with this order they are the consecutive features 16 h + 4 g + r, 32 B of a row.
+__device__ __forceinline__ int frag_feature(int i) { return (i & 4) * 4 + (i >> 3) * 4 + (i & 3); }
+
+// 16 B of a result row, at any element's address
+typedef sfenc::u32x4 u32x4_any __attribute__((aligned(2)));
+
+// What an epilogue writes to.
+struct Out {
+  char* out;
+  int64_t som;
+  int32_t* row_nnz;
+  int64_t M, N;
+  int act;
+};
+// Epilogue of a wave's (32 MB x 32 NB) tile at token m0, feature n0, 32 tokens at a time through `reg` (32
+// rows of 32 NB features, this wave's own), fragment rows in frag_feature order: 16-B stores at any
+// alignment, element by element only across the last feature. ES: bytes of a result.
+template <int ES, int MB, int NB, bool PLAIN>
+__device__ __forceinline__ void tile_epilogue(const Out& a, int out_dt, f32x16 (&acc)[NB][MB], int64_t m0, int64_t n0,
+                                              int lane, const float* s_t, char* reg) {
+  using namespace sfenc;
+  constexpr int RB = NB * 32 * ES, UPR = RB / 16, RPI = 64 / UPR, EPU = 16 / ES;
+  float lo = a.act == SF_ACT_NONE ? -__builtin_inff() : 0.f;
+  asm volatile("" : "+v"(lo));
+  const int h = lane >> 5, rl = lane & 31, unit = lane % UPR;
+  const int rows = (int)max((int64_t)0, min((int64_t)32 * MB, a.M - m0));
+  const int cols = (int)max((int64_t)0, min((int64_t)32 * NB, a.N - n0));
+  char* dst = a.out + ((m0 + lane / UPR) * a.som + n0 + unit * EPU) * ES;
+  const int64_t step = (int64_t)RPI * a.som * ES;
+#pragma unroll
+  for (int mb = 0; mb < MB; ++mb) {
+    int cnt = 0;
+#pragma unroll
+    for (int nb = 0; nb < NB; ++nb) {
+#pragma unroll
+      for (int g = 0; g < 16 / EPU; ++g) {
+        const int cl = nb * 32 + h * 16 + g * EPU;
+        float o[EPU];
+#pragma unroll
+        for (int e = 0; e < EPU; ++e) {
+          const float pre = acc[nb][mb][g * EPU + e];
+          if constexpr (PLAIN) {
+            o[e] = __builtin_elementwise_maximum(pre, lo);
+          } else {
+            const bool keep = !(pre <= s_t[cl + e]);
+            o[e] = keep ? pre : 0.f;
+            cnt += keep && cl + e < cols ? 1 : 0;
+          }
+        }
+        sfenc::u32x4 v;
+        if constexpr (ES == 4)
+          v = sfenc::u32x4{__float_as_uint(o[0]), __float_as_uint(o[1]), __float_as_uint(o[2]), __float_as_uint(o[3])};
+        else if (out_dt == SF_F16)
+          v = sfenc::u32x4{pack2<SF_F16>(o[0], o[1]), pack2<SF_F16>(o[2], o[3]), pack2<SF_F16>(o[4], o[5]), pack2<SF_F16>(o[6], o[7])};
+        else
+          v = sfenc::u32x4{pack2<SF_BF16>(o[0], o[1]), pack2<SF_BF16>(o[2], o[3]), pack2<SF_BF16>(o[4], o[5]), pack2<SF_BF16>(o[6], o[7])};
+        *(sfenc::u32x4*)(reg + rl * RB + (((cl / EPU) ^ (rl & (UPR - 1))) << 4)) = v;
+      }
+    }
+    if constexpr (!PLAIN) {
+      if (a.row_nnz) {
+        const int c = cnt + __shfl_xor(cnt, 32);
+        if (lane < 32 && mb * 32 + lane < rows && c > 0) atomicAdd(a.row_nnz + m0 + mb * 32 + lane, c);
+      }
+    }
+    __builtin_amdgcn_wave_barrier();  // the staged rows are this wave's own (in-order LDS)
+#pragma unroll
+    for (int it = 0; it < 32 / RPI; ++it) {
+      const int row = it * RPI + lane / UPR;
+      const sfenc::u32x4 v = *(const sfenc::u32x4*)(reg + row * RB + ((unit ^ (row & (UPR - 1))) << 4));
+      if (mb * 32 + row < rows) {
+        if (unit * EPU + EPU <= cols) {
+          *(u32x4_any*)dst = v;
+        } else {
+#pragma unroll
+          for (int e = 0; e < EPU; ++e)
+            if (unit * EPU + e < cols) {
+              if constexpr (ES == 4) ((uint32_t*)dst)[e] = v[e];
+              else ((u16*)dst)[e] = (u16)(v[e >> 1] >> ((e & 1) * 16));
+            }
+        }
+      }
+      dst += step;
+    }
+    __builtin_amdgcn_wave_barrier();
+  }
+}
+
 // One workgroup per tile of TL (encode_slim.h: 128-B K-steps), NS stage buffers, NS - 1 in flight; the
-// pipeline, its waits and the epilogues are gemm_slim_kernel's. The scale bytes of the tile's rows
-// lie in LDS as [group of four blocks][row] dwords, loaded for 4096 elements of K at a time.
-template <typename TL, int EPI, int AUX, bool WIDE>
+// pipeline and its waits are gemm_slim_kernel's. The scale bytes of the tile's rows lie in LDS as [group of
+// four blocks][row] dwords, loaded for 4096 elements of K at a time.
+//
+// FUSED (tokens of at most FUSED_BLOCKS blocks in all): the tokens come as they are; each workgroup, its
+// first stages of W under way, quantises all of them into LDS, where they stay. That costs a workgroup
+// about 2 us of latency and saves a launch.
+constexpr int FUSED_BLOCKS = 32;
+template <typename TL, bool WIDE, bool PLAIN, bool FUSED>
 __global__ __launch_bounds__(TL::NT, TL::ST * TL::NS > 81920 ? (TL::NW + 3) / 4 : (TL::NW + 1) / 2) void gemm_f8_kernel(F8Args a) {
   using namespace sfenc;
   constexpr int MB = TL::MB, NB = TL::NB, KC = TL::KC, NS = TL::NS, NW = TL::NW, TN = TL::TN, TM = TL::TM, NT = TL::NT;
-  constexpr int PW = TL::PW, PX = TL::PX, ROWS = TM + TN;
+  constexpr int PW = TL::PW, PX = FUSED ? 0 : TL::PX, ROWS = FUSED ? TN : TM + TN;
+  constexpr int ST = FUSED ? TL::WT : TL::ST;
+  static_assert(!FUSED || (TM == 32 && TL::WM == 1), "one block of tokens");
   static_assert(KC == 8 && NS >= 2 && NS <= 6 && NS != 5, "128-B rows");
-  __shared__ __attribute__((aligned(1024))) char s0[TL::ST];
-  __shared__ __attribute__((aligned(1024))) char s1[TL::ST];
-  __shared__ __attribute__((aligned(1024))) char s2[NS > 2 ? TL::ST : 16];
-  __shared__ __attribute__((aligned(1024))) char s3[NS > 3 ? TL::ST : 16];
-  __shared__ __attribute__((aligned(1024))) char s4[NS > 4 ? TL::ST : 16];
-  __shared__ __attribute__((aligned(1024))) char s5[NS > 5 ? TL::ST : 16];
+  __shared__ __attribute__((aligned(1024))) char s0[ST];
+  __shared__ __attribute__((aligned(1024))) char s1[ST];
+  __shared__ __attribute__((aligned(1024))) char s2[NS > 2 ? ST : 16];
+  __shared__ __attribute__((aligned(1024))) char s3[NS > 3 ? ST : 16];
+  __shared__ __attribute__((aligned(1024))) char s4[NS > 4 ? ST : 16];
+  __shared__ __attribute__((aligned(1024))) char s5[NS > 5 ? ST : 16];
   __shared__ __attribute__((aligned(16))) uint32_t s_sc[SG * ROWS];  // features first, then tokens
+  __shared__ __attribute__((aligned(16))) char s_x[FUSED ? FUSED_BLOCKS * BLOCK : 16];  // codes [token][block]
+  __shared__ __attribute__((aligned(16))) uint8_t s_xsc[FUSED ? FUSED_BLOCKS : 16];  // their scales
   __shared__ __attribute__((aligned(16))) float s_benc[TN];
   __shared__ __attribute__((aligned(16))) float s_thr[TN];
 
@@ -82,7 +186,7 @@ __global__ __launch_bounds__(TL::NT, TL::ST * TL::NS > 81920 ? (TL::NW + 3) / 4 
   const int KT = a.ksteps, KB = KT * BLOCK;
   const int groups = (KT + 3) >> 2;
 
-  uint32_t xo[PX], wo[PW];
+  uint32_t xo[FUSED ? 1 : PX], wo[PW];
 #pragma unroll
   for (int i = 0; i < PX; ++i) {
     const int P = (i * NW + w) * 64 + lane, m = P / KC;
@@ -102,7 +206,7 @@ __global__ __launch_bounds__(TL::NT, TL::ST * TL::NS > 81920 ? (TL::NW + 3) / 4 
 #pragma unroll
     for (int i = 0; i < PX; ++i) dma16(xr, st + TL::WT + (i * NW + w) * 1024, xo[i], (uint32_t)(kt * BLOCK));
 #pragma unroll
-    for (int i = 0; i < PW; ++i) dma16_w<AUX>(wr, st + (i * NW + w) * 1024, wo[i], (uint32_t)(kt * BLOCK));
+    for (int i = 0; i < PW; ++i) dma16(wr, st + (i * NW + w) * 1024, wo[i], (uint32_t)(kt * BLOCK));
   };
   // scale dwords of groups [g0, g0 + SG) of the tile's rows (the last valid row's past M and N, whose
   // codes are zeros), into registers and from there into LDS
@@ -150,6 +254,34 @@ __global__ __launch_bounds__(TL::NT, TL::ST * TL::NS > 81920 ? (TL::NW + 3) / 4 
   }
   static_assert(TN <= NT, "a thread's bias");
   put_scales();
+  if constexpr (FUSED) {
+    // sixteen lanes a block, all loads of a thread under way at once
+    auto quantize = [&](auto dt_tag, auto src_tag) {
+      constexpr int DT = decltype(dt_tag)::value, SRC = decltype(src_tag)::value, Q = NT / 16;
+      const int all = (int)a.M * KT;  // at most FUSED_BLOCKS
+      float v[FUSED_BLOCKS / Q][8];
+#pragma unroll
+      for (int i = 0; i < FUSED_BLOCKS / Q; ++i) {
+        const int b = min((t >> 4) + i * Q, all - 1), m = b / KT;
+        load_shifted<DT, SRC>(a.x, a.sxm, a.sxk, a.shift, a.shift_dt, a.shift_vec, a.K, m,
+                              (int64_t)(b - m * KT) * BLOCK + (t & 15) * 8, v[i]);
+      }
+#pragma unroll
+      for (int i = 0; i < FUSED_BLOCKS / Q; ++i) {
+        const int b = min((t >> 4) + i * Q, all - 1);
+        uint32_t byte;
+        *(sff8::u32x2*)(s_x + b * BLOCK + (t & 15) * 8) = quantize8(v[i], byte);
+        if ((t & 15) == 0) s_xsc[b] = (uint8_t)byte;
+      }
+    };
+    auto typed = [&](auto src_tag) {
+      if (a.x_dt == SF_BF16) quantize(std::integral_constant<int, SF_BF16>{}, src_tag);
+      else if (a.x_dt == SF_F16) quantize(std::integral_constant<int, SF_F16>{}, src_tag);
+      else quantize(std::integral_constant<int, SF_F32>{}, src_tag);
+    };
+    if (a.x_rows) typed(std::integral_constant<int, SRC_ROWS>{});
+    else typed(std::integral_constant<int, SRC_ANY>{});
+  }
   wait_lgkmcnt0();
   barrier_no_fence();
   f32x16 acc[NB][MB];
@@ -157,7 +289,7 @@ __global__ __launch_bounds__(TL::NT, TL::ST * TL::NS > 81920 ? (TL::NW + 3) / 4 
   for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
     for (int g = 0; g < 4; ++g) {
-      const float4 be = *(const float4*)(s_benc + (wn * NB + nb) * 32 + g * 8 + (lane >> 5) * 4);
+      const float4 be = *(const float4*)(s_benc + (wn * NB + nb) * 32 + (lane >> 5) * 16 + g * 4);
 #pragma unroll
       for (int mb = 0; mb < MB; ++mb) {
         acc[nb][mb][g * 4 + 0] = be.x;
@@ -176,11 +308,19 @@ __global__ __launch_bounds__(TL::NT, TL::ST * TL::NS > 81920 ? (TL::NW + 3) / 4 
     return join(*(const sfenc::u32x4*)(tile + row * 128 + ((c ^ z) << 4)),
                 *(const sfenc::u32x4*)(tile + row * 128 + (((c + 2) ^ z) << 4)));
   };
-  auto load_frag = [&](Frag& f, const char* st, int s) {
+  auto load_frag = [&](Frag& f, const char* st, int s, int kt) {
 #pragma unroll
-    for (int mb = 0; mb < MB; ++mb) f.b[mb] = row_frag(st + TL::WT, (wm * MB + mb) * 32 + (lane & 31), s);
+    for (int mb = 0; mb < MB; ++mb) {
+      if constexpr (FUSED) {
+        const char* row = s_x + (min(lane & 31, (int)a.M - 1) * KT + kt) * BLOCK;
+        const int c = 4 * s + (lane >> 5);
+        f.b[mb] = join(*(const sfenc::u32x4*)(row + (c << 4)), *(const sfenc::u32x4*)(row + ((c + 2) << 4)));
+      } else {
+        f.b[mb] = row_frag(st + TL::WT, (wm * MB + mb) * 32 + (lane & 31), s);
+      }
+    }
 #pragma unroll
-    for (int nb = 0; nb < NB; ++nb) f.a[nb] = row_frag(st, (wn * NB + nb) * 32 + (lane & 31), s);
+    for (int nb = 0; nb < NB; ++nb) f.a[nb] = row_frag(st, (wn * NB + nb) * 32 + frag_feature(lane & 31), s);
   };
   auto step = [&](int kt, char* cur, char* nxt) {
     wait_vm_lgkm0<(NS - 2) * (PW + PX)>();
@@ -195,14 +335,16 @@ __global__ __launch_bounds__(TL::NT, TL::ST * TL::NS > 81920 ? (TL::NW + 3) / 4 
     const char* sb = (const char*)s_sc + ((kt >> 2) & (SG - 1)) * ROWS * 4 + (kt & 3);
     int sa[NB], sx[MB];
 #pragma unroll
-    for (int nb = 0; nb < NB; ++nb) sa[nb] = *(const uint8_t*)(sb + ((wn * NB + nb) * 32 + (lane & 31)) * 4);
+    for (int nb = 0; nb < NB; ++nb) sa[nb] = *(const uint8_t*)(sb + ((wn * NB + nb) * 32 + frag_feature(lane & 31)) * 4);
 #pragma unroll
-    for (int mb = 0; mb < MB; ++mb) sx[mb] = *(const uint8_t*)(sb + (TN + (wm * MB + mb) * 32 + (lane & 31)) * 4);
+    for (int mb = 0; mb < MB; ++mb)
+      sx[mb] = FUSED ? s_xsc[min(lane & 31, (int)a.M - 1) * KT + kt]
+                     : *(const uint8_t*)(sb + (TN + (wm * MB + mb) * 32 + (lane & 31)) * 4);
     Frag f[2];
-    load_frag(f[0], cur, 0);
+    load_frag(f[0], cur, 0, kt);
 #pragma unroll
     for (int s = 0; s < 2; ++s) {
-      if (s == 0) load_frag(f[1], cur, 1);
+      if (s == 0) load_frag(f[1], cur, 1, kt);
       if constexpr (WIDE) {
 #pragma unroll
         for (int part = 0; part < 4; ++part) {
@@ -248,15 +390,12 @@ __global__ __launch_bounds__(TL::NT, TL::ST * TL::NS > 81920 ? (TL::NW + 3) / 4 
   const int64_t mw = m0 + wm * MB * 32, nw = n0 + wn * NB * 32;
   const float* st = s_thr + wn * NB * 32;
   wait_vmcnt0();  // no DMA (the empty-range ones included) outlives its wave or hits the staging
-  if constexpr (EPI != EPI_DENSE) {
-    slim_rows<MB, NB>(a, acc, mw, nw, lane, st);
-  } else {
-    __syncthreads();
-    constexpr int RG = 32 * NB * 32 * 4, WPS = TL::ST / RG;  // staging bytes per wave, waves per buffer
-    static_assert(NW <= 2 * WPS, "epilogue staging");
-    char* reg = w < WPS ? s0 + w * RG : s1 + (w - WPS) * RG;
-    slim_dense<WIDE ? 4 : 2, MB, NB>(a, acc, mw, nw, lane, st, reg);  // (fp32 results are wide)
-  }
+  __syncthreads();
+  constexpr int ES = WIDE ? 4 : 2;  // (fp32 results are wide)
+  constexpr int RG = 32 * NB * 32 * ES, WPS = ST / RG;  // staging bytes per wave, waves per buffer
+  static_assert(NW <= 2 * WPS, "epilogue staging");
+  char* reg = w < WPS ? s0 + w * RG : s1 + (w - WPS) * RG;
+  tile_epilogue<ES, MB, NB, PLAIN>(Out{(char*)a.out, a.som, a.row_nnz, a.M, a.N, a.act}, a.out_dt, acc, mw, nw, lane, st, reg);
 }
 
 
@@ -264,10 +403,6 @@ __global__ __launch_bounds__(TL::NT, TL::ST * TL::NS > 81920 ? (TL::NW + 3) / 4 
 __device__ __forceinline__ void dma4(__amdgpu_buffer_rsrc_t r, char* wave_base, uint32_t voff, uint32_t soff) {
   __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (lds_void*)wave_base, 4, (int)voff, (int)soff, 0, 0);
 }
-
-// Feature (within a block of 32) that row i of a W fragment holds. Lane half h of an MFMA result has the
-// rows 8 g + 4 h + r; with this order they are the consecutive features 16 h + 4 g + r, 32 B of a row.
-__device__ __forceinline__ int frag_feature(int i) { return (i & 4) * 4 + (i >> 3) * 4 + (i & 3); }
 
 // Three bf16 pieces of a fp32 value, whose sum it is (8 significant bits each; a lone first piece for
 // infinities and NaN), as two dwords.
@@ -279,20 +414,10 @@ __device__ __forceinline__ sfenc::u32x2 pieces(float v) {
   return sfenc::u32x2{f32_to_bf16(v) | (fine ? f32_to_bf16(r) << 16 : 0u), fine ? f32_to_bf16(r - p1) : 0u};
 }
 
-// 16 B of a result row, at any element's address
-typedef sfenc::u32x4 u32x4_any __attribute__((aligned(2)));
-
 // Epilogue of a wave's 128x128 tile of 16-bit results at token m0, feature n0, through 16 KiB of LDS, two
 // passes of 64 tokens; fragment rows in frag_feature order. PLAIN: relu or none and no counts, one
 // instruction an element (gfx950's v_maximum3_f32 keeps a NaN) before the conversion; otherwise as
 // sfenc::epilogue, with the thresholds s_t. RAGGED: the tile reaches past M or N.
-struct Out {
-  char* out;
-  int64_t som;
-  int32_t* row_nnz;
-  int64_t M, N;
-  int act;
-};
 template <int ODT, bool PLAIN, bool RAGGED>
 __device__ __forceinline__ void f8_epilogue(const Out& a, f32x16 (&acc)[4][4], int64_t m0, int64_t n0, int lane,
                                             const float* s_t, char* reg) {

@@ -1,4 +1,6 @@
 // Entry points of the encoder product on 8-bit rows (kernels: encode_fp8.h).
+#include <math.h>
+
 #include "encode_fp8.h"
 
 namespace sff8 {
@@ -6,21 +8,27 @@ namespace {
 
 using namespace sfenc;
 
-// Up to 32 tokens: the pass over W bounds it; two waves of 32 features, five stages in flight.
-typedef SlimTile<1, 1, 1, 2, 8, 6> F8x32;
-// Middling sizes: 128 x 128, three stages.
-typedef SlimTile<2, 2, 2, 2, 8, 3> F8x128;
-// Large: 256 x 256, 8 waves of 128 x 64.
-typedef SlimTile<4, 2, 2, 4, 8, 2> F8x256;
+// The tiles, tokens x features, with the stages that leave room for two workgroups a CU: narrow ones for few
+// tokens, where the pass over W bounds the product, wider ones where the matrix cores do.
+typedef SlimTile<1, 1, 1, 4, 8, 3> F8x32;    // 32 x 128
+typedef SlimTile<2, 1, 1, 4, 8, 3> F8x64;    // 64 x 128
+typedef SlimTile<2, 2, 2, 2, 8, 2> F8x128;   // 128 x 128
+typedef SlimTile<1, 1, 1, 2, 8, 6> F8few;    // 32 x 64, tokens quantised in the kernel
 
-template <typename TL, int AUX>
+template <typename TL, bool FUSED = false>
 hipError_t launch_tile(F8Args& a, hipStream_t s) {
   a.tiles_m = (int)((a.M + TL::TM - 1) / TL::TM);
   a.tiles_n = (int)((a.N + TL::TN - 1) / TL::TN);
   a.group_n = std::min(a.group_n, a.tiles_n);
   const dim3 grid(a.tiles_m * a.tiles_n), block(TL::NT);
-  if (a.out_dt == SF_F32) hipLaunchKernelGGL((gemm_f8_kernel<TL, EPI_DENSE, AUX, true>), grid, block, 0, s, a);
-  else hipLaunchKernelGGL((gemm_f8_kernel<TL, EPI_DENSE, AUX, false>), grid, block, 0, s, a);
+  const bool plain = a.act != SF_ACT_JUMPRELU && !a.row_nnz;
+  if (a.out_dt == SF_F32) {
+    if (plain) hipLaunchKernelGGL((gemm_f8_kernel<TL, true, true, FUSED>), grid, block, 0, s, a);
+    else hipLaunchKernelGGL((gemm_f8_kernel<TL, true, false, FUSED>), grid, block, 0, s, a);
+  } else {
+    if (plain) hipLaunchKernelGGL((gemm_f8_kernel<TL, false, true, FUSED>), grid, block, 0, s, a);
+    else hipLaunchKernelGGL((gemm_f8_kernel<TL, false, false, FUSED>), grid, block, 0, s, a);
+  }
   return hipGetLastError();
 }
 
@@ -75,9 +83,63 @@ int check_call(const char* fn, const void* b_enc, int benc_dt, const void* thr, 
   return SF_OK;
 }
 
-int product(const char* fn, const void* xq, int64_t sxq, const void* xs, int64_t sxs, const void* wq, int64_t swq,
-            const void* ws, int64_t sws, const void* b_enc, int benc_dt, const void* thr, int thr_dt, void* out,
-            int64_t som, int out_dt, int32_t* row_nnz, int64_t M, int64_t N, int64_t K, int act, void* ctr, hipStream_t s) {
+// Tokens are quantised by each workgroup of the product for itself where their blocks are one round of
+// loads for it and there are at most two workgroups a CU: one token of d_in 2304 over 16384 features 11.8 us a
+// call against 13.1 with a quantisation of its own, over 65536 (four a CU) 30 against 27.
+constexpr int64_t FUSED_FEATURES = 32768;
+struct Tokens {
+  const void* x;
+  int64_t sxm, sxk;
+  int x_dt;
+  const void* shift;
+  int shift_dt;
+};
+
+// Estimated time of a product in us with tiles of tm x tn: a fixed part, and for each round of tiles over
+// the CUs a part per block of K (`alone` times that with one workgroup a CU) and one per tile; at least
+// the bytes at the rate that the shape streams them. Fitted to 176 shapes of 1 to 4096 tokens, d_in 256 to
+// 4096, 4096 to 131072 features, in both result sizes: the pick is 0.9% slower than the best of the
+// four in the mean, 14% at most. Where each wins at d_in 2304, d_sae 65536, bf16 (us of the four in order):
+// 32 tokens 26 24 25 33 (d_sae 16384: 10 11 18 27), 128 tokens 58 33 28 36, 256 tokens 108 59 47 40, 4096
+// tokens 1690 880 710 525.
+struct Shape {
+  int tm, tn;
+  float fixed, step, alone, tile, tail, tbs;
+};
+constexpr Shape SHAPES[2][4] = {
+    // 16-bit results
+    {{32, 128, 2.48f, 0.206f, 1.27f, 1.00f, 0.39f, 5.95f}, {64, 128, 2.28f, 0.295f, 1.38f, 1.26f, 0.42f, 6.54f},
+     {128, 128, 1.52f, 0.469f, 1.65f, 1.94f, 0.39f, 6.22f}, {256, 256, 3.10f, 1.346f, 0.76f, 6.38f, 0.27f, 5.11f}},
+    // fp32 results
+    {{32, 128, 2.23f, 0.314f, 1.47f, 1.25f, 0.28f, 6.41f}, {64, 128, 2.04f, 0.496f, 1.27f, 1.74f, 0.25f, 5.53f},
+     {128, 128, 1.87f, 0.830f, 1.18f, 2.34f, 0.37f, 5.08f}, {}}};
+// What result rows off 16 B cost a 256x256 tile (d_sae 10007, d_in 1000, 4096 tokens: 72 us against 52).
+constexpr float UNALIGNED_TILE = 6.f;
+
+int pick_shape(int64_t M, int64_t N, int64_t K, int out_dt, bool unaligned) {
+  const int nb = (int)blocks_of(K), wide = out_dt == SF_F32;
+  const double bytes = (double)N * K + (double)M * K + (double)M * N * sf_dtype_size(out_dt);
+  int best = -1;
+  double least = 0;
+  for (int i = 0; i < (wide ? 3 : 4); ++i) {
+    const Shape& h = SHAPES[wide][i];
+    const double x = (double)((M + h.tm - 1) / h.tm) * (double)((N + h.tn - 1) / h.tn) / 256;
+    const double rounds = x <= 1 ? 1 : (x < 3 ? ceil(x) : x + h.tail);
+    const double tile = h.tile + (i == 3 && unaligned ? UNALIGNED_TILE : 0.f);
+    const double t = std::max(h.fixed + (nb * h.step * (x <= 1 ? h.alone : 1) + tile) * rounds,
+                              h.fixed + tile + bytes / h.tbs * 1e-6);
+    if (best < 0 || t < least) {
+      best = i;
+      least = t;
+    }
+  }
+  return best;
+}
+
+int product(const char* fn, const Tokens* tokens, const void* xq, int64_t sxq, const void* xs, int64_t sxs,
+            const void* wq, int64_t swq, const void* ws, int64_t sws, const void* b_enc, int benc_dt, const void* thr,
+            int thr_dt, void* out, int64_t som, int out_dt, int32_t* row_nnz, int64_t M, int64_t N, int64_t K, int act,
+            void* ctr, hipStream_t s) {
   F8Args a = {};
   a.xw = (const char*)xq; a.Kp = sxq; a.xs = (const uint8_t*)xs; a.sxs = sxs;
   a.w = (const char*)wq; a.swn = swq; a.swk = 1; a.ws = (const uint8_t*)ws; a.sws = sws;
@@ -87,15 +149,24 @@ int product(const char* fn, const void* xq, int64_t sxq, const void* xs, int64_t
   a.group_m = 1;
   a.group_n = 8;
   a.ksteps = (int)blocks_of(K);
-  a.vec_store = som * sf_dtype_size(out_dt) % 16 == 0 && aligned(out, 16);
-  const int64_t tiles = ((M + 255) / 256) * ((N + 255) / 256);
-  SF_REQUIRE(((M + 31) / 32) * ((N + 63) / 64) < (1ll << 24) || M > 32, "%s: too many tiles", fn);
-  SF_REQUIRE(tiles < (1ll << 22), "%s: too many tiles", fn);
   hipError_t e;
-  if (M <= 32) e = launch_tile<F8x32, AUX_NT>(a, s);
-  else if (tiles >= 256 && out_dt != SF_F32) e = launch_persist(a, ctr, s);
-  else if (tiles < 512) e = launch_tile<F8x128, 0>(a, s);
-  else e = launch_tile<F8x256, 0>(a, s);
+  if (tokens) {
+    a.x = tokens->x; a.sxm = tokens->sxm; a.sxk = tokens->sxk; a.x_dt = tokens->x_dt;
+    a.x_rows = a.sxk == 1 && aligned(a.x, 16) && a.sxm * sf_dtype_size(a.x_dt) % 16 == 0;
+    a.shift = tokens->shift; a.shift_dt = tokens->shift_dt;
+    a.shift_vec = a.shift && a.shift_dt == a.x_dt && aligned(a.shift, 16);
+    e = launch_tile<F8few, true>(a, s);
+  } else {
+    const int shape = pick_shape(M, N, K, out_dt, som * sf_dtype_size(out_dt) % 16 != 0 || !aligned(out, 16));
+    const Shape& h = SHAPES[out_dt == SF_F32][shape];
+    SF_REQUIRE(((M + h.tm - 1) / h.tm) * ((N + h.tn - 1) / h.tn) < (1ll << 23), "%s: too many tiles", fn);
+    switch (shape) {
+      case 0: e = launch_tile<F8x32>(a, s); break;
+      case 1: e = launch_tile<F8x64>(a, s); break;
+      case 2: e = launch_tile<F8x128>(a, s); break;
+      default: e = launch_persist(a, ctr, s); break;
+    }
+  }
   if (e != hipSuccess) return sf_fail(SF_EHIP, "%s: kernel launch failed: %s", fn, hipGetErrorString(e));
   return SF_OK;
 }
@@ -116,7 +187,7 @@ extern "C" int sf_encode_fp8_rows(const void* xq, int64_t sxq, const void* xs, i
              "%s: needs a 16-B aligned workspace of %lld bytes", fn, (long long)TILE_CTR_BYTES);
   if (const int rc = check_rows(fn, "x", xq, sxq, xs, sxs, K)) return rc;
   if (const int rc = check_rows(fn, "w", wq, swq, ws, sws, K)) return rc;
-  return product(fn, xq, sxq, xs, sxs, wq, swq, ws, sws, b_enc, benc_dt, thr, thr_dt, out, som, out_dt, row_nnz, M, N, K,
+  return product(fn, nullptr, xq, sxq, xs, sxs, wq, swq, ws, sws, b_enc, benc_dt, thr, thr_dt, out, som, out_dt, row_nnz, M, N, K,
                  act, workspace, (hipStream_t)stream);
 }
 
@@ -147,10 +218,15 @@ extern "C" int sf_encode_fp8(const void* x, int64_t sxm, int64_t sxk, int x_dt, 
   SF_REQUIRE(workspace && aligned(workspace, 16) && workspace_bytes >= ctr + TILE_CTR_BYTES,
              "%s: needs a 16-B aligned workspace of %lld bytes", fn, (long long)(ctr + TILE_CTR_BYTES));
   if (const int rc = check_rows(fn, "w", wq, swq, ws, sws, K)) return rc;
+  if (M * blocks_of(K) <= FUSED_BLOCKS && N <= FUSED_FEATURES) {
+    const Tokens tokens = {x, sxm, sxk, x_dt, b_dec, bdec_dt};
+    return product(fn, &tokens, nullptr, 0, nullptr, 0, wq, swq, ws, sws, b_enc, benc_dt, thr, thr_dt, out, som, out_dt,
+                   row_nnz, M, N, K, act, nullptr, (hipStream_t)stream);
+  }
   char* xs = (char*)workspace + M * sq;
   if (const int rc = launch_quantize(x, sxm, sxk, x_dt, b_dec, bdec_dt, M, K, workspace, sq, xs, ss, 0, M,
                                      (hipStream_t)stream))
     return rc;
-  return product(fn, workspace, sq, xs, ss, wq, swq, ws, sws, b_enc, benc_dt, thr, thr_dt, out, som, out_dt, row_nnz, M,
+  return product(fn, nullptr, workspace, sq, xs, ss, wq, swq, ws, sws, b_enc, benc_dt, thr, thr_dt, out, som, out_dt, row_nnz, M,
                  N, K, act, (char*)workspace + ctr, (hipStream_t)stream);
 }

@@ -85,6 +85,47 @@ __device__ __forceinline__ void load8(const void* p, int64_t i, float (&v)[8]) {
   }
 }
 
+// How the source of a quantisation lies: rows contiguous and 16-B aligned, or anything (element by element).
+enum Src { SRC_ROWS = 0, SRC_ANY = 1 };
+
+// Elements k0 .. k0 + 7 of row m minus the shift, in fp32; zeros past K.
+template <int DT, int SRC>
+__device__ __forceinline__ void load_shifted(const void* x, int64_t sxm, int64_t sxk, const void* shift, int shift_dt,
+                                             int shift_vec, int64_t K, int64_t m, int64_t k0, float (&v)[8]) {
+  if (SRC == SRC_ROWS && k0 + 8 <= K) {
+    load8<DT>(x, m * sxm + k0, v);
+    if (shift_vec) {  // shift of x's type, 16-B aligned
+      float c[8];
+      load8<DT>(shift, k0, c);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[e] -= c[e];
+    } else if (shift) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[e] -= load_as_f32(shift, shift_dt, k0 + e);
+    }
+  } else {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      v[e] = 0.f;
+      if (k0 + e < K) {
+        v[e] = load_as_f32(x, DT, m * sxm + (k0 + e) * sxk);
+        if (shift) v[e] -= load_as_f32(shift, shift_dt, k0 + e);
+      }
+    }
+  }
+}
+// The codes of eight elements of a block that sixteen lanes hold together, and the block's scale byte.
+__device__ __forceinline__ u32x2 quantize8(float (&v)[8], uint32_t& byte) {
+  uint32_t top = 0;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) top = max(top, finite_bits(v[e]));
+  byte = scale_byte(max16(top));
+  const float inv = inverse_of(byte);
+#pragma unroll
+  for (int e = 0; e < 8; ++e) v[e] = scaled(v[e], inv);
+  return u32x2{pack4(v[0], v[1], v[2], v[3]), pack4(v[4], v[5], v[6], v[7])};
+}
+
 // Quantises x [M, K] (any strides) minus shift (or NULL) into rows (row0 + m) % R; the arguments have
 // been checked. Defined in fp8_rows.hip.
 int launch_quantize(const void* x, int64_t sxm, int64_t sxk, int x_dt, const void* shift, int shift_dt, int64_t M,

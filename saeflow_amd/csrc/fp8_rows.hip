@@ -5,9 +5,6 @@
 
 namespace sff8 {
 
-// How the source lies: rows contiguous and 16-B aligned, or anything (element by element).
-enum Src { SRC_ROWS = 0, SRC_ANY = 1 };
-
 // Sixteen lanes take one block of 128, eight elements each: the maximum is four rotations within a
 // DPP row, each lane's eight codes are one 8-B store and the sixteen of a block one cache line.
 // Blocks are numbered row by row over [0, total), total < 2^31, so the row is a 32-bit division.
@@ -21,38 +18,12 @@ __global__ __launch_bounds__(256) void quantize_kernel(const void* x, int64_t sx
     const uint32_t m = b / nb, kb = b - m * nb;
     const int64_t k0 = (int64_t)kb * BLOCK + lane16 * 8;
     float v[8];
-    if (SRC == SRC_ROWS && k0 + 8 <= K) {
-      load8<DT>(x, (int64_t)m * sxm + k0, v);
-      if (shift_vec) {  // shift of x's type, 16-B aligned
-        float c[8];
-        load8<DT>(shift, k0, c);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) v[e] -= c[e];
-      } else if (shift) {
-#pragma unroll
-        for (int e = 0; e < 8; ++e) v[e] -= load_as_f32(shift, shift_dt, k0 + e);
-      }
-    } else {
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        v[e] = 0.f;
-        if (k0 + e < K) {
-          v[e] = load_as_f32(x, DT, (int64_t)m * sxm + (k0 + e) * sxk);
-          if (shift) v[e] -= load_as_f32(shift, shift_dt, k0 + e);
-        }
-      }
-    }
-    uint32_t top = 0;
-#pragma unroll
-    for (int e = 0; e < 8; ++e) top = max(top, finite_bits(v[e]));
-    const uint32_t byte = scale_byte(max16(top));
-    const float inv = inverse_of(byte);
-    float u[8];
-#pragma unroll
-    for (int e = 0; e < 8; ++e) u[e] = scaled(v[e], inv);
+    load_shifted<DT, SRC>(x, sxm, sxk, shift, shift_dt, shift_vec, K, m, k0, v);
+    uint32_t byte;
+    const u32x2 codes = quantize8(v, byte);
     int64_t r = row0 + m;
     if (r >= R) r -= R;
-    *(u32x2*)(q + r * sq + k0) = u32x2{pack4(u[0], u[1], u[2], u[3]), pack4(u[4], u[5], u[6], u[7])};
+    *(u32x2*)(q + r * sq + k0) = codes;
     if (lane16 == 0) scale[r * ss + kb] = (uint8_t)byte;
     if (lane16 > 0 && lane16 <= (uint32_t)pad && kb + 1 == nb) scale[r * ss + kb + lane16] = 0;
   }
