@@ -676,9 +676,7 @@ __global__ __launch_bounds__(256, 1) void gemm_f8_persist_kernel(F8Args a) {
         }
       }
     }
-    int claim = 0;
-    if (t == 0) claim = atomicAdd(ctr, 1);
-    if (t == 0) s_claim = claim;  // visible past the next barrier
+    if (t == 0) s_claim = a.tile_ctr ? atomicAdd(ctr, 1) : 1 << 28;  // visible past the next barrier
 
     struct Frag {
       sfenc::u32x4 lo[8], hi[8];  // x' fragments 0 to 3, W fragments 4 to 7

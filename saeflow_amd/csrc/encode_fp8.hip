@@ -33,17 +33,18 @@ hipError_t launch_tile(F8Args& a, hipStream_t s) {
 }
 
 // 256x256 tiles of 16-bit results: the persistent form, one workgroup per CU (at most one per
-// tile, whole XCD groups of eight). ctr: TILE_CTR_BYTES of the caller's workspace.
-hipError_t launch_persist(F8Args& a, void* ctr, hipStream_t s) {
+// tile, whole XCD groups of eight). ctr: TILE_CTR_BYTES of the caller's workspace, `cleared` already or not.
+hipError_t launch_persist(F8Args& a, void* ctr, bool cleared, hipStream_t s) {
   a.tiles_m = (int)((a.M + BM - 1) / BM);
   a.tiles_n = (int)((a.N + BN - 1) / BN);
   a.group_n = std::min(a.group_n, a.tiles_n);
-  a.tile_ctr = (int32_t*)ctr;
   const int cus = device_cus();
   if (cus <= 0) return hipErrorInvalidDevice;
   const int total = a.tiles_m * a.tiles_n;
   const dim3 grid((unsigned)std::max(8, std::min(cus / 8 * 8, (total + 7) / 8 * 8))), block(256);
-  hipLaunchKernelGGL(clear_counters_kernel, dim3(1), dim3(64), 0, s, a.tile_ctr);
+  // (with a workgroup for every tile nothing is claimed)
+  a.tile_ctr = total > (int)grid.x ? (int32_t*)ctr : nullptr;
+  if (a.tile_ctr && !cleared) hipLaunchKernelGGL(clear_counters_kernel, dim3(1), dim3(64), 0, s, a.tile_ctr);
   const bool plain = a.act != SF_ACT_JUMPRELU && !a.row_nnz;
   if (a.out_dt == SF_F16) {
     if (plain) hipLaunchKernelGGL((gemm_f8_persist_kernel<SF_F16, true>), grid, block, 0, s, a);
@@ -139,7 +140,7 @@ int pick_shape(int64_t M, int64_t N, int64_t K, int out_dt, bool unaligned) {
 int product(const char* fn, const Tokens* tokens, const void* xq, int64_t sxq, const void* xs, int64_t sxs,
             const void* wq, int64_t swq, const void* ws, int64_t sws, const void* b_enc, int benc_dt, const void* thr,
             int thr_dt, void* out, int64_t som, int out_dt, int32_t* row_nnz, int64_t M, int64_t N, int64_t K, int act,
-            void* ctr, hipStream_t s) {
+            void* ctr, bool cleared, hipStream_t s) {
   F8Args a = {};
   a.xw = (const char*)xq; a.Kp = sxq; a.xs = (const uint8_t*)xs; a.sxs = sxs;
   a.w = (const char*)wq; a.swn = swq; a.swk = 1; a.ws = (const uint8_t*)ws; a.sws = sws;
@@ -164,7 +165,7 @@ int product(const char* fn, const Tokens* tokens, const void* xq, int64_t sxq, c
       case 0: e = launch_tile<F8x32>(a, s); break;
       case 1: e = launch_tile<F8x64>(a, s); break;
       case 2: e = launch_tile<F8x128>(a, s); break;
-      default: e = launch_persist(a, ctr, s); break;
+      default: e = launch_persist(a, ctr, cleared, s); break;
     }
   }
   if (e != hipSuccess) return sf_fail(SF_EHIP, "%s: kernel launch failed: %s", fn, hipGetErrorString(e));
@@ -188,7 +189,7 @@ extern "C" int sf_encode_fp8_rows(const void* xq, int64_t sxq, const void* xs, i
   if (const int rc = check_rows(fn, "x", xq, sxq, xs, sxs, K)) return rc;
   if (const int rc = check_rows(fn, "w", wq, swq, ws, sws, K)) return rc;
   return product(fn, nullptr, xq, sxq, xs, sxs, wq, swq, ws, sws, b_enc, benc_dt, thr, thr_dt, out, som, out_dt, row_nnz, M, N, K,
-                 act, workspace, (hipStream_t)stream);
+                 act, workspace, false, (hipStream_t)stream);
 }
 
 extern "C" int sf_encode_fp8_workspace_size(int64_t M, int64_t K, int64_t* bytes) {
@@ -221,12 +222,13 @@ extern "C" int sf_encode_fp8(const void* x, int64_t sxm, int64_t sxk, int x_dt, 
   if (M * blocks_of(K) <= FUSED_BLOCKS && N <= FUSED_FEATURES) {
     const Tokens tokens = {x, sxm, sxk, x_dt, b_dec, bdec_dt};
     return product(fn, &tokens, nullptr, 0, nullptr, 0, wq, swq, ws, sws, b_enc, benc_dt, thr, thr_dt, out, som, out_dt,
-                   row_nnz, M, N, K, act, nullptr, (hipStream_t)stream);
+                   row_nnz, M, N, K, act, nullptr, false, (hipStream_t)stream);
   }
   char* xs = (char*)workspace + M * sq;
+  int32_t* counters = (int32_t*)((char*)workspace + ctr);
   if (const int rc = launch_quantize(x, sxm, sxk, x_dt, b_dec, bdec_dt, M, K, workspace, sq, xs, ss, 0, M,
-                                     (hipStream_t)stream))
+                                     counters, (hipStream_t)stream))
     return rc;
   return product(fn, nullptr, workspace, sq, xs, ss, wq, swq, ws, sws, b_enc, benc_dt, thr, thr_dt, out, som, out_dt, row_nnz, M,
-                 N, K, act, (char*)workspace + ctr, (hipStream_t)stream);
+                 N, K, act, counters, true, (hipStream_t)stream);
 }

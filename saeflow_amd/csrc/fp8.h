@@ -127,8 +127,9 @@ __device__ __forceinline__ u32x2 quantize8(float (&v)[8], uint32_t& byte) {
 }
 
 // Quantises x [M, K] (any strides) minus shift (or NULL) into rows (row0 + m) % R; the arguments have
-// been checked. Defined in fp8_rows.hip.
+// been checked. ctr (or NULL): 8 ints, 16 apart, that are set to zero on the way. Defined in fp8_rows.hip.
 int launch_quantize(const void* x, int64_t sxm, int64_t sxk, int x_dt, const void* shift, int shift_dt, int64_t M,
-                    int64_t K, void* q, int64_t sq, void* scale, int64_t ss, int64_t row0, int64_t R, hipStream_t s);
+                    int64_t K, void* q, int64_t sq, void* scale, int64_t ss, int64_t row0, int64_t R, int32_t* ctr,
+                    hipStream_t s);
 
 }  // namespace sff8

@@ -1,5 +1,6 @@
 // 8-bit rows written and read back (format: fp8.h). Both are one pass over the data, bound by HBM.
 #include <algorithm>
+#include <type_traits>
 
 #include "fp8.h"
 
@@ -7,12 +8,16 @@ namespace sff8 {
 
 // Sixteen lanes take one block of 128, eight elements each: the maximum is four rotations within a
 // DPP row, each lane's eight codes are one 8-B store and the sixteen of a block one cache line.
-// Blocks are numbered row by row over [0, total), total < 2^31, so the row is a 32-bit division.
+// Blocks are numbered row by row over [0, total), total < 2^31, so the row is a 32-bit division. Bound by
+// memory: 16384 rows of 2304 take 28 us in bf16 and 34 us in fp32 where x was just written (4.0 and 5.6 TB/s),
+// 42 and 64 us out of HBM with dirty lines to evict; loads past the caches 30 and 36, 35 and 47; two blocks a
+// lane under way change nothing.
 template <int DT, int SRC>
 __global__ __launch_bounds__(256) void quantize_kernel(const void* x, int64_t sxm, int64_t sxk, const void* shift,
                                                        int shift_dt, int shift_vec, int64_t K, uint32_t nb,
                                                        uint32_t total, uint8_t* q, int64_t sq, uint8_t* scale,
-                                                       int64_t ss, int64_t row0, int64_t R, int pad) {
+                                                       int64_t ss, int64_t row0, int64_t R, int pad, int32_t* ctr) {
+  if (ctr && blockIdx.x == 0 && threadIdx.x < 8) ctr[threadIdx.x * 16] = 0;
   const uint32_t lane16 = threadIdx.x & 15;
   for (uint32_t b = blockIdx.x * 16 + (threadIdx.x >> 4); b < total; b += gridDim.x * 16) {
     const uint32_t m = b / nb, kb = b - m * nb;
@@ -29,37 +34,42 @@ __global__ __launch_bounds__(256) void quantize_kernel(const void* x, int64_t sx
   }
 }
 
-// Columns contiguous (x[m, k] at m + k * sxk, a dictionary's W_enc^T): a workgroup takes 64 rows x one
-// block of 128, read as 128 row pieces of 64 elements (128 B of bf16) into LDS, and every four lanes
-// write one row's 128 codes, a whole cache line. LDS piece k lies at k * 64 E + (k / 32) * 16 E: the
-// four lanes of a row read pieces 32 apart, 16 rows at once, which fills the 64 banks exactly.
+// Columns contiguous (x[m, k] at m + k * sxk, a dictionary's W_enc^T): a workgroup takes CROWS rows x one
+// block of 128, read as 128 pieces of CROWS elements (512 B) into LDS, and every four lanes write one
+// row's 128 codes, a whole cache line. LDS piece k lies at k * CROWS E + (k / 32) * 16 E: the four lanes of
+// a row read pieces 32 apart, 16 rows at once, which fills the 64 banks exactly. Bound by HBM, and by how
+// much of a row of x one workgroup takes: 65536 columns of 2304 bf16 elements 97 us out of HBM (4.7 TB/s)
+// with 512-B pieces, 101 with 256 B, 103 with 128 B.
 template <int DT>
-__global__ __launch_bounds__(256) void quantize_columns_kernel(const void* x, int64_t sxk, int vec, const void* shift,
+constexpr int CROWS = DT == SF_F32 ? 128 : 256;
+template <int DT>
+__global__ __launch_bounds__(4 * CROWS<DT>) void quantize_columns_kernel(const void* x, int64_t sxk, int vec, const void* shift,
                                                                int shift_dt, int64_t M, int64_t K, int64_t nb,
                                                                uint8_t* q, int64_t sq, uint8_t* scale, int64_t ss,
-                                                               int64_t row0, int64_t R, int pad) {
-  constexpr int E = DT == SF_F32 ? 4 : 2, EPC = 16 / E, CPR = 64 / EPC, PER = 128 * CPR / 256;
-  __shared__ __attribute__((aligned(16))) char st[128 * 64 * E + 4 * 16 * E];
+                                                               int64_t row0, int64_t R, int pad, int32_t* ctr) {
+  if (ctr && blockIdx.x == 0 && blockIdx.y == 0 && threadIdx.x < 8) ctr[threadIdx.x * 16] = 0;
+  constexpr int CROWS = sff8::CROWS<DT>, E = DT == SF_F32 ? 4 : 2, EPC = 16 / E, CPR = CROWS / EPC, NT = 4 * CROWS, PER = 128 * CPR / NT;
+  __shared__ __attribute__((aligned(16))) char st[128 * CROWS * E + 4 * 16 * E];
   const int t = threadIdx.x;
-  const int64_t m0 = (int64_t)blockIdx.x * 64, kb = blockIdx.y, k0 = kb * BLOCK;
-  if (vec && m0 + 64 <= M) {
+  const int64_t m0 = (int64_t)blockIdx.x * CROWS, kb = blockIdx.y, k0 = kb * BLOCK;
+  if (vec && m0 + CROWS <= M) {
     u32x4 v[PER];
 #pragma unroll
     for (int i = 0; i < PER; ++i) {
-      const int k = (i * 256 + t) / CPR, c = t % CPR;
+      const int k = (i * NT + t) / CPR, c = t % CPR;
       v[i] = u32x4{0, 0, 0, 0};
-      if (k0 + k < K) v[i] = *(const u32x4*)((const char*)x + ((k0 + k) * sxk + m0) * E + c * 16);
+      if (k0 + k < K) v[i] = __builtin_nontemporal_load((const u32x4*)((const char*)x + ((k0 + k) * sxk + m0) * E + c * 16));
     }
 #pragma unroll
     for (int i = 0; i < PER; ++i) {
-      const int k = (i * 256 + t) / CPR, c = t % CPR;
-      *(u32x4*)(st + k * 64 * E + (k >> 5) * 16 * E + c * 16) = v[i];
+      const int k = (i * NT + t) / CPR, c = t % CPR;
+      *(u32x4*)(st + k * CROWS * E + (k >> 5) * 16 * E + c * 16) = v[i];
     }
   } else {
-    for (int i = t; i < 128 * 64; i += 256) {
-      const int k = i >> 6, m = i & 63;
+    for (int i = t; i < 128 * CROWS; i += NT) {
+      const int k = i / CROWS, m = i % CROWS;
       const uint32_t bits = k0 + k < K && m0 + m < M ? load_bits(x, DT, (k0 + k) * sxk + m0 + m) : 0u;
-      char* dst = st + k * 64 * E + (k >> 5) * 16 * E + m * E;
+      char* dst = st + k * CROWS * E + (k >> 5) * 16 * E + m * E;
       if constexpr (E == 4) *(uint32_t*)dst = bits;
       else *(u16*)dst = (u16)bits;
     }
@@ -71,7 +81,7 @@ __global__ __launch_bounds__(256) void quantize_columns_kernel(const void* x, in
 #pragma unroll
   for (int i = 0; i < 32; ++i) {
     const int k = kq * 32 + i;
-    v[i] = load_as_f32(st + k * 64 * E + kq * 16 * E, DT, m);
+    v[i] = load_as_f32(st + k * CROWS * E + kq * 16 * E, DT, m);
     if (shift && k0 + k < K) v[i] -= load_as_f32(shift, shift_dt, k0 + k);
     top = max(top, finite_bits(v[i]));
   }
@@ -91,33 +101,48 @@ __global__ __launch_bounds__(256) void quantize_columns_kernel(const void* x, in
   if (kq > 0 && kq <= pad && kb + 1 == nb) scale[r * ss + kb + kq] = 0;
 }
 
-// Eight codes a lane, sixteen lanes a block, as quantize_kernel. Row m of the result is row
-// (row0 + m) % R of the store, or rows[m]; an id outside [0, R) gives zeros.
-template <int ODT>
+// Eight codes a lane, sixteen lanes a block, U blocks a lane under way, as quantize_kernel. Row m of the
+// result is row (row0 + m) % R of the store, or rows[m]; an id outside [0, R) gives zeros. Bound by memory:
+// 16384 rows of 2304 to bf16 take 20 us with two blocks a lane under way (5.7 TB/s), 22 with one; to fp32
+// (whose lanes write twice as much) 50 with one, 57 with two. Stores go past the caches: 65536 rows 92 us
+// against 96, 177 against 183 with a pass over the result behind it (16384: 46 against 44).
+template <int ODT, int U>
 __global__ __launch_bounds__(256) void dequantize_kernel(const uint8_t* q, int64_t sq, const uint8_t* scale, int64_t ss,
                                                          int64_t R, const int64_t* rows, int64_t row0,
                                                          const void* shift, int shift_dt, int shift_vec, int64_t K,
                                                          uint32_t nb, uint32_t total, void* out, int64_t som, int vec) {
-  const uint32_t lane16 = threadIdx.x & 15;
-  for (uint32_t b = blockIdx.x * 16 + (threadIdx.x >> 4); b < total; b += gridDim.x * 16) {
-    const uint32_t m = b / nb, kb = b - m * nb;
-    const int64_t k0 = (int64_t)kb * BLOCK + lane16 * 8;
-    if (k0 >= K) continue;
-    int64_t r;
-    if (rows) {
-      r = rows[m];
-    } else {
-      r = row0 + m;
-      if (r >= R) r -= R;
+  const uint32_t lane16 = threadIdx.x & 15, stride = gridDim.x * 16;
+  for (uint32_t b0 = blockIdx.x * 16 + (threadIdx.x >> 4); b0 < total; b0 += U * stride) {
+    u32x2 c[U];
+    uint32_t byte[U], m[U], kb[U];
+    bool in[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const uint32_t b = min(b0 + u * stride, total - 1);
+      m[u] = b / nb;
+      kb[u] = b - m[u] * nb;
+      int64_t r;
+      if (rows) {
+        r = rows[m[u]];
+      } else {
+        r = row0 + m[u];
+        if (r >= R) r -= R;
+      }
+      in[u] = r >= 0 && r < R;
+      if (!in[u]) r = 0;
+      c[u] = *(const u32x2*)(q + r * sq + (int64_t)kb[u] * BLOCK + lane16 * 8);  // (rows are padded to whole blocks)
+      byte[u] = scale[r * ss + kb[u]];
     }
-    float v[8];
-    if (r >= 0 && r < R) {
-      const u32x2 c = *(const u32x2*)(q + r * sq + k0);
-      const float f = scale_of(scale[r * ss + kb]);
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int64_t k0 = (int64_t)kb[u] * BLOCK + lane16 * 8;
+      if (k0 >= K || (U > 1 && b0 + u * stride >= total)) continue;
+      float v[8];
+      const float f = scale_of(byte[u]);
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
-        const f32x2 lo = __builtin_amdgcn_cvt_pk_f32_fp8((int)c[i], false);
-        const f32x2 hi = __builtin_amdgcn_cvt_pk_f32_fp8((int)c[i], true);
+        const f32x2 lo = __builtin_amdgcn_cvt_pk_f32_fp8((int)c[u][i], false);
+        const f32x2 hi = __builtin_amdgcn_cvt_pk_f32_fp8((int)c[u][i], true);
         v[4 * i] = lo[0] * f;
         v[4 * i + 1] = lo[1] * f;
         v[4 * i + 2] = hi[0] * f;
@@ -133,28 +158,29 @@ __global__ __launch_bounds__(256) void dequantize_kernel(const uint8_t* q, int64
         for (int e = 0; e < 8; ++e)
           if (k0 + e < K) v[e] += load_as_f32(shift, shift_dt, k0 + e);
       }
-    } else {
 #pragma unroll
-      for (int e = 0; e < 8; ++e) v[e] = 0.f;
-    }
-    if (vec && k0 + 8 <= K) {
-      if constexpr (ODT == SF_F32) {
-        float* dst = (float*)out + m * som + k0;
-        *(float4*)dst = float4{v[0], v[1], v[2], v[3]};
-        *(float4*)(dst + 4) = float4{v[4], v[5], v[6], v[7]};
-      } else {
-        u32x4 o;
+      for (int e = 0; e < 8; ++e) v[e] = in[u] ? v[e] : 0.f;
+      if (vec && k0 + 8 <= K) {
+        if constexpr (ODT == SF_F32) {
+          u32x4* dst = (u32x4*)((float*)out + m[u] * som + k0);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) o[e] = f32_to_bits(v[2 * e], ODT) | f32_to_bits(v[2 * e + 1], ODT) << 16;
-        *(u32x4*)((u16*)out + m * som + k0) = o;
-      }
-    } else {
+          for (int i = 0; i < 2; ++i)
+            __builtin_nontemporal_store(u32x4{__float_as_uint(v[4 * i]), __float_as_uint(v[4 * i + 1]),
+                                              __float_as_uint(v[4 * i + 2]), __float_as_uint(v[4 * i + 3])}, dst + i);
+        } else {
+          u32x4 o;
 #pragma unroll
-      for (int e = 0; e < 8; ++e)
-        if (k0 + e < K) {
-          if constexpr (ODT == SF_F32) ((float*)out)[m * som + k0 + e] = v[e];
-          else ((u16*)out)[m * som + k0 + e] = (u16)f32_to_bits(v[e], ODT);
+          for (int e = 0; e < 4; ++e) o[e] = f32_to_bits(v[2 * e], ODT) | f32_to_bits(v[2 * e + 1], ODT) << 16;
+          __builtin_nontemporal_store(o, (u32x4*)((u16*)out + m[u] * som + k0));
         }
+      } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+          if (k0 + e < K) {
+            if constexpr (ODT == SF_F32) ((float*)out)[m[u] * som + k0 + e] = v[e];
+            else ((u16*)out)[m[u] * som + k0 + e] = (u16)f32_to_bits(v[e], ODT);
+          }
+      }
     }
   }
 }
@@ -165,8 +191,13 @@ constexpr int64_t MOST_BLOCKS = 1ll << 30;  // of one launch (32-bit block numbe
 
 bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
 
-// Workgroups of 16 blocks each: enough to fill the chip several times over, then a grid stride.
-unsigned grid_of(int64_t total) { return (unsigned)std::min<int64_t>((total + 15) / 16, 1 << 16); }
+// Blocks under way in a lane: one where there are few, so that they spread over the chip.
+constexpr int64_t UNROLL_FROM = 65536;
+// Workgroups of 16 blocks (times those under way): enough to fill the chip several times over, then a
+// grid stride.
+unsigned grid_of(int64_t total, int unroll) {
+  return (unsigned)std::min<int64_t>((total + 16 * unroll - 1) / (16 * unroll), 1 << 16);
+}
 
 int check_store(const void* q, int64_t sq, const void* scale, int64_t ss, int64_t R, int64_t K) {
   SF_REQUIRE(q && scale, "codes and scales must not be NULL");
@@ -182,19 +213,19 @@ int check_store(const void* q, int64_t sq, const void* scale, int64_t ss, int64_
 
 template <int DT>
 int quantize_typed(const void* x, int64_t sxm, int64_t sxk, const void* shift, int shift_dt, int64_t M, int64_t K,
-                   void* q, int64_t sq, void* scale, int64_t ss, int64_t row0, int64_t R, hipStream_t s) {
-  constexpr int E = DT == SF_F32 ? 4 : 2;
+                   void* q, int64_t sq, void* scale, int64_t ss, int64_t row0, int64_t R, int32_t* ctr, hipStream_t s) {
+  constexpr int E = DT == SF_F32 ? 4 : 2, CR = CROWS<DT>;
   const int64_t nb = blocks_of(K);
   const int pad = (int)(scale_bytes(K) - nb);
   if (sxm == 1 && sxk != 1 && M >= 16 && nb < 65536) {
-    // 65536 * 64 rows a launch at most
+    // 65536 * CR rows a launch at most
     const int vec = aligned16(x) && sxk * E % 16 == 0;
-    for (int64_t m = 0; m < M; m += 64 << 16) {
-      const int64_t n = std::min<int64_t>(M - m, 64 << 16);
+    for (int64_t m = 0; m < M; m += (int64_t)CR << 16) {
+      const int64_t n = std::min<int64_t>(M - m, (int64_t)CR << 16);
       const int64_t at = (row0 + m) % R;
-      hipLaunchKernelGGL((quantize_columns_kernel<DT>), dim3((unsigned)((n + 63) / 64), (unsigned)nb), dim3(256), 0, s,
+      hipLaunchKernelGGL((quantize_columns_kernel<DT>), dim3((unsigned)((n + CR - 1) / CR), (unsigned)nb), dim3(4 * CR), 0, s,
                          (const char*)x + m * E, sxk, vec, shift, shift_dt, n, K, nb, (uint8_t*)q, sq, (uint8_t*)scale,
-                         ss, at, R, pad);
+                         ss, at, R, pad, ctr);
       SF_LAUNCH_CHECK("quantize_columns");
     }
     return SF_OK;
@@ -205,14 +236,13 @@ int quantize_typed(const void* x, int64_t sxm, int64_t sxk, const void* shift, i
   for (int64_t m = 0; m < M; m += step) {
     const int64_t n = std::min(M - m, step);
     const int64_t at = (row0 + m) % R;
-    const dim3 grid(grid_of(n * nb)), block(256);
     const char* xm = (const char*)x + m * sxm * E;
-    if (rows)
-      hipLaunchKernelGGL((quantize_kernel<DT, SRC_ROWS>), grid, block, 0, s, xm, sxm, sxk, shift, shift_dt, svec, K,
-                         (uint32_t)nb, (uint32_t)(n * nb), (uint8_t*)q, sq, (uint8_t*)scale, ss, at, R, pad);
-    else
-      hipLaunchKernelGGL((quantize_kernel<DT, SRC_ANY>), grid, block, 0, s, xm, sxm, sxk, shift, shift_dt, svec, K,
-                         (uint32_t)nb, (uint32_t)(n * nb), (uint8_t*)q, sq, (uint8_t*)scale, ss, at, R, pad);
+    auto go = [&](auto kernel) {
+      hipLaunchKernelGGL(kernel, dim3(grid_of(n * nb, 1)), dim3(256), 0, s, xm, sxm, sxk, shift, shift_dt, svec, K,
+                         (uint32_t)nb, (uint32_t)(n * nb), (uint8_t*)q, sq, (uint8_t*)scale, ss, at, R, pad, ctr);
+    };
+    if (rows) go(quantize_kernel<DT, SRC_ROWS>);
+    else go(quantize_kernel<DT, SRC_ANY>);
     SF_LAUNCH_CHECK("quantize");
   }
   return SF_OK;
@@ -221,11 +251,12 @@ int quantize_typed(const void* x, int64_t sxm, int64_t sxk, const void* shift, i
 }  // namespace
 
 int launch_quantize(const void* x, int64_t sxm, int64_t sxk, int x_dt, const void* shift, int shift_dt, int64_t M,
-                    int64_t K, void* q, int64_t sq, void* scale, int64_t ss, int64_t row0, int64_t R, hipStream_t s) {
+                    int64_t K, void* q, int64_t sq, void* scale, int64_t ss, int64_t row0, int64_t R, int32_t* ctr,
+                    hipStream_t s) {
   switch (x_dt) {
-    case SF_F32: return quantize_typed<SF_F32>(x, sxm, sxk, shift, shift_dt, M, K, q, sq, scale, ss, row0, R, s);
-    case SF_BF16: return quantize_typed<SF_BF16>(x, sxm, sxk, shift, shift_dt, M, K, q, sq, scale, ss, row0, R, s);
-    default: return quantize_typed<SF_F16>(x, sxm, sxk, shift, shift_dt, M, K, q, sq, scale, ss, row0, R, s);
+    case SF_F32: return quantize_typed<SF_F32>(x, sxm, sxk, shift, shift_dt, M, K, q, sq, scale, ss, row0, R, ctr, s);
+    case SF_BF16: return quantize_typed<SF_BF16>(x, sxm, sxk, shift, shift_dt, M, K, q, sq, scale, ss, row0, R, ctr, s);
+    default: return quantize_typed<SF_F16>(x, sxm, sxk, shift, shift_dt, M, K, q, sq, scale, ss, row0, R, ctr, s);
   }
 }
 
@@ -243,7 +274,7 @@ extern "C" int sf_quantize_rows(const void* x, int64_t sxm, int64_t sxk, int x_d
   if (const int rc = check_store(q, sq, scale, ss, R, K)) return rc;
   SF_REQUIRE(M <= R, "%lld rows do not fit %lld", (long long)M, (long long)R);
   SF_REQUIRE(row0 >= 0 && row0 < R, "first row %lld outside [0, %lld)", (long long)row0, (long long)R);
-  return launch_quantize(x, sxm, sxk, x_dt, shift, shift_dt, M, K, q, sq, scale, ss, row0, R, (hipStream_t)stream);
+  return launch_quantize(x, sxm, sxk, x_dt, shift, shift_dt, M, K, q, sq, scale, ss, row0, R, nullptr, (hipStream_t)stream);
 }
 
 extern "C" int sf_dequantize_rows(const void* q, int64_t sq, const void* scale, int64_t ss, int64_t R,
@@ -269,16 +300,20 @@ extern "C" int sf_dequantize_rows(const void* q, int64_t sq, const void* scale, 
     const int64_t n = std::min(M - m, step);
     const int64_t at = rows ? 0 : (row0 + m) % R;
     const int64_t* ids = rows ? rows + m : nullptr;
-    const dim3 grid(grid_of(n * nb)), block(256);
     void* o = (char*)out + m * som * E;
-    const hipStream_t s = (hipStream_t)stream;
-    auto go = [&](auto kernel) {
-      hipLaunchKernelGGL(kernel, grid, block, 0, s, (const uint8_t*)q, sq, (const uint8_t*)scale, ss, R, ids, at, shift,
-                         shift_dt, svec, K, (uint32_t)nb, (uint32_t)(n * nb), o, som, vec);
+    auto go = [&](auto kernel, int unroll) {
+      hipLaunchKernelGGL(kernel, dim3(grid_of(n * nb, unroll)), dim3(256), 0, (hipStream_t)stream, (const uint8_t*)q, sq,
+                         (const uint8_t*)scale, ss, R, ids, at, shift, shift_dt, svec, K, (uint32_t)nb, (uint32_t)(n * nb),
+                         o, som, vec);
     };
-    if (out_dt == SF_F32) go(dequantize_kernel<SF_F32>);
-    else if (out_dt == SF_BF16) go(dequantize_kernel<SF_BF16>);
-    else go(dequantize_kernel<SF_F16>);
+    auto typed = [&](auto dt_tag) {
+      constexpr int DT = decltype(dt_tag)::value;
+      if (DT == SF_F32 || n * nb < UNROLL_FROM) go(dequantize_kernel<DT, 1>, 1);
+      else go(dequantize_kernel<DT, 2>, 2);
+    };
+    if (out_dt == SF_F32) typed(std::integral_constant<int, SF_F32>{});
+    else if (out_dt == SF_BF16) typed(std::integral_constant<int, SF_BF16>{});
+    else typed(std::integral_constant<int, SF_F16>{});
     SF_LAUNCH_CHECK("dequantize");
   }
   return SF_OK;
