@@ -503,7 +503,7 @@ __device__ __forceinline__ void f8_epilogue(const Out& a, f32x16 (&acc)[4][4], i
   }
 }
 
-// Persistent form for 256x256 tiles of 16-bit results: gemm_persist_kernel's walk of an XCD's tiles, its claims, its alternating stage buffers
+// Persistent form for 256x256 tiles: gemm_persist_kernel's walk of an XCD's tiles, its claims, its alternating stage buffers
 // and its epilogue, four waves of 128x128 (one per SIMD; eight waves of 128x64 would need the registers of
 // both halves' fragments twice), with a K loop of its own:
 //   Y(kt)      16 MFMAs on the first half (64 elements) of block kt, the second half's fragments read
@@ -518,7 +518,8 @@ template <int ODT, bool PLAIN>
 __global__ __launch_bounds__(256, 1) void gemm_f8_persist_kernel(F8Args a) {
   using namespace sfenc;
   constexpr int NW = 4, NB = 4, MB = 4, NMF = NB * MB;
-  constexpr int NST = 32;                 // the epilogue's stores per lane
+  constexpr bool WIDE = ODT == SF_F32;
+  constexpr int NST = WIDE ? 63 : 32;     // the epilogue's stores per lane (64 of fp32; vmcnt counts to 63)
   constexpr int PER = 32 / NW;            // DMAs a wave issues per operand and K-step
   // Y's schedule: two reads after each of the first YD MFMAs and one after the others, the barrier after
   // MFMA YB, one DMA an MFMA from there on
@@ -592,7 +593,7 @@ __global__ __launch_bounds__(256, 1) void gemm_f8_persist_kernel(F8Args a) {
     const auto c = cold();
     s_bias[slot][t] = bits_as_f32(r.bias, c->benc_dt);
     if constexpr (!PLAIN) {
-      constexpr float h = ODT == SF_BF16 ? 0x1p-126f : 0x1p-25f;
+      constexpr float h = ODT == SF_F32 ? 0.f : (ODT == SF_BF16 ? 0x1p-126f : 0x1p-25f);
       float tv = c->act == SF_ACT_NONE ? __builtin_nanf("") : h;
       if (t > T.rn) {
         tv = __builtin_inff();
@@ -752,27 +753,96 @@ __global__ __launch_bounds__(256, 1) void gemm_f8_persist_kernel(F8Args a) {
 #pragma unroll
       for (int q = 0; q < 8; ++q) sc[q] = scn[q];
     };
+    // The wide form of both phases: four parts of 16 bf16 MFMAs each. b: this part's and the next part's x'
+    // fragments, a: this group of four MFMAs' W fragment and the next's, widened one dword each an
+    // MFMA ahead of their use; the last part prepares the next phase's first (its fragments g, scales gs).
+    // Reads, barrier and DMAs lie where they lie among a quarter as many MFMAs in the narrow form.
+    bf16x8 wb[2][MB], wa[2];
+    auto widen = [&](const Frag& f, const int (&s)[8], int q, int part) {
+      return widen8(join(f.lo[q], f.hi[q]), part, scale_of(s[q]));
+    };
+    auto phase_wide = [&](auto y_tag, auto dma_tag, const Frag& f, const int (&fs)[8], Frag& g, const int (&gs)[8],
+                          char* cur, const char* nxt, int kt) {
+      constexpr bool Y = decltype(y_tag)::value, DMA = decltype(dma_tag)::value;
+#pragma unroll
+      for (int part = 0; part < 4; ++part) {
+#pragma unroll
+        for (int i = 0; i < NMF; ++i) {
+          const int j = part * NMF + i, nb = i >> 2, mb = i & 3;
+          acc[nb][mb] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(wa[nb & 1], wb[part & 1][mb], acc[nb][mb], 0, 0, 0);
+          asm volatile("" : "+a"(acc[nb][mb]));
+          if (j % 2 == 0 && j < 32) {
+            if constexpr (Y) read(g, cur, 1, j / 2);
+            else read(g, nxt, 0, j / 2);
+          }
+          if (Y && j == 4 * YB) {
+            wait_vm_lgkm0<0>();
+            barrier_no_fence();
+            read_scales(scn, kt + 1);
+          }
+          if constexpr (DMA) {
+            const int e = j / 4;
+            if (j % 4 == 2 && (!Y || e > YB)) {
+              if constexpr (Y) stage(T, off, kt + 2, cur, e - YB - 1, e - YB);
+              else stage(T, off, kt + 2, cur, 15 - YB + e, 16 - YB + e);
+            }
+          }
+          if (mb == 2) {
+            // the next group's W fragment, and one of the next part's x' fragments
+            const int na = (nb + 1) & 3, pa = nb == 3 ? part + 1 : part;
+            if (pa < 4) wa[(nb + 1) & 1] = widen(f, fs, 4 + na, pa);
+            else wa[(nb + 1) & 1] = widen(g, gs, 4 + na, 0);
+          }
+          if (mb == 0) {
+            if (part < 3) wb[(part + 1) & 1][nb] = widen(f, fs, nb, part + 1);
+            else wb[(part + 1) & 1][nb] = widen(g, gs, nb, 0);
+          }
+          __builtin_amdgcn_sched_barrier(0);
+        }
+      }
+    };
+    // K-step kt from its first half on: Y, then (more than one K-step left) X into kt + 1
+    auto wide_y = [&](auto dma_tag, char* cur, int kt) { phase_wide(std::true_type{}, dma_tag, F0, sc, F1, sc, cur, nullptr, kt); };
+    auto wide_x = [&](auto dma_tag, const char* nxt, char* cur, int kt) {
+      phase_wide(std::false_type{}, dma_tag, F1, sc, F0, scn, cur, nxt, kt);
+      if (decltype(dma_tag)::value && ((kt + 2) & 3) == 0) stage_scales(T, (kt + 2) >> 2, w, thread());
+#pragma unroll
+      for (int q = 0; q < 8; ++q) sc[q] = scn[q];
+    };
+    auto run_y = [&](auto dma_tag, char* cur, int kt) {
+      if constexpr (WIDE) wide_y(dma_tag, cur, kt);
+      else phase_y(dma_tag, cur, kt);
+    };
+    auto run_x = [&](auto dma_tag, const char* nxt, char* cur, int kt) {
+      if constexpr (WIDE) wide_x(dma_tag, nxt, cur, kt);
+      else phase_x(dma_tag, nxt, cur, kt);
+    };
     read_scales(sc, 0);
 #pragma unroll
     for (int i = 0; i < 16; ++i) read(F0, B0, 0, i);
+    if constexpr (WIDE) {
+      wa[0] = widen(F0, sc, 4, 0);
+#pragma unroll
+      for (int mb = 0; mb < MB; ++mb) wb[0][mb] = widen(F0, sc, mb, 0);
+    }
     using Yes = std::true_type;
     using No = std::false_type;
     int end = KT;
     asm volatile("" : "+s"(end));  // (opaque: whether there is a loop is not remembered across tiles)
     for (int kt = 0; kt + 2 < end; kt += 2) {
-      phase_y(Yes{}, B0, kt);
-      phase_x(Yes{}, B1, B0, kt);
-      phase_y(Yes{}, B1, kt + 1);
-      phase_x(Yes{}, B0, B1, kt + 1);
+      run_y(Yes{}, B0, kt);
+      run_x(Yes{}, B1, B0, kt);
+      run_y(Yes{}, B1, kt + 1);
+      run_x(Yes{}, B0, B1, kt + 1);
     }
-    phase_y(No{}, B0, KT - 2);
+    run_y(No{}, B0, KT - 2);
     // (behind a barrier of this tile, even where it has two K-steps only: s_claim is this tile's)
     const int nlid = first + step + s_claim;  // claims past the range fail: the loop ends
     const bool more = nlid < last;
     const Tile U = open_tile(more ? nlid : lid);
     const Raw raw = load_raw(U, thread());
-    phase_x(No{}, B1, B0, KT - 2);
-    phase_y(No{}, B1, KT - 1);
+    run_x(No{}, B1, B0, KT - 2);
+    run_y(No{}, B1, KT - 1);
     // both buffers are free past the last barrier: the next tile's block 0 goes to B1 (its B0), the
     // epilogue stages through B0
     t = thread();
@@ -784,16 +854,33 @@ __global__ __launch_bounds__(256, 1) void gemm_f8_persist_kernel(F8Args a) {
       stage_scales(U, 0, w, t);
     }
     T = U;
+    if constexpr (WIDE) {
+      // the last half: its fragments are in F1, its first part is widened
 #pragma unroll
-    for (int i = 0; i < NMF; ++i) mma(F1, i);
+      for (int part = 0; part < 4; ++part) {
+#pragma unroll
+        for (int nb = 0; nb < NB; ++nb) {
+          const bf16x8 pa = widen(F1, sc, 4 + nb, part);
+#pragma unroll
+          for (int mb = 0; mb < MB; ++mb)
+            acc[nb][mb] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(pa, widen(F1, sc, mb, part), acc[nb][mb], 0, 0, 0);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < NMF; ++i) mma(F1, i);
+    }
     const Out out = {(char*)cold()->out, cold()->som, cold()->row_nnz, cold()->M, cold()->N, cold()->act};
     if (mw + 128 <= out.M && nw + 128 <= out.N) {
-      f8_epilogue<ODT, PLAIN, false>(out, acc, mw, nw, lane, s_thr[P] + wn * 128, B0 + w * 16384);
+      if constexpr (WIDE) tile_epilogue<4, MB, NB, PLAIN>(out, SF_F32, acc, mw, nw, lane, s_thr[P] + wn * 128, B0 + w * 16384);
+      else f8_epilogue<ODT, PLAIN, false>(out, acc, mw, nw, lane, s_thr[P] + wn * 128, B0 + w * 16384);
       // vector-memory operations retire in issue order: at most the epilogue's NST stores outstanding
       // means that the next tile's DMAs have landed
       __builtin_amdgcn_s_waitcnt(0x0F70 | (NST & 15) | (((NST >> 4) & 3) << 14));
     } else {
-      f8_epilogue<ODT, PLAIN, true>(out, acc, mw, nw, lane, s_thr[P] + wn * 128, B0 + w * 16384);
+      if constexpr (WIDE) tile_epilogue<4, MB, NB, PLAIN>(out, SF_F32, acc, mw, nw, lane, s_thr[P] + wn * 128, B0 + w * 16384);
+      else f8_epilogue<ODT, PLAIN, true>(out, acc, mw, nw, lane, s_thr[P] + wn * 128, B0 + w * 16384);
       wait_vmcnt0();
     }
     return more;

@@ -32,7 +32,7 @@ hipError_t launch_tile(F8Args& a, hipStream_t s) {
   return hipGetLastError();
 }
 
-// 256x256 tiles of 16-bit results: the persistent form, one workgroup per CU (at most one per
+// 256x256 tiles: the persistent form, one workgroup per CU (at most one per
 // tile, whole XCD groups of eight). ctr: TILE_CTR_BYTES of the caller's workspace, `cleared` already or not.
 hipError_t launch_persist(F8Args& a, void* ctr, bool cleared, hipStream_t s) {
   a.tiles_m = (int)((a.M + BM - 1) / BM);
@@ -46,7 +46,10 @@ hipError_t launch_persist(F8Args& a, void* ctr, bool cleared, hipStream_t s) {
   a.tile_ctr = total > (int)grid.x ? (int32_t*)ctr : nullptr;
   if (a.tile_ctr && !cleared) hipLaunchKernelGGL(clear_counters_kernel, dim3(1), dim3(64), 0, s, a.tile_ctr);
   const bool plain = a.act != SF_ACT_JUMPRELU && !a.row_nnz;
-  if (a.out_dt == SF_F16) {
+  if (a.out_dt == SF_F32) {
+    if (plain) hipLaunchKernelGGL((gemm_f8_persist_kernel<SF_F32, true>), grid, block, 0, s, a);
+    else hipLaunchKernelGGL((gemm_f8_persist_kernel<SF_F32, false>), grid, block, 0, s, a);
+  } else if (a.out_dt == SF_F16) {
     if (plain) hipLaunchKernelGGL((gemm_f8_persist_kernel<SF_F16, true>), grid, block, 0, s, a);
     else hipLaunchKernelGGL((gemm_f8_persist_kernel<SF_F16, false>), grid, block, 0, s, a);
   } else {
@@ -100,9 +103,10 @@ struct Tokens {
 // the CUs a part per block of K (`alone` times that with one workgroup a CU) and one per tile; at least
 // the bytes at the rate that the shape streams them. Fitted to 176 shapes of 1 to 4096 tokens, d_in 256 to
 // 4096, 4096 to 131072 features, in both result sizes: the pick is 0.9% slower than the best of the
-// four in the mean, 14% at most. Where each wins at d_in 2304, d_sae 65536, bf16 (us of the four in order):
+// four in the mean, 17% at most. Where each wins at d_in 2304, d_sae 65536, bf16 (us of the four in order):
 // 32 tokens 26 24 25 33 (d_sae 16384: 10 11 18 27), 128 tokens 58 33 28 36, 256 tokens 108 59 47 40, 4096
-// tokens 1690 880 710 525.
+// tokens 1690 880 710 525; fp32 results of 128 tokens 62 49 42 62, of 256 118 94 81 70, of 4096 1750 1370 1140
+// 1040.
 struct Shape {
   int tm, tn;
   float fixed, step, alone, tile, tail, tbs;
@@ -112,17 +116,18 @@ constexpr Shape SHAPES[2][4] = {
     {{32, 128, 2.48f, 0.206f, 1.27f, 1.00f, 0.39f, 5.95f}, {64, 128, 2.28f, 0.295f, 1.38f, 1.26f, 0.42f, 6.54f},
      {128, 128, 1.52f, 0.469f, 1.65f, 1.94f, 0.39f, 6.22f}, {256, 256, 3.10f, 1.346f, 0.76f, 6.38f, 0.27f, 5.11f}},
     // fp32 results
-    {{32, 128, 2.23f, 0.314f, 1.47f, 1.25f, 0.28f, 6.41f}, {64, 128, 2.04f, 0.496f, 1.27f, 1.74f, 0.25f, 5.53f},
-     {128, 128, 1.87f, 0.830f, 1.18f, 2.34f, 0.37f, 5.08f}, {}}};
-// What result rows off 16 B cost a 256x256 tile (d_sae 10007, d_in 1000, 4096 tokens: 72 us against 52).
-constexpr float UNALIGNED_TILE = 6.f;
+    {{32, 128, 2.06f, 0.326f, 1.46f, 1.27f, 0.60f, 6.30f}, {64, 128, 1.84f, 0.510f, 1.26f, 1.83f, 0.37f, 5.50f},
+     {128, 128, 1.61f, 0.851f, 1.16f, 2.38f, 0.50f, 4.84f}, {256, 256, 0.04f, 2.986f, 0.73f, 9.65f, 0.27f, 3.53f}}};
+// What result rows off 16 B cost a 256x256 tile (d_in 1000 and 1024: 319 us for 5303 tokens over 49153 features,
+// 128x128 tiles 357; 72 for 4096 over 10007, 128x128 tiles 62).
+constexpr float UNALIGNED_TILE = 3.f;
 
 int pick_shape(int64_t M, int64_t N, int64_t K, int out_dt, bool unaligned) {
   const int nb = (int)blocks_of(K), wide = out_dt == SF_F32;
   const double bytes = (double)N * K + (double)M * K + (double)M * N * sf_dtype_size(out_dt);
   int best = -1;
   double least = 0;
-  for (int i = 0; i < (wide ? 3 : 4); ++i) {
+  for (int i = 0; i < 4; ++i) {
     const Shape& h = SHAPES[wide][i];
     const double x = (double)((M + h.tm - 1) / h.tm) * (double)((N + h.tn - 1) / h.tn) / 256;
     const double rounds = x <= 1 ? 1 : (x < 3 ? ceil(x) : x + h.tail);

@@ -24,7 +24,7 @@ class Fp8Rows:
     """R rows of d elements in 8 bits: `q` [R, d rounded up to 128] float8_e4m3fn, zeros behind d, and
     `scale` [R, ceil(d / 128) rounded up to 4] uint8. Slicing rows gives a view."""
 
-    __slots__ = ("q", "scale", "d")
+    __slots__ = ("q", "scale", "d", "_args")
 
     def __init__(self, q, scale, d):
         if q.dtype != torch.float8_e4m3fn or scale.dtype != torch.uint8:
@@ -36,7 +36,11 @@ class Fp8Rows:
                              f"scales, got {q.shape[1]} and {scale.shape[1]}")
         if q.stride(1) != 1 or scale.stride(1) != 1:
             raise ValueError("codes and scales must be contiguous along a row")
+        if q.device != scale.device:
+            raise ValueError(f"codes are on {q.device}, scales on {scale.device}")
         self.q, self.scale, self.d = q, scale, d
+        # the C ABI's (codes, their stride, scales, their stride)
+        self._args = (q.data_ptr(), q.stride(0), scale.data_ptr(), scale.stride(0))
 
     @classmethod
     def empty(cls, rows, d, device="cuda"):
@@ -89,6 +93,18 @@ def _shift(t, n, name):
     return None if t is None else _vector(t, n, name)
 
 
+def _device(first, *named):
+    """first's device, which the other tensors (or None) have to share; require_gpu's errors."""
+    dev = first.device
+    if dev.type == "cuda":
+        for _, t in named:
+            if t is not None and t.device != dev:
+                break
+        else:
+            return dev
+    return _lib.require_gpu(("rows", first), *named)
+
+
 def quantize_rows(x, *, shift=None, out=None, row0=0):
     """x [M, d] in fp32, bf16 or fp16 (any strides; a transposed matrix is read along its own rows) as
     8-bit rows, minus `shift` [d] if given (the difference in fp32).
@@ -104,18 +120,18 @@ def quantize_rows(x, *, shift=None, out=None, row0=0):
     if out is None:
         if row0:
             raise ValueError("row0 is a row of `out`, which is not given")
-        _lib.require_gpu(("x", x))
-        out = Fp8Rows.empty(M, d, x.device)
+        out = Fp8Rows.empty(M, d, _device(x))
     elif out.d != d:
         raise ValueError(f"out holds rows of {out.d}, x has {d}")
-    dev = _lib.require_gpu(("x", x), ("shift", shift), ("out", out.q), ("out", out.scale))
+    dev = _device(x, ("out", out.q), ("shift", shift))
     if M == 0:
         return out
+    sxm, sxk = x.stride()
     with _lib.device(dev):
         _lib.check(_lib.load().sf_quantize_rows(
-            x.data_ptr(), x.stride(0), x.stride(1), _lib.dtype_code(x, "x"), _lib.ptr(shift),
-            0 if shift is None else _lib.dtype_code(shift, "shift"), M, d, out.q.data_ptr(), out.q.stride(0),
-            out.scale.data_ptr(), out.scale.stride(0), row0, len(out), _lib.stream(dev)))
+            x.data_ptr(), sxm, sxk, _lib.dtype_code(x, "x"), None if shift is None else shift.data_ptr(),
+            0 if shift is None else _lib.dtype_code(shift, "shift"), M, d, *out._args, row0, out.q.shape[0],
+            _lib.stream(dev)))
     return out
 
 
@@ -123,7 +139,7 @@ def dequantize_rows(rows8, rows=None, *, row0=0, count=None, shift=None, out_dty
     """Rows read back, plus `shift` [d] if given (the sum in fp32, then rounded to out_dtype): those with
     the ids `rows` (int64, in any order; an id outside the store gives zeros), or `count` rows from row0 on,
     going on at row 0 behind the last (all of them by default)."""
-    R, d = rows8.shape
+    R, d = rows8.q.shape[0], rows8.d
     if rows is not None:
         if rows.dtype != torch.int64 or rows.dim() != 1:
             raise ValueError(f"rows must be a one-dimensional int64 tensor, got {rows.dtype} {list(rows.shape)}")
@@ -136,16 +152,16 @@ def dequantize_rows(rows8, rows=None, *, row0=0, count=None, shift=None, out_dty
         if M < 0 or M > R:
             raise ValueError(f"count must lie in [0, {R}], got {M}")
     shift = _shift(shift, d, "shift")
-    dev = _lib.require_gpu(("rows8", rows8.q), ("rows8", rows8.scale), ("rows", rows), ("shift", shift))
-    out = torch.empty(M, d, dtype=out_dtype, device=dev)
+    dev = _device(rows8.q, ("rows", rows), ("shift", shift))
+    out = torch.empty((M, d), dtype=out_dtype, device=dev)
     code = _lib.dtype_code(out, "out_dtype")
     if M == 0:
         return out
     with _lib.device(dev):
         _lib.check(_lib.load().sf_dequantize_rows(
-            rows8.q.data_ptr(), rows8.q.stride(0), rows8.scale.data_ptr(), rows8.scale.stride(0), R, _lib.ptr(rows),
-            row0, _lib.ptr(shift), 0 if shift is None else _lib.dtype_code(shift, "shift"), M, d, out.data_ptr(), d,
-            code, _lib.stream(dev)))
+            *rows8._args, R, None if rows is None else rows.data_ptr(), row0,
+            None if shift is None else shift.data_ptr(), 0 if shift is None else _lib.dtype_code(shift, "shift"), M, d,
+            out.data_ptr(), d, code, _lib.stream(dev)))
     return out
 
 
@@ -169,32 +185,30 @@ def fused_encode_fp8(x, W, b_enc=None, threshold=None, activation="relu", *, b_d
         raise ValueError("b_dec is subtracted before tokens are quantised; 8-bit rows are taken as they are")
     if not held and x.dim() != 2:
         raise ValueError(f"x must have two dimensions, got {list(x.shape)}")
-    (M, d), (N, d_w) = x.shape, W.shape
+    (M, d), N, d_w = x.shape, W.q.shape[0], W.d
     if d != d_w:
         raise ValueError(f"x has d_in={d} but W has d_in={d_w}")
     if out_dtype is None:
         out_dtype = torch.bfloat16 if held else x.dtype
-    dev = _lib.require_gpu(("x", x.q if held else x), ("x", x.scale if held else None), ("W", W.q), ("W", W.scale),
-                           ("b_enc", b_enc), ("b_dec", b_dec), ("threshold", threshold), ("row_nnz", row_nnz))
+    dev = _device(x.q if held else x, ("W", W.q), ("b_enc", b_enc), ("b_dec", b_dec), ("threshold", threshold),
+                  ("row_nnz", row_nnz))
     b_enc, b_dec = _shift(b_enc, N, "b_enc"), _shift(b_dec, d, "b_dec")
     threshold = _vector(threshold, N, "threshold") if activation == "jumprelu" else None
     if row_nnz is not None:
         if row_nnz.dtype != torch.int32 or row_nnz.dim() != 1 or row_nnz.numel() != M or not row_nnz.is_contiguous():
             raise ValueError(f"row_nnz must be a contiguous int32 tensor of shape [{M}]")
-    out = torch.empty(M, N, dtype=out_dtype, device=dev)
+    out = torch.empty((M, N), dtype=out_dtype, device=dev)
     code = _lib.dtype_code(out, "out_dtype")
     if M == 0 or N == 0:
         return out
     lib = _lib.load()
-    tail = (W.q.data_ptr(), W.q.stride(0), W.scale.data_ptr(), W.scale.stride(0), _lib.ptr(b_enc),
-            0 if b_enc is None else _lib.dtype_code(b_enc, "b_enc"), _lib.ptr(threshold),
+    tail = (*W._args, _lib.ptr(b_enc), 0 if b_enc is None else _lib.dtype_code(b_enc, "b_enc"), _lib.ptr(threshold),
             0 if threshold is None else _lib.dtype_code(threshold, "threshold"), out.data_ptr(), N, code,
             _lib.ptr(row_nnz), M, N, d, ACTIVATIONS[activation])
     with _lib.device(dev):
         ws = torch.empty(_lib.fp8_workspace_bytes(0 if held else M, d), dtype=torch.uint8, device=dev)
         if held:
-            _lib.check(lib.sf_encode_fp8_rows(x.q.data_ptr(), x.q.stride(0), x.scale.data_ptr(), x.scale.stride(0),
-                                              *tail, ws.data_ptr(), ws.numel(), _lib.stream(dev)))
+            _lib.check(lib.sf_encode_fp8_rows(*x._args, *tail, ws.data_ptr(), ws.numel(), _lib.stream(dev)))
         else:
             x_code = _lib.dtype_code(x, "x")
             _lib.check(lib.sf_encode_fp8(x.data_ptr(), x.stride(0), x.stride(1), x_code, _lib.ptr(b_dec),
