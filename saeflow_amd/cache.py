@@ -7,6 +7,8 @@ so a cache written by either side reads on the other (cache.py:1-13):
     manifest.json                                   {"config", "hooks", "shards"}
     <hook>/<shard:05d>.npy                          dense activations [rows, d]
     <hook>/<shard:05d>.{indptr,indices,values}.npy  CSR features [rows, d_sae] (encoded hooks)
+    <hook>/<shard:05d>.{codes,scale}.npy            dense activations in 8 bits (dtype float8_e4m3fn, not
+                                                    in the reference), as kernels.Fp8Rows holds them
 
 Rows are token positions in sequence-major order, a shard holds `batches_per_shard`
 forward batches, bfloat16 arrays hold the raw 16-bit patterns (numpy has no bfloat16; the
@@ -43,6 +45,9 @@ import torch
 
 _DTYPE_NAMES = {torch.float32: "float32", torch.float16: "float16", torch.bfloat16: "bfloat16"}
 _CSR_FILES = ("indptr", "indices", "values")
+# Dense hooks in 8 bits: quantised on the GPU, so a row leaves it and is stored at a little over a byte an
+# element. Encoded hooks of such a cache keep their values in bfloat16.
+_FP8, _FP8_NAME, _FP8_FILES = torch.float8_e4m3fn, "float8_e4m3fn", ("codes", "scale")
 
 
 # ----------------------------------------------------------------------------- format
@@ -139,7 +144,7 @@ def _save_rows(fh, pieces):
             fh.write(np.ascontiguousarray(p).data)
 
 
-def _shard_arrays(out_dir, shard, held, csr_hooks):
+def _shard_arrays(out_dir, shard, held, csr_hooks, fp8=False):
     """The files of a finished shard as lists of stored numpy pieces, one list per file, to be
     written one after the other: per hook, the row-wise concatenation of its batches (CSR
     pieces with their indptr offsets moved, dense rows as they are). Plain numpy and no joined
@@ -154,6 +159,9 @@ def _shard_arrays(out_dir, shard, held, csr_hooks):
             indptr = [np.zeros(1, np.int64)] + [p[0][1:] + s for p, s in zip(parts, starts)]
             for part, rows in zip(_CSR_FILES, (indptr, [p[1] for p in parts], [p[2] for p in parts])):
                 files.append((_shard_file(out_dir, h, shard, part), rows))
+        elif fp8:
+            for i, part in enumerate(_FP8_FILES):
+                files.append((_shard_file(out_dir, h, shard, part), [p[i] for p in parts]))
         else:
             files.append((_shard_file(out_dir, h, shard), [p[0] for p in parts]))
     return files
@@ -210,21 +218,29 @@ def cache_activations(model, tokens, hook_names, out_dir, *, batch_size=8, batch
     model: anything with a TransformerLens-style run_with_cache(tokens, names_filter=,
       stop_at_layer=, return_type=) and parameters().
     encoders: optional {hook_name: sae}; those hooks are SAE-encoded on the fly on the GPU
-      and stored as CSR feature activations instead of dense ones.
+      and stored as CSR feature activations instead of dense ones. A saeflow_amd.Fp8Encoder is
+      taken in place of an SAE.
+    dtype: of the stored activations; float8_e4m3fn (not in the reference) holds dense hooks in 8 bits
+      with a scale for each block of 128, quantised on the model's GPU.
     A second call with identical arguments after an interruption picks up at the first shard
     the manifest does not list. The return value is the cache directory (a Path).
     """
     out_dir, hook_names, encoders = Path(out_dir), list(hook_names), dict(encoders or {})
-    if dtype not in _DTYPE_NAMES:
-        raise ValueError(f"cache dtype must be one of {list(_DTYPE_NAMES)}, got {dtype}")
+    fp8 = dtype == _FP8
+    if dtype not in _DTYPE_NAMES and not fp8:
+        raise ValueError(f"cache dtype must be one of {[*_DTYPE_NAMES, _FP8]}, got {dtype}")
     stray = sorted(set(encoders) - set(hook_names))
     if stray:
         raise ValueError(f"encoders given for hooks not being cached: {stray}")
-    if encoders:
+    if encoders or fp8:
+        from .fp8 import Fp8Encoder
+        from .kernels import quantize_rows
         from .ops import encode_sparse
+    value_dtype = torch.bfloat16 if fp8 else dtype
 
     config = {"hook_names": hook_names, "n_seqs": len(tokens), "seq_len": int(tokens.shape[1]),
-              "batch_size": batch_size, "batches_per_shard": batches_per_shard, "dtype": _DTYPE_NAMES[dtype],
+              "batch_size": batch_size, "batches_per_shard": batches_per_shard,
+              "dtype": _FP8_NAME if fp8 else _DTYPE_NAMES[dtype],
               "encoded": sorted(encoders)}
     manifest_path = out_dir / "manifest.json"
     manifest = {"config": config, "hooks": {}, "shards": []}
@@ -249,7 +265,7 @@ def cache_activations(model, tokens, hook_names, out_dir, *, batch_size=8, batch
         for shard in range(len(manifest["shards"]), len(shard_starts)):
             lo = shard_starts[shard]
             hi = min(lo + per_shard, len(tokens))
-            held = {h: [] for h in hook_names}
+            held, widths = {h: [] for h in hook_names}, {}
             for b0 in range(lo, hi, batch_size):
                 batch = tokens[b0:min(b0 + batch_size, hi)].to(device, non_blocking=True)
                 _, acts = model.run_with_cache(batch, names_filter=hook_names, stop_at_layer=depth, return_type=None)
@@ -257,15 +273,24 @@ def cache_activations(model, tokens, hook_names, out_dir, *, batch_size=8, batch
                     rows = acts[h].reshape(acts[h].shape[0] * acts[h].shape[1], -1)  # per-head hooks concatenated
                     sae = encoders.get(h)
                     if sae is None:
-                        held[h].append(staging.to_host(rows.to(dtype)))
+                        widths[h] = int(rows.shape[1])
+                        if fp8:
+                            r8 = quantize_rows(rows)
+                            held[h].append((staging.to_host(r8.q.view(torch.uint8)), staging.to_host(r8.scale)))
+                        else:
+                            held[h].append(staging.to_host(rows.to(dtype)))
                     else:
-                        csr = encode_sparse(sae, rows.to(sae.W_enc.device, sae.W_enc.dtype))
+                        if isinstance(sae, Fp8Encoder):
+                            csr, widths[h] = sae.encode_sparse(rows.to(sae.W.device)), len(sae.W)
+                        else:
+                            csr = encode_sparse(sae, rows.to(sae.W_enc.device, sae.W_enc.dtype))
+                            widths[h] = int(sae.W_enc.shape[1])
                         held[h].append((staging.to_host(csr[0]), staging.to_host(csr[1]),
-                                        staging.to_host(csr[2].to(dtype))))
-            hook_meta = {h: {"format": "csr", "d": int(encoders[h].W_enc.shape[1])} if h in encoders
-                         else {"format": "dense", "d": int(held[h][0].shape[1])} for h in hook_names}
+                                        staging.to_host(csr[2].to(value_dtype))))
+            dense = "fp8" if fp8 else "dense"
+            hook_meta = {h: {"format": "csr" if h in encoders else dense, "d": widths[h]} for h in hook_names}
             # the shard is assembled (CSR pieces joined, dense rows stacked) by the writer thread
-            build = functools.partial(_shard_arrays, out_dir, shard, held, frozenset(encoders))
+            build = functools.partial(_shard_arrays, out_dir, shard, held, frozenset(encoders), fp8)
             writer.hand_over((staging.take(), build, hook_meta, {"n_seqs": hi - lo, "n_rows": (hi - lo) * config["seq_len"]}))
     finally:
         writer.close()  # shards already handed over are written even when the run fails
@@ -280,7 +305,8 @@ class ActivationReader:
     def __init__(self, path):
         self.path = Path(path)
         self.manifest = json.loads((self.path / "manifest.json").read_text())
-        self.dtype = {v: k for k, v in _DTYPE_NAMES.items()}[self.manifest["config"]["dtype"]]
+        name = self.manifest["config"]["dtype"]
+        self.dtype = _FP8 if name == _FP8_NAME else {v: k for k, v in _DTYPE_NAMES.items()}[name]
         rows = [s["n_rows"] for s in self.manifest["shards"]]
         self._first_row = np.concatenate([[0], np.cumsum(rows)]).astype(np.int64).tolist()
 
@@ -294,24 +320,33 @@ class ActivationReader:
     def _sparse(self, hook):
         return self.manifest["hooks"][hook]["format"] == "csr"
 
+    def _fp8(self, hook):
+        return self.manifest["hooks"][hook]["format"] == "fp8"
+
     def _load(self, hook, shard):
+        if self._fp8(hook):
+            return tuple(np.load(_shard_file(self.path, hook, shard, p), mmap_mode="r") for p in _FP8_FILES)
         if self._sparse(hook):
             return tuple(np.load(_shard_file(self.path, hook, shard, p), mmap_mode="r") for p in _CSR_FILES)
         return np.load(_shard_file(self.path, hook, shard), mmap_mode="r")
 
     def _piece(self, hook, arrays, a, b):
         """Rows [a, b) of one shard."""
+        if self._fp8(hook):
+            return tuple(_as_tensor(part[a:b], torch.uint8) for part in arrays)
         if not self._sparse(hook):
             return _as_tensor(arrays[a:b], self.dtype)
         indptr, indices, values = arrays
         lo, hi = int(indptr[a]), int(indptr[b])
         return (torch.from_numpy(np.asarray(indptr[a:b + 1], dtype=np.int64) - lo),
-                _as_tensor(indices[lo:hi], torch.int32), _as_tensor(values[lo:hi], self.dtype))
+                _as_tensor(indices[lo:hi], torch.int32),
+                _as_tensor(values[lo:hi], torch.bfloat16 if self.dtype == _FP8 else self.dtype))
 
     def iter_batches(self, hook, batch_size):
         """Yield `batch_size`-row batches in cache order (the last may be short). Dense hooks
         yield [rows, d] tensors; encoded hooks yield CSR (indptr, indices, values) tuples, which
-        decode_sparse takes once they are on the GPU."""
+        decode_sparse takes once they are on the GPU; dense hooks in 8 bits yield kernels.Fp8Rows,
+        which dequantize_rows and Fp8Encoder take once they are there (rows.to("cuda"))."""
         total, opened = self.n_rows(), {}
         for start in range(0, total, batch_size):
             stop = min(start + batch_size, total)
@@ -324,4 +359,12 @@ class ActivationReader:
                 end = min(stop, self._first_row[shard + 1])
                 pieces.append(self._piece(hook, opened[shard], r - base, end - base))
                 r = end
-            yield _join_csr(pieces) if self._sparse(hook) else torch.cat(pieces)
+            if self._sparse(hook):
+                yield _join_csr(pieces)
+            elif self._fp8(hook):
+                from .kernels import Fp8Rows
+
+                codes, scale = (torch.cat(part) for part in zip(*pieces))
+                yield Fp8Rows(codes.view(_FP8), scale, self.manifest["hooks"][hook]["d"])
+            else:
+                yield torch.cat(pieces)

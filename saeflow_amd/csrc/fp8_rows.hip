@@ -286,6 +286,7 @@ extern "C" int sf_dequantize_rows(const void* q, int64_t sq, const void* scale, 
   SF_REQUIRE(M >= 0 && K >= 1 && K <= (1 << 24), "bad shape [%lld, %lld]", (long long)M, (long long)K);
   if (M == 0) return SF_OK;
   if (const int rc = check_store(q, sq, scale, ss, R, K)) return rc;
+  SF_REQUIRE(R >= 1, "a store of no rows has none to read");
   SF_REQUIRE(out, "out must not be NULL");
   SF_REQUIRE(som >= K || M == 1, "rows of the result overlap");
   if (!rows) {

@@ -261,6 +261,40 @@ def test_nan_stays_in_its_row_and_padding_is_never_read():
                        f[10:33].nan_to_num(-1.0))
 
 
+@pytest.mark.parametrize("out_dtype", [F32, BF16])
+def test_large_products_keep_nan_infinite_biases_and_thresholds(out_dtype):
+    """The persistent tiles: NaN rows and features, biases that are infinite, NaN, tiny and huge, a NaN
+    threshold (keeps nothing), counts; d_sae cuts the last tile."""
+    x, xv = whole(2300, 640, 5)
+    W, wv = whole(16200, 640, 6)
+    x.q.view(torch.uint8)[77, 3] = 0x7F
+    W.q.view(torch.uint8)[16199, 600] = 0xFF
+    W.q.view(torch.uint8)[300, 0] = 0x7F
+    xv[77], wv[16199], wv[300] = float("nan"), float("nan"), float("nan")
+    b = torch.randint(-50, 50, (16200,), device="cuda").float()
+    b[5], b[6], b[7], b[8], b[9] = float("inf"), float("-inf"), float("nan"), 1e-30, 3e38
+    pre = (xv @ wv.T.contiguous()).float() + b
+    pre[:, 9] = 3e38
+    pre[77, 9] = float("nan")
+    pre[:, 8] = (xv @ wv[8]).float() + torch.where(xv @ wv[8] == 0, 1e-30, 0.0).float()
+
+    def same(got, want):
+        return torch.equal(got.nan_to_num(-7.0, 1e38, -1e38), want.to(out_dtype).nan_to_num(-7.0, 1e38, -1e38))
+
+    assert same(fused_encode_fp8(x, W, b, activation="none", out_dtype=out_dtype), pre)
+    relu = torch.where(pre <= 0, 0.0, pre)
+    assert same(fused_encode_fp8(x, W, b, out_dtype=out_dtype), relu)
+    nnz = torch.zeros(2300, dtype=torch.int32, device="cuda")
+    f = fused_encode_fp8(x, W, b, out_dtype=out_dtype, row_nnz=nnz)
+    assert same(f, relu) and torch.equal(nnz, (f != 0).sum(1, dtype=torch.int32))
+    thr = torch.randint(0, 30, (16200,), device="cuda").float()
+    thr[100] = float("nan")
+    want = torch.relu(pre) * (pre > thr)  # (a NaN stays one, whatever its threshold)
+    nnz.zero_()
+    f = fused_encode_fp8(x, W, b, thr, "jumprelu", out_dtype=out_dtype, row_nnz=nnz)
+    assert same(f, want) and torch.equal(nnz, (f != 0).sum(1, dtype=torch.int32))
+
+
 @pytest.mark.parametrize("dtype", [F32, BF16, F16])
 @pytest.mark.parametrize("M", [0, 1, 5, 70, 300])
 def test_tokens_are_quantised_on_the_way(dtype, M):
