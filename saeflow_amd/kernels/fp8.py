@@ -128,10 +128,12 @@ def quantize_rows(x, *, shift=None, out=None, row0=0):
         return out
     sxm, sxk = x.stride()
     with _lib.device(dev):
-        _lib.check(_lib.load().sf_quantize_rows(
+        rc = _lib.load().sf_quantize_rows(
             x.data_ptr(), sxm, sxk, _lib.dtype_code(x, "x"), None if shift is None else shift.data_ptr(),
             0 if shift is None else _lib.dtype_code(shift, "shift"), M, d, *out._args, row0, out.q.shape[0],
-            _lib.stream(dev)))
+            _lib.stream(dev))
+    if rc:
+        _lib.check(rc)
     return out
 
 
@@ -146,22 +148,25 @@ def dequantize_rows(rows8, rows=None, *, row0=0, count=None, shift=None, out_dty
         if row0 or count is not None:
             raise ValueError("rows are named by ids or by row0 and count, not by both")
         rows = rows.contiguous()
-        M = rows.numel()
+        M, ids = rows.shape[0], rows.data_ptr()
     else:
-        M = R if count is None else count
+        M, ids = R if count is None else count, None
         if M < 0 or M > R:
             raise ValueError(f"count must lie in [0, {R}], got {M}")
-    shift = _shift(shift, d, "shift")
+    at, code = None, 0
+    if shift is not None:
+        shift = _vector(shift, d, "shift")
+        at, code = shift.data_ptr(), _lib.dtype_code(shift, "shift")
     dev = _device(rows8.q, ("rows", rows), ("shift", shift))
     out = torch.empty((M, d), dtype=out_dtype, device=dev)
-    code = _lib.dtype_code(out, "out_dtype")
+    out_code = _lib.dtype_code(out, "out_dtype")
     if M == 0:
         return out
     with _lib.device(dev):
-        _lib.check(_lib.load().sf_dequantize_rows(
-            *rows8._args, R, None if rows is None else rows.data_ptr(), row0,
-            None if shift is None else shift.data_ptr(), 0 if shift is None else _lib.dtype_code(shift, "shift"), M, d,
-            out.data_ptr(), d, code, _lib.stream(dev)))
+        rc = _lib.load().sf_dequantize_rows(*rows8._args, R, ids, row0, at, code, M, d, out.data_ptr(), d, out_code,
+                                            _lib.stream(dev))
+    if rc:
+        _lib.check(rc)
     return out
 
 
