@@ -154,8 +154,7 @@ __device__ __forceinline__ void tile_epilogue(const Out& a, int out_dt, f32x16 (
 // four blocks][row] dwords, loaded for 4096 elements of K at a time.
 //
 // FUSED (tokens of at most FUSED_BLOCKS blocks in all): the tokens come as they are; each workgroup, its
-// first stages of W under way, quantises all of them into LDS, where they stay. That costs a workgroup
-// about 2 us of latency and saves a launch.
+// first stages of W under way, quantises all of them into LDS, where they stay, and a launch is saved.
 constexpr int FUSED_BLOCKS = 32;
 template <typename TL, bool WIDE, bool PLAIN, bool FUSED>
 __global__ __launch_bounds__(TL::NT, TL::ST * TL::NS > 81920 ? (TL::NW + 3) / 4 : (TL::NW + 1) / 2) void gemm_f8_kernel(F8Args a) {
@@ -233,6 +232,29 @@ __global__ __launch_bounds__(TL::NT, TL::ST * TL::NS > 81920 ? (TL::NW + 3) / 4 
   const int64_t nb_ = min(n0 + t % TN, a.N - 1);
   const uint32_t rb = a.b_enc ? load_bits(a.b_enc, a.benc_dt, nb_) : 0u;
   const uint32_t rt = a.act == SF_ACT_JUMPRELU ? load_bits(a.thr, a.thr_dt, nb_) : 0u;
+  // FUSED: the raw bits of a thread's tokens and their shift, loaded before the stages of W (loads return in
+  // order: behind them they would arrive when all of those have), where they are whole 16-B units
+  constexpr int Q = NT / 16, XI = FUSED ? FUSED_BLOCKS / Q : 1;  // blocks taken at a time, and per sixteen lanes
+  sff8::u32x4 xraw[XI][2], craw[XI][2];
+  const int all = (int)min((int64_t)FUSED_BLOCKS, a.M * KT);  // blocks there are
+  const bool raw = FUSED && a.x_rows && a.K % 8 == 0 && (!a.shift || a.shift_vec);
+  if constexpr (FUSED) {
+#pragma unroll
+    for (int i = 0; i < XI; ++i) {
+      xraw[i][0] = xraw[i][1] = craw[i][0] = craw[i][1] = sff8::u32x4{0, 0, 0, 0};
+      const int b = min((t >> 4) + i * Q, all - 1), m = b / KT;
+      const int64_t k0 = (int64_t)(b - m * KT) * BLOCK + (t & 15) * 8;
+      if (raw && k0 < a.K) {
+        const int E = sf_dtype_size(a.x_dt);
+        const char* px = (const char*)a.x + (m * a.sxm + k0) * E;
+        const char* pc = (const char*)a.shift + k0 * E;
+        xraw[i][0] = *(const sff8::u32x4*)px;
+        if (E == 4) xraw[i][1] = *(const sff8::u32x4*)(px + 16);
+        if (a.shift) craw[i][0] = *(const sff8::u32x4*)pc;
+        if (a.shift && E == 4) craw[i][1] = *(const sff8::u32x4*)(pc + 16);
+      }
+    }
+  }
   load_scales(0);
   issue(0, s0);
   if constexpr (NS > 2) issue(1, s1);
@@ -255,32 +277,39 @@ __global__ __launch_bounds__(TL::NT, TL::ST * TL::NS > 81920 ? (TL::NW + 3) / 4 
   static_assert(TN <= NT, "a thread's bias");
   put_scales();
   if constexpr (FUSED) {
-    // sixteen lanes a block, all loads of a thread under way at once
-    auto quantize = [&](auto dt_tag, auto src_tag) {
-      constexpr int DT = decltype(dt_tag)::value, SRC = decltype(src_tag)::value, Q = NT / 16;
-      const int all = (int)a.M * KT;  // at most FUSED_BLOCKS
-      float v[FUSED_BLOCKS / Q][8];
+    auto put = [&](int i, float (&v)[8]) {
+      const int b = min((t >> 4) + i * Q, all - 1);
+      uint32_t byte;
+      *(sff8::u32x2*)(s_x + b * BLOCK + (t & 15) * 8) = quantize8(v, byte);
+      if ((t & 15) == 0) s_xsc[b] = (uint8_t)byte;
+    };
+    if (raw) {
 #pragma unroll
-      for (int i = 0; i < FUSED_BLOCKS / Q; ++i) {
+      for (int i = 0; i < XI; ++i) {
+        float v[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          if (a.x_dt == SF_F32) {
+            v[e] = __uint_as_float(xraw[i][e >> 2][e & 3]) - __uint_as_float(craw[i][e >> 2][e & 3]);
+          } else {
+            const int at = (e & 1) * 16;
+            v[e] = bits_as_f32((xraw[i][0][e >> 1] >> at) & 0xffffu, a.x_dt) -
+                   bits_as_f32((craw[i][0][e >> 1] >> at) & 0xffffu, a.x_dt);
+          }
+        }
+        put(i, v);
+      }
+    } else {
+      for (int i = 0; i < XI; ++i) {
         const int b = min((t >> 4) + i * Q, all - 1), m = b / KT;
-        load_shifted<DT, SRC>(a.x, a.sxm, a.sxk, a.shift, a.shift_dt, a.shift_vec, a.K, m,
-                              (int64_t)(b - m * KT) * BLOCK + (t & 15) * 8, v[i]);
+        const int64_t k0 = (int64_t)(b - m * KT) * BLOCK + (t & 15) * 8;
+        float v[8];
+        if (a.x_dt == SF_BF16) load_shifted<SF_BF16, SRC_ANY>(a.x, a.sxm, a.sxk, a.shift, a.shift_dt, 0, a.K, m, k0, v);
+        else if (a.x_dt == SF_F16) load_shifted<SF_F16, SRC_ANY>(a.x, a.sxm, a.sxk, a.shift, a.shift_dt, 0, a.K, m, k0, v);
+        else load_shifted<SF_F32, SRC_ANY>(a.x, a.sxm, a.sxk, a.shift, a.shift_dt, 0, a.K, m, k0, v);
+        put(i, v);
       }
-#pragma unroll
-      for (int i = 0; i < FUSED_BLOCKS / Q; ++i) {
-        const int b = min((t >> 4) + i * Q, all - 1);
-        uint32_t byte;
-        *(sff8::u32x2*)(s_x + b * BLOCK + (t & 15) * 8) = quantize8(v[i], byte);
-        if ((t & 15) == 0) s_xsc[b] = (uint8_t)byte;
-      }
-    };
-    auto typed = [&](auto src_tag) {
-      if (a.x_dt == SF_BF16) quantize(std::integral_constant<int, SF_BF16>{}, src_tag);
-      else if (a.x_dt == SF_F16) quantize(std::integral_constant<int, SF_F16>{}, src_tag);
-      else quantize(std::integral_constant<int, SF_F32>{}, src_tag);
-    };
-    if (a.x_rows) typed(std::integral_constant<int, SRC_ROWS>{});
-    else typed(std::integral_constant<int, SRC_ANY>{});
+    }
   }
   wait_lgkmcnt0();
   barrier_no_fence();

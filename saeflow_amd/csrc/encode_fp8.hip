@@ -88,8 +88,8 @@ int check_call(const char* fn, const void* b_enc, int benc_dt, const void* thr, 
 }
 
 // Tokens are quantised by each workgroup of the product for itself where their blocks are one round of
-// loads for it and there are at most two workgroups a CU: one token of d_in 2304 over 16384 features 11.8 us a
-// call against 13.1 with a quantisation of its own, over 65536 (four a CU) 30 against 27.
+// loads for it and there are at most two workgroups a CU: one token of d_in 2304 over 16384 features 10.6 us a
+// call against 13.1 with a quantisation of its own, over 65536 (four a CU) 27.5 against 26.5.
 constexpr int64_t FUSED_FEATURES = 32768;
 struct Tokens {
   const void* x;

@@ -306,6 +306,20 @@ def test_tokens_are_quantised_on_the_way(dtype, M):
         assert got.dtype == dtype and torch.equal(got, want)
 
 
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("M,d", [(1, 8), (3, 128), (8, 504), (1, 1000), (1, 2304), (4, 1024), (1, 4096), (2, 2300)])
+def test_few_tokens_quantised_by_the_product_itself(dtype, M, d):
+    x, W = wide(M, d, dtype, seed=d), quantize_rows(torch.randn(500, d, device="cuda"))
+    x[0, d - 1] = float("nan") if M > 1 else 3.0
+    b_dec = torch.randn(d + 1)
+    for c in (None, b_dec[:d].to(dtype).cuda(), b_dec.to(dtype).cuda()[1:], b_dec[:d].to(F16 if dtype == BF16 else BF16).cuda()):
+        rows8 = quantize_rows(x.cuda(), shift=c)
+        for out_dtype in (F32, BF16):
+            want = fused_encode_fp8(rows8, W, out_dtype=out_dtype)
+            got = fused_encode_fp8(x.cuda(), W, b_dec=c, out_dtype=out_dtype)
+            assert torch.equal(got.nan_to_num(-1.0), want.nan_to_num(-1.0))
+
+
 def test_calls_repeat_bit_for_bit_on_another_stream_and_in_a_graph():
     x, W = torch.randn(90, 700, device="cuda"), quantize_rows(torch.randn(2000, 700, device="cuda"))
     want = fused_encode_fp8(x, W)
