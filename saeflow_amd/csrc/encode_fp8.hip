@@ -13,9 +13,10 @@ using namespace sfenc;
 typedef SlimTile<1, 1, 1, 4, 8, 3> F8x32;    // 32 x 128
 typedef SlimTile<2, 1, 1, 4, 8, 3> F8x64;    // 64 x 128
 typedef SlimTile<2, 2, 2, 2, 8, 2> F8x128;   // 128 x 128
+typedef SlimTile<2, 1, 2, 4, 8, 4> F8x128one;  // 128 x 128, a CU to itself
 typedef SlimTile<1, 1, 1, 2, 8, 6> F8few;    // 32 x 64, tokens quantised in the kernel
 
-template <typename TL, bool FUSED = false>
+template <typename TL, bool FUSED = false, bool F32 = true>  // F32: fp32 results are asked of it
 hipError_t launch_tile(F8Args& a, hipStream_t s) {
   a.tiles_m = (int)((a.M + TL::TM - 1) / TL::TM);
   a.tiles_n = (int)((a.N + TL::TN - 1) / TL::TN);
@@ -23,8 +24,12 @@ hipError_t launch_tile(F8Args& a, hipStream_t s) {
   const dim3 grid(a.tiles_m * a.tiles_n), block(TL::NT);
   const bool plain = a.act != SF_ACT_JUMPRELU && !a.row_nnz;
   if (a.out_dt == SF_F32) {
-    if (plain) hipLaunchKernelGGL((gemm_f8_kernel<TL, true, true, FUSED>), grid, block, 0, s, a);
-    else hipLaunchKernelGGL((gemm_f8_kernel<TL, true, false, FUSED>), grid, block, 0, s, a);
+    if constexpr (F32) {
+      if (plain) hipLaunchKernelGGL((gemm_f8_kernel<TL, true, true, FUSED>), grid, block, 0, s, a);
+      else hipLaunchKernelGGL((gemm_f8_kernel<TL, true, false, FUSED>), grid, block, 0, s, a);
+    } else {
+      return hipErrorInvalidValue;
+    }
   } else {
     if (plain) hipLaunchKernelGGL((gemm_f8_kernel<TL, false, true, FUSED>), grid, block, 0, s, a);
     else hipLaunchKernelGGL((gemm_f8_kernel<TL, false, false, FUSED>), grid, block, 0, s, a);
@@ -101,9 +106,10 @@ struct Tokens {
 
 // Estimated time of a product in us with tiles of tm x tn: a fixed part, and for each round of tiles over
 // the CUs a part per block of K (`alone` times that with one workgroup a CU) and one per tile; at least
-// the bytes at the rate that the shape streams them. Fitted to 176 shapes of 1 to 4096 tokens, d_in 256 to
-// 4096, 4096 to 131072 features, in both result sizes: the pick is 0.9% slower than the best of the
-// four in the mean, 17% at most. Where each wins at d_in 2304, d_sae 65536, bf16 (us of the four in order):
+// the bytes at the rate that the shape streams them. Fitted to 220 shapes of 1 to 4096 tokens, d_in 256 to
+// 4096, 4096 to 131072 features, in both result sizes: the pick is 1.2% (fp32 0.7%) slower than the best in
+// the mean, 22% at most. Where each of the first four wins at d_in 2304, d_sae 65536, bf16 (us in
+// order):
 // 32 tokens 26 24 25 33 (d_sae 16384: 10 11 18 27), 128 tokens 58 33 28 36, 256 tokens 108 59 47 40, 4096
 // tokens 1690 880 710 525; fp32 results of 128 tokens 62 49 42 62, of 256 118 94 81 70, of 4096 1750 1370 1140
 // 1040.
@@ -111,13 +117,18 @@ struct Shape {
   int tm, tn;
   float fixed, step, alone, tile, tail, tbs;
 };
-constexpr Shape SHAPES[2][4] = {
+constexpr Shape SHAPES[2][5] = {
     // 16-bit results
-    {{32, 128, 2.48f, 0.206f, 1.27f, 1.00f, 0.39f, 5.95f}, {64, 128, 2.28f, 0.295f, 1.38f, 1.26f, 0.42f, 6.54f},
-     {128, 128, 1.52f, 0.469f, 1.65f, 1.94f, 0.39f, 6.22f}, {256, 256, 3.10f, 1.346f, 0.76f, 6.38f, 0.27f, 5.11f}},
+    {{32, 128, 2.14f, 0.215f, 1.64f, 1.06f, 0.41f, 6.65f}, {64, 128, 2.12f, 0.299f, 1.34f, 1.41f, 0.34f, 6.71f},
+     {128, 128, 1.59f, 0.489f, 1.57f, 1.85f, 0.38f, 5.14f}, {256, 256, 3.19f, 1.568f, 0.64f, 4.75f, 0.35f, 6.15f},
+     {128, 128, 1.63f, 0.520f, 0.81f, 2.30f, 0.23f, 6.67f}},
     // fp32 results
-    {{32, 128, 2.06f, 0.326f, 1.46f, 1.27f, 0.60f, 6.30f}, {64, 128, 1.84f, 0.510f, 1.26f, 1.83f, 0.37f, 5.50f},
-     {128, 128, 1.61f, 0.851f, 1.16f, 2.38f, 0.50f, 4.84f}, {256, 256, 0.04f, 2.986f, 0.73f, 9.65f, 0.27f, 3.53f}}};
+    {{32, 128, 2.38f, 0.323f, 1.34f, 1.20f, 0.41f, 7.04f}, {64, 128, 2.26f, 0.500f, 1.18f, 1.77f, 0.35f, 6.39f},
+     {128, 128, 1.46f, 0.815f, 1.20f, 2.57f, 0.41f, 4.16f}, {256, 256, 3.24f, 3.008f, 0.68f, 7.84f, 0.09f, 3.83f}, {}}};
+// The fifth, 128 x 128 with eight waves and four stages, has a CU to itself: for one round of 16-bit
+// results only (d_in 4096, d_sae 12288, 256 tokens 18 us against 23 with 64 x 128; from two rounds on two
+// workgroups a CU win).
+constexpr int ONE_ROUND = 4;
 // What result rows off 16 B cost a 256x256 tile (d_in 1000 and 1024: 319 us for 5303 tokens over 49153 features,
 // 128x128 tiles 357; 72 for 4096 over 10007, 128x128 tiles 62).
 constexpr float UNALIGNED_TILE = 3.f;
@@ -127,9 +138,10 @@ int pick_shape(int64_t M, int64_t N, int64_t K, int out_dt, bool unaligned) {
   const double bytes = (double)N * K + (double)M * K + (double)M * N * sf_dtype_size(out_dt);
   int best = -1;
   double least = 0;
-  for (int i = 0; i < 4; ++i) {
+  for (int i = 0; i < (wide ? 4 : 5); ++i) {
     const Shape& h = SHAPES[wide][i];
     const double x = (double)((M + h.tm - 1) / h.tm) * (double)((N + h.tn - 1) / h.tn) / 256;
+    if (i == ONE_ROUND && x > 1) continue;
     const double rounds = x <= 1 ? 1 : (x < 3 ? ceil(x) : x + h.tail);
     const double tile = h.tile + (i == 3 && unaligned ? UNALIGNED_TILE : 0.f);
     const double t = std::max(h.fixed + (nb * h.step * (x <= 1 ? h.alone : 1) + tile) * rounds,
@@ -170,6 +182,7 @@ int product(const char* fn, const Tokens* tokens, const void* xq, int64_t sxq, c
       case 0: e = launch_tile<F8x32>(a, s); break;
       case 1: e = launch_tile<F8x64>(a, s); break;
       case 2: e = launch_tile<F8x128>(a, s); break;
+      case ONE_ROUND: e = launch_tile<F8x128one, false, false>(a, s); break;
       default: e = launch_persist(a, ctr, cleared, s); break;
     }
   }

@@ -167,7 +167,7 @@ def whole(R, d, seed, top=3):
 # few tokens and many, panels cut short, blocks cut short, more blocks than LDS holds scales for, odd d_sae
 SHAPES = [(1, 64, 128), (1, 257, 2304), (7, 1000, 129), (32, 4099, 768), (33, 130, 4096), (100, 777, 1000),
           (137, 2048, 1), (128, 512, 4224), (250, 1001, 8320), (1000, 10007, 256), (16, 100, 8448), (515, 65536, 300),
-          (2048, 16384, 130), (2000, 16391, 127), (4099, 8200, 4352)]
+          (2048, 16384, 130), (2000, 16391, 127), (4099, 8200, 4352), (200, 12291, 2304), (250, 12288, 4352)]
 
 
 @pytest.mark.parametrize("M,N,K", SHAPES)
