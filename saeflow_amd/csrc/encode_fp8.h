@@ -153,6 +153,11 @@ __device__ __forceinline__ void tile_epilogue(const Out& a, int out_dt, f32x16 (
 // pipeline and its waits are gemm_slim_kernel's. The scale bytes of the tile's rows lie in LDS as [group of
 // four blocks][row] dwords, loaded for 4096 elements of K at a time.
 //
+// Bound by the pass over W where tokens are few (32 tokens over 65536 features of d_in 2304, bf16: 24 us, 6.3
+// TB/s), by the latency of a K-step where tiles are one round, by LDS where they are
+// many (waves of 64x64 read 8 KB for four MFMAs of 64 cycles, four such waves all of LDS's 128 B a cycle: 4096
+// tokens, 128x128 tiles, 710 us, 1.74 PFLOP/s).
+//
 // FUSED (tokens of at most FUSED_BLOCKS blocks in all): the tokens come as they are; each workgroup, its
 // first stages of W under way, quantises all of them into LDS, where they stay, and a launch is saved.
 constexpr int FUSED_BLOCKS = 32;
@@ -433,14 +438,14 @@ __device__ __forceinline__ void dma4(__amdgpu_buffer_rsrc_t r, char* wave_base, 
   __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (lds_void*)wave_base, 4, (int)voff, (int)soff, 0, 0);
 }
 
-// Three bf16 pieces of a fp32 value, whose sum it is (8 significant bits each; a lone first piece for
-// infinities and NaN), as two dwords.
+// Three bf16 pieces of a fp32 value, whose sum it is (8 significant bits each, cut off, so that none passes the
+// value; a lone first piece for infinities and NaN), as two dwords.
 __device__ __forceinline__ sfenc::u32x2 pieces(float v) {
-  const float p0 = bf16_to_f32(f32_to_bf16(v));
-  const float r = v - p0;
-  const bool fine = r == r && fabsf(p0) < __builtin_inff();
-  const float p1 = bf16_to_f32(f32_to_bf16(r));
-  return sfenc::u32x2{f32_to_bf16(v) | (fine ? f32_to_bf16(r) << 16 : 0u), fine ? f32_to_bf16(r - p1) : 0u};
+  const uint32_t u = __float_as_uint(v);
+  const bool fine = fabsf(v) < __builtin_inff();
+  const float r = v - __uint_as_float(u & 0xffff0000u);
+  const uint32_t p1 = __float_as_uint(r) & 0xffff0000u, p2 = __float_as_uint(r - __uint_as_float(p1)) >> 16;
+  return sfenc::u32x2{fine ? u >> 16 | p1 : f32_to_bf16(v), fine ? p2 : 0u};
 }
 
 // Epilogue of a wave's 128x128 tile of 16-bit results at token m0, feature n0, through 16 KiB of LDS, two
@@ -541,7 +546,10 @@ __device__ __forceinline__ void f8_epilogue(const Out& a, f32x16 (&acc)[4][4], i
 //              DMAs of block kt + 2 go into it at once, a whole K-step before they are awaited.
 //   X(kt + 1)  16 MFMAs on the second half of kt, the first half of kt + 1 read under them.
 // The order of MFMAs, LDS reads and DMAs is pinned (a scheduling barrier after each MFMA): left to itself
-// the compiler puts all reads of a half before its first MFMA. An odd number of blocks is rounded
+// the compiler puts all reads of a half before its first MFMA (16384 x 2304 x 65536, bf16 results: 1.67
+// PFLOP/s so, 2.58 pinned, 1920 us). Bound there by the power limit: the matrix cores are busy 66% of 1.78 GHz,
+// waves wait 15% of their time, no LDS bank conflicts; fp32 results (the wide form) take 2.0 times as long,
+// bound by the 16-bit instruction. An odd number of blocks is rounded
 // up; the one past the end reads zeros.
 template <int ODT, bool PLAIN>
 __global__ __launch_bounds__(256, 1) void gemm_f8_persist_kernel(F8Args a) {

@@ -39,8 +39,11 @@ class Fp8Rows:
         if q.device != scale.device:
             raise ValueError(f"codes are on {q.device}, scales on {scale.device}")
         self.q, self.scale, self.d = q, scale, d
-        # the C ABI's (codes, their stride, scales, their stride)
-        self._args = (q.data_ptr(), q.stride(0), scale.data_ptr(), scale.stride(0))
+        # the C ABI's (codes, their stride, scales, their stride); a lone row's stride is not used and may be
+        # anything
+        many = q.shape[0] > 1
+        self._args = (q.data_ptr(), q.stride(0) if many else q.shape[1],
+                      scale.data_ptr(), scale.stride(0) if many else scale.shape[1])
 
     @classmethod
     def empty(cls, rows, d, device="cuda"):
@@ -51,16 +54,21 @@ class Fp8Rows:
 
     @classmethod
     def from_parts(cls, codes, scale):
-        """Rows from codes [R, d] (float8_e4m3fn) and scale bytes [R, ceil(d / 128)], padded as needed."""
+        """Rows from codes [R, d] (float8_e4m3fn) and scale bytes [R, ceil(d / 128)], copied where they are
+        not padded and aligned as rows are held."""
         if codes.dtype != torch.float8_e4m3fn or codes.dim() != 2:
             raise ValueError(f"codes must be a float8_e4m3fn matrix, got {codes.dtype} {list(codes.shape)}")
         R, d = codes.shape
         kp, sp = _up(d, BLOCK), _up(_up(d, BLOCK) // BLOCK, 4)
         if scale.shape != (R, kp // BLOCK):
             raise ValueError(f"codes {tuple(codes.shape)} need scales of shape {(R, kp // BLOCK)}, got {tuple(scale.shape)}")
-        if kp != d or codes.stride(1) != 1:
-            codes = torch.nn.functional.pad(codes.view(torch.uint8), (0, kp - d)).view(torch.float8_e4m3fn)
-        return cls(codes, torch.nn.functional.pad(scale, (0, sp - kp // BLOCK)), d)
+        if kp != d or codes.stride(1) != 1 or codes.stride(0) % 16 or codes.data_ptr() % 16:
+            padded = torch.zeros(R, kp, dtype=torch.uint8, device=codes.device)
+            padded[:, :d] = codes.view(torch.uint8)
+            codes = padded.view(torch.float8_e4m3fn)
+        scales = torch.zeros(R, sp, dtype=scale.dtype, device=scale.device)
+        scales[:, :kp // BLOCK] = scale
+        return cls(codes, scales, d)
 
     @property
     def shape(self):

@@ -233,6 +233,73 @@ def test_smallest_and_largest_scales_in_the_product(out_dtype):
         assert torch.equal(got.cpu(), w.to(F32).to(out_dtype))
 
 
+def test_product_past_four_gigabytes():
+    """Operands and results whose offsets pass 32 bits, through narrow and wide tiles."""
+    R, d = (1 << 25) + 40, 128
+    W = Fp8Rows.empty(R, d)  # 4.3 GB of codes
+    W.q.view(torch.uint8).zero_()
+    W.scale.fill_(127)
+    tail, tv = whole(300, d, 5)
+    W.q[R - 300:].view(torch.uint8).copy_(tail.q.view(torch.uint8))
+    W.scale[R - 300:] = tail.scale
+    x, xv = whole(300, d, 6)
+    want = (xv @ tv.T.contiguous()).float()
+    for M, dtype in ((1, BF16), (33, F32)):
+        got = fused_encode_fp8(x[:M], W, activation="none", out_dtype=dtype)
+        assert torch.equal(got[:, R - 300:], want[:M].to(dtype)) and not got[:, R - 900:R - 300].any()
+        del got
+    sparse = Fp8Rows(W.q.view(R // 8, 8 * 128)[:, :128], W.scale.view(R // 8, 32)[:, :4], d)  # rows 1 KB apart
+    wide_rows = Fp8Rows(sparse.q[::16], sparse.scale[::16], d)  # and 16 KB
+    n = len(wide_rows)
+    wide_rows.q[n - 300:].view(torch.uint8).copy_(tail.q.view(torch.uint8))
+    wide_rows.scale[n - 300:] = tail.scale
+    for M in (1, 40, 100, 300):
+        for dtype in (BF16, F32):
+            got = fused_encode_fp8(x[:M], wide_rows, activation="none", out_dtype=dtype)
+            assert torch.equal(got[:, n - 300:], want[:M].to(dtype))
+            got = fused_encode_fp8(wide_rows[n - 300:], x[:M], activation="none", out_dtype=dtype)
+            assert torch.equal(got, want[:M].T.to(dtype))
+    del W, sparse, wide_rows, got
+    x, xv = whole(9000, d, 7)
+    W, wv = whole(131072, d, 8)  # 4.7 GB of fp32 results, 2.4 GB of bf16
+    for dtype in (F32, BF16):
+        got = fused_encode_fp8(x, W, activation="none", out_dtype=dtype)
+        for m in (0, 4000, 8900):
+            assert torch.equal(got[m:m + 100], (xv[m:m + 100] @ wv.T.contiguous()).to(dtype))
+
+
+def test_one_row_of_any_stride():
+    """A lone row's stride addresses nothing."""
+    W, wv = whole(70, 256, 9)
+    x, xv = whole(3, 256, 10)
+    one = Fp8Rows(x.q.view(torch.uint8)[1].as_strided((1, 256), (1, 1)).view(torch.float8_e4m3fn),
+                  x.scale[1].as_strided((1, 4), (3, 1)), 256)
+    want = (xv[1:2] @ wv.T.contiguous()).float()
+    assert torch.equal(fused_encode_fp8(one, W, activation="none", out_dtype=F32), want)
+    assert torch.equal(dequantize_rows(one, out_dtype=F32).double(), xv[1:2])
+    # codes that lie off 16 B are laid out anew
+    codes = torch.zeros(3, 300, dtype=torch.uint8, device="cuda")
+    codes[:, 7:263] = x.q.view(torch.uint8)
+    moved = Fp8Rows.from_parts(codes[:, 7:263].view(torch.float8_e4m3fn), x.scale[:, :2])
+    assert torch.equal(fused_encode_fp8(moved, W, activation="none", out_dtype=F32), (xv @ wv.T.contiguous()).float())
+
+
+@pytest.mark.parametrize("M", [5, 300, 2048])
+def test_biases_up_to_the_largest_and_with_every_bit(M):
+    """A zero product plus a bias is the bias, whole, in fp32, at the largest finite and the smallest normal
+    magnitudes too."""
+    N = 16384
+    x, W = quantize_rows(torch.zeros(M, 200, device="cuda")), quantize_rows(torch.zeros(N, 200, device="cuda"))
+    g = torch.Generator().manual_seed(4)
+    b = (torch.rand(N, generator=g) + 1) * 2.0 ** torch.randint(-100, 127, (N,), generator=g) * torch.randn(N, generator=g).sign()
+    b[:4] = torch.tensor([torch.finfo(F32).max, -torch.finfo(F32).max, 0.0, float("inf")])
+    b = b.cuda()
+    got = fused_encode_fp8(x, W, b, activation="none", out_dtype=F32)
+    assert torch.equal(got, b.expand(M, N))
+    for dtype in (BF16, F16):
+        assert torch.equal(fused_encode_fp8(x, W, b, activation="none", out_dtype=dtype), b.to(dtype).expand(M, N))
+
+
 def test_fp32_results_are_as_good_as_fp32_sums():
     """Normal operands, K terms added one after the other in fp32: each of the K roundings is at most
     2^-24 of a partial sum no larger than a few standard deviations of the result, so the root mean
