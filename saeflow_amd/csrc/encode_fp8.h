@@ -153,10 +153,10 @@ __device__ __forceinline__ void tile_epilogue(const Out& a, int out_dt, f32x16 (
 // pipeline and its waits are gemm_slim_kernel's. The scale bytes of the tile's rows lie in LDS as [group of
 // four blocks][row] dwords, loaded for 4096 elements of K at a time.
 //
-// Bound by the pass over W where tokens are few (32 tokens over 65536 features of d_in 2304, bf16: 24 us, 6.3
-// TB/s), by the latency of a K-step where tiles are one round, by LDS where they are
-// many (waves of 64x64 read 8 KB for four MFMAs of 64 cycles, four such waves all of LDS's 128 B a cycle: 4096
-// tokens, 128x128 tiles, 710 us, 1.74 PFLOP/s).
+// Bound by the pass over W where tokens are few (32 tokens over 65536 features of d_in 2304, bf16: 25 us, 6.2
+// TB/s), by the latency of a K-step where tiles are one round, by that and LDS where they are many (128x128:
+// eight waves of 32x64 read 96 KB a K-step, 768 cycles of LDS and 512 of the matrix cores; 4096 tokens 690 us,
+// 1.79 PFLOP/s).
 //
 // FUSED (tokens of at most FUSED_BLOCKS blocks in all): the tokens come as they are; each workgroup, its
 // first stages of W under way, quantises all of them into LDS, where they stay, and a launch is saved.

@@ -9,10 +9,13 @@ namespace {
 using namespace sfenc;
 
 // The tiles, tokens x features, with the stages that leave room for two workgroups a CU: narrow ones for few
-// tokens, where the pass over W bounds the product, wider ones where the matrix cores do.
+// tokens, where the pass over W bounds the product, wider ones where the matrix cores do. Eight waves each from
+// 64 tokens on: 128x128 tiles with waves of 32x64 5.5% faster than four waves of 64x64 over 148 shapes
+// (128 tokens and more, 16-bit results; -18 to +4%), 64x128 with waves of 32x32 2.3% faster than four of 64x32.
+// fp32 results alike on average.
 typedef SlimTile<1, 1, 1, 4, 8, 3> F8x32;    // 32 x 128
-typedef SlimTile<2, 1, 1, 4, 8, 3> F8x64;    // 64 x 128
-typedef SlimTile<2, 2, 2, 2, 8, 2> F8x128;   // 128 x 128
+typedef SlimTile<1, 1, 2, 4, 8, 3> F8x64;    // 64 x 128
+typedef SlimTile<1, 2, 4, 2, 8, 2> F8x128;   // 128 x 128
 typedef SlimTile<2, 1, 2, 4, 8, 4> F8x128one;  // 128 x 128, a CU to itself
 typedef SlimTile<1, 1, 1, 2, 8, 6> F8few;    // 32 x 64, tokens quantised in the kernel
 
@@ -107,26 +110,25 @@ struct Tokens {
 // Estimated time of a product in us with tiles of tm x tn: a fixed part, and for each round of tiles over
 // the CUs a part per block of K (`alone` times that with one workgroup a CU) and one per tile; at least
 // the bytes at the rate that the shape streams them. Fitted to 220 shapes of 1 to 4096 tokens, d_in 256 to
-// 4096, 4096 to 131072 features, in both result sizes: the pick is 1.2% (fp32 0.7%) slower than the best in
-// the mean, 22% at most. Where each of the first four wins at d_in 2304, d_sae 65536, bf16 (us in
-// order):
-// 32 tokens 26 24 25 33 (d_sae 16384: 10 11 18 27), 128 tokens 58 33 28 36, 256 tokens 108 59 47 40, 4096
-// tokens 1690 880 710 525; fp32 results of 128 tokens 62 49 42 62, of 256 118 94 81 70, of 4096 1750 1370 1140
-// 1040.
+// 4096, 4096 to 131072 features, in both result sizes: the pick is 1.1% (fp32 0.4%) slower than the best in
+// the mean, 23% at most. Where each of the first four wins at d_in 2304, d_sae 65536, bf16 (us in
+// order): 32 tokens 25 25 25 31 (d_sae 16384: 10 11 16 26), 128 tokens 43 30 27 32, 256 tokens 80 59 44 37, 4096
+// tokens 1175 867 690 530; fp32 results of 128 tokens 60 49 41 61, of 256 117 97 78 67, of 4096 1717 1424 1155
+// 1041.
 struct Shape {
   int tm, tn;
   float fixed, step, alone, tile, tail, tbs;
 };
 constexpr Shape SHAPES[2][5] = {
     // 16-bit results
-    {{32, 128, 2.14f, 0.215f, 1.64f, 1.06f, 0.41f, 6.65f}, {64, 128, 2.12f, 0.299f, 1.34f, 1.41f, 0.34f, 6.71f},
-     {128, 128, 1.59f, 0.489f, 1.57f, 1.85f, 0.38f, 5.14f}, {256, 256, 3.19f, 1.568f, 0.64f, 4.75f, 0.35f, 6.15f},
-     {128, 128, 1.63f, 0.520f, 0.81f, 2.30f, 0.23f, 6.67f}},
+    {{32, 128, 2.27f, 0.215f, 1.61f, 0.94f, 0.40f, 6.66f}, {64, 128, 1.81f, 0.300f, 1.38f, 1.29f, 0.38f, 6.90f},
+     {128, 128, 1.16f, 0.472f, 1.47f, 1.77f, 0.30f, 5.50f}, {256, 256, 4.42f, 1.655f, 0.61f, 3.43f, 0.24f, 6.65f},
+     {128, 128, 1.20f, 0.487f, 0.84f, 2.78f, 0.14f, 6.72f}},
     // fp32 results
-    {{32, 128, 2.38f, 0.323f, 1.34f, 1.20f, 0.41f, 7.04f}, {64, 128, 2.26f, 0.500f, 1.18f, 1.77f, 0.35f, 6.39f},
-     {128, 128, 1.46f, 0.815f, 1.20f, 2.57f, 0.41f, 4.16f}, {256, 256, 3.24f, 3.008f, 0.68f, 7.84f, 0.09f, 3.83f}, {}}};
+    {{32, 128, 2.30f, 0.319f, 1.37f, 1.22f, 0.27f, 6.91f}, {64, 128, 2.02f, 0.534f, 1.06f, 1.70f, 0.14f, 6.53f},
+     {128, 128, 1.87f, 0.840f, 0.96f, 2.40f, 0.39f, 5.01f}, {256, 256, 0.f, 2.815f, 0.69f, 11.99f, 0.20f, 3.90f}, {}}};
 // The fifth, 128 x 128 with eight waves and four stages, has a CU to itself: for one round of 16-bit
-// results only (d_in 4096, d_sae 12288, 256 tokens 18 us against 23 with 64 x 128; from two rounds on two
+// results only (d_in 4096, d_sae 12288, 256 tokens 18 us against 21 with 64 x 128; from two rounds on two
 // workgroups a CU win).
 constexpr int ONE_ROUND = 4;
 // What result rows off 16 B cost a 256x256 tile (d_in 1000 and 1024: 319 us for 5303 tokens over 49153 features,
