@@ -131,9 +131,9 @@ constexpr Shape SHAPES[2][5] = {
 // results only (d_in 4096, d_sae 12288, 256 tokens 18 us against 21 with 64 x 128; from two rounds on two
 // workgroups a CU win).
 constexpr int ONE_ROUND = 4;
-// What result rows off 16 B cost a 256x256 tile (d_in 1000 and 1024: 319 us for 5303 tokens over 49153 features,
-// 128x128 tiles 357; 72 for 4096 over 10007, 128x128 tiles 62).
-constexpr float UNALIGNED_TILE = 3.f;
+// What result rows off 16 B cost a 256x256 tile (bf16: 4096 tokens of d_in 768 over 16391 features 92 us,
+// 128x128 tiles 79; 2048 of d_in 4096 over 12289 106, 128x128 tiles 121).
+constexpr float UNALIGNED_TILE = 4.f;
 
 int pick_shape(int64_t M, int64_t N, int64_t K, int out_dt, bool unaligned) {
   const int nb = (int)blocks_of(K), wide = out_dt == SF_F32;
