@@ -20,11 +20,16 @@ def _up(n, m):
     return -(-n // m) * m
 
 
+def _rows_of_bytes(q, scale, d):
+    return Fp8Rows(q.view(torch.float8_e4m3fn), scale, d)
+
+
 class Fp8Rows:
     """R rows of d elements in 8 bits: `q` [R, d rounded up to 128] float8_e4m3fn, zeros behind d, and
-    `scale` [R, ceil(d / 128) rounded up to 4] uint8. Slicing rows gives a view."""
+    `scale` [R, ceil(d / 128) rounded up to 4] uint8. Slicing rows gives a view. The three belong together, so
+    they are not assigned to; copies and pickles are made of them alone."""
 
-    __slots__ = ("q", "scale", "d", "_args")
+    __slots__ = ("q", "scale", "d")
 
     def __init__(self, q, scale, d):
         if q.dtype != torch.float8_e4m3fn or scale.dtype != torch.uint8:
@@ -38,12 +43,23 @@ class Fp8Rows:
             raise ValueError("codes and scales must be contiguous along a row")
         if q.device != scale.device:
             raise ValueError(f"codes are on {q.device}, scales on {scale.device}")
-        self.q, self.scale, self.d = q, scale, d
-        # the C ABI's (codes, their stride, scales, their stride); a lone row's stride is not used and may be
-        # anything
-        many = q.shape[0] > 1
-        self._args = (q.data_ptr(), q.stride(0) if many else q.shape[1],
-                      scale.data_ptr(), scale.stride(0) if many else scale.shape[1])
+        for name, value in (("q", q), ("scale", scale), ("d", d)):
+            object.__setattr__(self, name, value)
+
+    def __setattr__(self, name, value):
+        raise AttributeError(f"{name} of 8-bit rows is not assigned to; make new Fp8Rows")
+
+    def __reduce__(self):
+        # (the codes as bytes: torch has no plain pickles of float8 tensors)
+        return _rows_of_bytes, (self.q.view(torch.uint8), self.scale, self.d)
+
+    def _args(self):
+        """The C ABI's (codes, their stride, scales, their stride); a lone row's stride is not used and may be
+        anything."""
+        q, scale = self.q, self.scale
+        if q.shape[0] > 1:
+            return q.data_ptr(), q.stride(0), scale.data_ptr(), scale.stride(0)
+        return q.data_ptr(), q.shape[1], scale.data_ptr(), scale.shape[1]
 
     @classmethod
     def empty(cls, rows, d, device="cuda"):
@@ -138,7 +154,7 @@ def quantize_rows(x, *, shift=None, out=None, row0=0):
     with _lib.device(dev):
         rc = _lib.load().sf_quantize_rows(
             x.data_ptr(), sxm, sxk, _lib.dtype_code(x, "x"), None if shift is None else shift.data_ptr(),
-            0 if shift is None else _lib.dtype_code(shift, "shift"), M, d, *out._args, row0, out.q.shape[0],
+            0 if shift is None else _lib.dtype_code(shift, "shift"), M, d, *out._args(), row0, out.q.shape[0],
             _lib.stream(dev))
     if rc:
         _lib.check(rc)
@@ -171,7 +187,7 @@ def dequantize_rows(rows8, rows=None, *, row0=0, count=None, shift=None, out_dty
     if M == 0:
         return out
     with _lib.device(dev):
-        rc = _lib.load().sf_dequantize_rows(*rows8._args, R, ids, row0, at, code, M, d, out.data_ptr(), d, out_code,
+        rc = _lib.load().sf_dequantize_rows(*rows8._args(), R, ids, row0, at, code, M, d, out.data_ptr(), d, out_code,
                                             _lib.stream(dev))
     if rc:
         _lib.check(rc)
@@ -215,13 +231,13 @@ def fused_encode_fp8(x, W, b_enc=None, threshold=None, activation="relu", *, b_d
     if M == 0 or N == 0:
         return out
     lib = _lib.load()
-    tail = (*W._args, _lib.ptr(b_enc), 0 if b_enc is None else _lib.dtype_code(b_enc, "b_enc"), _lib.ptr(threshold),
+    tail = (*W._args(), _lib.ptr(b_enc), 0 if b_enc is None else _lib.dtype_code(b_enc, "b_enc"), _lib.ptr(threshold),
             0 if threshold is None else _lib.dtype_code(threshold, "threshold"), out.data_ptr(), N, code,
             _lib.ptr(row_nnz), M, N, d, ACTIVATIONS[activation])
     with _lib.device(dev):
         ws = torch.empty(_lib.fp8_workspace_bytes(0 if held else M, d), dtype=torch.uint8, device=dev)
         if held:
-            _lib.check(lib.sf_encode_fp8_rows(*x._args, *tail, ws.data_ptr(), ws.numel(), _lib.stream(dev)))
+            _lib.check(lib.sf_encode_fp8_rows(*x._args(), *tail, ws.data_ptr(), ws.numel(), _lib.stream(dev)))
         else:
             x_code = _lib.dtype_code(x, "x")
             _lib.check(lib.sf_encode_fp8(x.data_ptr(), x.stride(0), x.stride(1), x_code, _lib.ptr(b_dec),

@@ -1,7 +1,9 @@
 """CPU: the 64-bit definition of 8-bit rows against torch's own e4m3, Fp8Rows on the host, and what the
 wrappers and the C ABI refuse before anything reaches a GPU."""
 
+import copy
 import ctypes
+import pickle
 
 import numpy as np
 import pytest
@@ -50,6 +52,18 @@ def test_rows_on_the_host(d):
     part = r[1:4]
     assert len(part) == 3 and part.q.data_ptr() == r.q[1:].data_ptr()
     assert len(Fp8Rows.empty(0, d, "cpu")) == 0 and "x" in repr(r)
+
+
+def test_copies_and_pickles_hold_their_own_memory():
+    r = Fp8Rows(torch.randn(5, 256).to(torch.float8_e4m3fn), torch.randint(120, 130, (5, 4), dtype=torch.uint8), 200)
+    for other in (copy.deepcopy(r), pickle.loads(pickle.dumps(r))):
+        assert other.shape == r.shape and other.q.data_ptr() != r.q.data_ptr()
+        assert torch.equal(other.q.view(torch.uint8), r.q.view(torch.uint8)) and torch.equal(other.scale, r.scale)
+        assert other._args() == (other.q.data_ptr(), 256, other.scale.data_ptr(), 4)
+    for name, value in (("q", r.q[:3]), ("scale", r.scale[:3]), ("d", 100)):
+        with pytest.raises(AttributeError):
+            setattr(r, name, value)
+    assert len(r) == 5 and r.d == 200
 
 
 def test_bad_rows_are_refused():
