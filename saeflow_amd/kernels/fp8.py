@@ -29,7 +29,7 @@ class Fp8Rows:
     `scale` [R, ceil(d / 128) rounded up to 4] uint8. Slicing rows gives a view. The three belong together, so
     they are not assigned to; copies and pickles are made of them alone."""
 
-    __slots__ = ("q", "scale", "d")
+    __slots__ = ("q", "scale", "d", "_strides")
 
     def __init__(self, q, scale, d):
         if q.dtype != torch.float8_e4m3fn or scale.dtype != torch.uint8:
@@ -43,7 +43,9 @@ class Fp8Rows:
             raise ValueError("codes and scales must be contiguous along a row")
         if q.device != scale.device:
             raise ValueError(f"codes are on {q.device}, scales on {scale.device}")
-        for name, value in (("q", q), ("scale", scale), ("d", d)):
+        # a lone row's stride is not used and may be anything
+        strides = (q.stride(0), scale.stride(0)) if q.shape[0] > 1 else (q.shape[1], scale.shape[1])
+        for name, value in (("q", q), ("scale", scale), ("d", d), ("_strides", strides)):
             object.__setattr__(self, name, value)
 
     def __setattr__(self, name, value):
@@ -54,12 +56,9 @@ class Fp8Rows:
         return _rows_of_bytes, (self.q.view(torch.uint8), self.scale, self.d)
 
     def _args(self):
-        """The C ABI's (codes, their stride, scales, their stride); a lone row's stride is not used and may be
-        anything."""
-        q, scale = self.q, self.scale
-        if q.shape[0] > 1:
-            return q.data_ptr(), q.stride(0), scale.data_ptr(), scale.stride(0)
-        return q.data_ptr(), q.shape[1], scale.data_ptr(), scale.shape[1]
+        """The C ABI's (codes, their stride, scales, their stride)."""
+        sq, ss = self._strides
+        return self.q.data_ptr(), sq, self.scale.data_ptr(), ss
 
     @classmethod
     def empty(cls, rows, d, device="cuda"):
