@@ -35,6 +35,7 @@ struct F8Args : sfenc::GemmArgs {
   int x_dt, x_rows;  // x_rows: rows contiguous and 16-B aligned
   const void* shift;
   int shift_dt, shift_vec;
+  int stream;  // result rows begin on whole cache lines (Out)
 };
 
 constexpr int SG = 8;              // groups of four blocks whose scales LDS holds at a time
@@ -67,14 +68,28 @@ __device__ __forceinline__ int frag_feature(int i) { return (i & 4) * 4 + (i >> 
 // 16 B of a result row, at any element's address
 typedef sfenc::u32x4 u32x4_any __attribute__((aligned(2)));
 
-// What an epilogue writes to.
+// What an epilogue writes to. stream: rows begin on whole cache lines, and stores go past the caches; lines that
+// two stores share are put together in L2 instead.
+// Either kind of store for all rows (us, d_in 120 / 768 / 2304): past the caches 197 / 334 / 722 against 204 / 464 / 836
+// for 16000 tokens over 24576 features in bf16 with 256x256 tiles, 272 / 648 / 1428 against 350 / 712 / 1459 in fp32, but
+// 57 / 82 / 137 against 42 / 66 / 122 for 4096 tokens over 12936 in bf16.
 struct Out {
   char* out;
   int64_t som;
   int32_t* row_nnz;
   int64_t M, N;
-  int act;
+  int act, stream;
 };
+// (the empty asm keeps the compiler from making one ordinary store of the two)
+__device__ __forceinline__ void put16(const sfenc::u32x4& v, char* dst, int stream) {
+  if (stream) {
+    asm volatile("");
+    __builtin_nontemporal_store(v, (u32x4_any*)dst);
+    asm volatile("");
+  } else {
+    *(u32x4_any*)dst = v;
+  }
+}
 // Epilogue of a wave's (32 MB x 32 NB) tile at token m0, feature n0, 32 tokens at a time through `reg` (32
 // rows of 32 NB features, this wave's own), fragment rows in frag_feature order: 16-B stores at any
 // alignment, element by element only across the last feature. ES: bytes of a result.
@@ -133,7 +148,7 @@ __device__ __forceinline__ void tile_epilogue(const Out& a, int out_dt, f32x16 (
       const sfenc::u32x4 v = *(const sfenc::u32x4*)(reg + row * RB + ((unit ^ (row & (UPR - 1))) << 4));
       if (mb * 32 + row < rows) {
         if (unit * EPU + EPU <= cols) {
-          *(u32x4_any*)dst = v;
+          put16(v, dst, a.stream);
         } else {
 #pragma unroll
           for (int e = 0; e < EPU; ++e)
@@ -429,7 +444,7 @@ __global__ __launch_bounds__(TL::NT, TL::ST * TL::NS > 81920 ? (TL::NW + 3) / 4 
   constexpr int RG = 32 * NB * 32 * ES, WPS = ST / RG;  // staging bytes per wave, waves per buffer
   static_assert(NW <= 2 * WPS, "epilogue staging");
   char* reg = w < WPS ? s0 + w * RG : s1 + (w - WPS) * RG;
-  tile_epilogue<ES, MB, NB, PLAIN>(Out{(char*)a.out, a.som, a.row_nnz, a.M, a.N, a.act}, a.out_dt, acc, mw, nw, lane, st, reg);
+  tile_epilogue<ES, MB, NB, PLAIN>(Out{(char*)a.out, a.som, a.row_nnz, a.M, a.N, a.act, a.stream}, a.out_dt, acc, mw, nw, lane, st, reg);
 }
 
 
@@ -519,17 +534,26 @@ __device__ __forceinline__ void f8_epilogue(const Out& a, f32x16 (&acc)[4][4], i
         const int rl = (part * 8 + it) * 4 + lane / 16;
         v[it] = *(const sfenc::u32x4*)(reg + rl * 256 + ((unit ^ (rl & 15)) << 4));
       }
+      auto store = [&](auto put) {
 #pragma unroll
-      for (int it = 0; it < 8; ++it) {
-        const int rl = pass * 64 + (part * 8 + it) * 4;
-        if (!RAGGED || (rl + lane / 16 < rows && unit * 8 + 8 <= cols)) {
-          __builtin_nontemporal_store(v[it], (u32x4_any*)dst);
-        } else if (rl + lane / 16 < rows) {
+        for (int it = 0; it < 8; ++it) {
+          const int rl = pass * 64 + (part * 8 + it) * 4;
+          if (!RAGGED || (rl + lane / 16 < rows && unit * 8 + 8 <= cols)) {
+            put(v[it], (u32x4_any*)dst);
+          } else if (rl + lane / 16 < rows) {
 #pragma unroll
-          for (int e = 0; e < 8; ++e)
-            if (unit * 8 + e < cols) ((u16*)dst)[e] = (u16)(v[it][e >> 1] >> ((e & 1) * 16));
+            for (int e = 0; e < 8; ++e)
+              if (unit * 8 + e < cols) ((u16*)dst)[e] = (u16)(v[it][e >> 1] >> ((e & 1) * 16));
+          }
+          dst += 8 * som;
         }
-        dst += 8 * som;
+      };
+      if (a.stream) {  // (as put16)
+        asm volatile("");
+        store([](const sfenc::u32x4& x, u32x4_any* d) { __builtin_nontemporal_store(x, d); });
+        asm volatile("");
+      } else {
+        store([](const sfenc::u32x4& x, u32x4_any* d) { *d = x; });
       }
       __builtin_amdgcn_sched_barrier(0);
     }
@@ -908,7 +932,7 @@ __global__ __launch_bounds__(256, 1) void gemm_f8_persist_kernel(F8Args a) {
 #pragma unroll
       for (int i = 0; i < NMF; ++i) mma(F1, i);
     }
-    const Out out = {(char*)cold()->out, cold()->som, cold()->row_nnz, cold()->M, cold()->N, cold()->act};
+    const Out out = {(char*)cold()->out, cold()->som, cold()->row_nnz, cold()->M, cold()->N, cold()->act, cold()->stream};
     if (mw + 128 <= out.M && nw + 128 <= out.N) {
       if constexpr (WIDE) tile_epilogue<4, MB, NB, PLAIN>(out, SF_F32, acc, mw, nw, lane, s_thr[P] + wn * 128, B0 + w * 16384);
       else f8_epilogue<ODT, PLAIN, false>(out, acc, mw, nw, lane, s_thr[P] + wn * 128, B0 + w * 16384);

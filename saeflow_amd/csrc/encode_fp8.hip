@@ -131,9 +131,13 @@ constexpr Shape SHAPES[2][5] = {
 // results only (d_in 4096, d_sae 12288, 256 tokens 18 us against 21 with 64 x 128; from two rounds on two
 // workgroups a CU win).
 constexpr int ONE_ROUND = 4;
-// What result rows off 16 B cost a 256x256 tile (bf16: 4096 tokens of d_in 768 over 16391 features 92 us,
+// What result rows off 16 B cost a 256x256 tile (bf16, stored past the caches: 4096 tokens of d_in 768 over 16391 features 92 us,
 // 128x128 tiles 79; 2048 of d_in 4096 over 12289 106, 128x128 tiles 121).
 constexpr float UNALIGNED_TILE = 4.f;
+
+// Bytes of 16-bit results from which on 256x256 tiles store rows off whole lines past the caches too: 16000 tokens
+// over 12936 features (414 MB) 404 us so and 419 past the caches, over 16416 (525 MB) 571 and 494 (d_in 2304).
+constexpr double STREAM_FROM = 448e6;
 
 int pick_shape(int64_t M, int64_t N, int64_t K, int out_dt, bool unaligned) {
   const int nb = (int)blocks_of(K), wide = out_dt == SF_F32;
@@ -169,6 +173,7 @@ int product(const char* fn, const Tokens* tokens, const void* xq, int64_t sxq, c
   a.group_m = 1;
   a.group_n = 8;
   a.ksteps = (int)blocks_of(K);
+  a.stream = aligned(out, 128) && som * sf_dtype_size(out_dt) % 128 == 0;
   hipError_t e;
   if (tokens) {
     a.x = tokens->x; a.sxm = tokens->sxm; a.sxk = tokens->sxk; a.x_dt = tokens->x_dt;
@@ -179,6 +184,7 @@ int product(const char* fn, const Tokens* tokens, const void* xq, int64_t sxq, c
   } else {
     const int shape = pick_shape(M, N, K, out_dt, som * sf_dtype_size(out_dt) % 16 != 0 || !aligned(out, 16));
     const Shape& h = SHAPES[out_dt == SF_F32][shape];
+    if (shape == 3 && out_dt != SF_F32 && (double)M * N * 2 > STREAM_FROM) a.stream = 1;
     SF_REQUIRE(((M + h.tm - 1) / h.tm) * ((N + h.tn - 1) / h.tn) < (1ll << 23), "%s: too many tiles", fn);
     switch (shape) {
       case 0: e = launch_tile<F8x32>(a, s); break;

@@ -268,6 +268,19 @@ def test_product_past_four_gigabytes():
             assert torch.equal(got[m:m + 100], (xv[m:m + 100] @ wv.T.contiguous()).to(dtype))
 
 
+@pytest.mark.parametrize("M,N,out_dtype", [(16384, 16391, BF16), (16384, 16416, F16), (16384, 16384, BF16),
+                                           (4096, 12936, BF16), (4096, 12921, F16), (2048, 12921, F32),
+                                           (2048, 12928, F32), (300, 24640, F16), (300, 24600, BF16)])
+def test_results_of_rows_on_and_off_whole_lines(M, N, out_dtype):
+    """Rows that begin on cache lines and rows that do not, few bytes and many: small whole numbers, whose sums
+    (at most 9 * 130) are exact in fp32 and rounded once."""
+    g = torch.Generator(device="cuda").manual_seed(M + N)
+    x = torch.randint(-3, 4, (M, 130), generator=g, device="cuda").float()
+    W = torch.randint(-3, 4, (N, 130), generator=g, device="cuda").float()
+    got = fused_encode_fp8(quantize_rows(x), quantize_rows(W), activation="none", out_dtype=out_dtype)
+    assert torch.equal(got, (x @ W.T.contiguous()).to(out_dtype))
+
+
 def test_one_row_of_any_stride():
     """A lone row's stride addresses nothing."""
     W, wv = whole(70, 256, 9)
