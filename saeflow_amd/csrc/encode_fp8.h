@@ -284,7 +284,7 @@ __global__ __launch_bounds__(TL::NT, TL::ST * TL::NS > 81920 ? (TL::NW + 3) / 4 
   for (int i = t; i < TN; i += NT) {  // (TN <= NT, or each thread's one feature)
     const int64_t n = n0 + i;
     const float h = a.out_dt == SF_F32 ? 0.f : (a.out_dt == SF_BF16 ? 0x1p-126f : 0x1p-25f);
-    float tv = a.act == SF_ACT_NONE ? __builtin_nanf("") : h;
+    float tv = h;
     if (n >= a.N) {
       tv = __builtin_inff();
     } else if (a.act == SF_ACT_JUMPRELU) {
@@ -655,7 +655,7 @@ __global__ __launch_bounds__(256, 1) void gemm_f8_persist_kernel(F8Args a) {
     s_bias[slot][t] = bits_as_f32(r.bias, c->benc_dt);
     if constexpr (!PLAIN) {
       constexpr float h = ODT == SF_F32 ? 0.f : (ODT == SF_BF16 ? 0x1p-126f : 0x1p-25f);
-      float tv = c->act == SF_ACT_NONE ? __builtin_nanf("") : h;
+      float tv = h;
       if (t > T.rn) {
         tv = __builtin_inff();
       } else if (c->act == SF_ACT_JUMPRELU) {

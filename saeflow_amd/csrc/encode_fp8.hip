@@ -81,9 +81,10 @@ int check_rows(const char* fn, const char* what, const void* q, int64_t sq, cons
 }
 
 int check_call(const char* fn, const void* b_enc, int benc_dt, const void* thr, int thr_dt, const void* out,
-               int64_t som, int out_dt, int64_t M, int64_t N, int64_t K, int act) {
+               int64_t som, int out_dt, const int32_t* row_nnz, int64_t M, int64_t N, int64_t K, int act) {
   SF_REQUIRE(sf_valid_dtype(out_dt) && (!b_enc || sf_valid_dtype(benc_dt)), "%s: bad dtype code", fn);
   SF_REQUIRE(act == SF_ACT_RELU || act == SF_ACT_JUMPRELU || act == SF_ACT_NONE, "%s: bad activation %d", fn, act);
+  SF_REQUIRE(act != SF_ACT_NONE || !row_nnz, "%s: row counts need relu or jumprelu", fn);
   SF_REQUIRE(M >= 0 && N >= 0 && K >= 1, "%s: bad size (M=%lld N=%lld K=%lld)", fn, (long long)M, (long long)N,
              (long long)K);
   SF_REQUIRE(M <= INT32_MAX && N <= INT32_MAX && K <= (1 << 22), "%s: size too large (M=%lld N=%lld K=%lld)", fn,
@@ -208,7 +209,7 @@ extern "C" int sf_encode_fp8_rows(const void* xq, int64_t sxq, const void* xs, i
   using namespace sff8;
   static const char* fn = "sf_encode_fp8_rows";
   sf_clear_error();
-  if (const int rc = check_call(fn, b_enc, benc_dt, thr, thr_dt, out, som, out_dt, M, N, K, act)) return rc;
+  if (const int rc = check_call(fn, b_enc, benc_dt, thr, thr_dt, out, som, out_dt, row_nnz, M, N, K, act)) return rc;
   if (M == 0 || N == 0) return SF_OK;
   SF_REQUIRE(workspace && aligned(workspace, 16) && workspace_bytes >= TILE_CTR_BYTES,
              "%s: needs a 16-B aligned workspace of %lld bytes", fn, (long long)TILE_CTR_BYTES);
@@ -237,7 +238,7 @@ extern "C" int sf_encode_fp8(const void* x, int64_t sxm, int64_t sxk, int x_dt, 
   static const char* fn = "sf_encode_fp8";
   sf_clear_error();
   SF_REQUIRE(sf_valid_dtype(x_dt) && (!b_dec || sf_valid_dtype(bdec_dt)), "%s: bad dtype code", fn);
-  if (const int rc = check_call(fn, b_enc, benc_dt, thr, thr_dt, out, som, out_dt, M, N, K, act)) return rc;
+  if (const int rc = check_call(fn, b_enc, benc_dt, thr, thr_dt, out, som, out_dt, row_nnz, M, N, K, act)) return rc;
   if (M == 0 || N == 0) return SF_OK;
   SF_REQUIRE(x, "%s: x must not be NULL", fn);
   const int64_t sq = code_bytes(K), ss = scale_bytes(K);

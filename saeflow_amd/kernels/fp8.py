@@ -200,12 +200,14 @@ def fused_encode_fp8(x, W, b_enc=None, threshold=None, activation="relu", *, b_d
       (minus `b_dec` if given).
     W: Fp8Rows [d_sae, d_in], a row a feature (quantize_rows(W_enc.T)).
     activation: "relu", "none", or "jumprelu" with a per-feature `threshold` [d_sae].
-    out_dtype: x's own, bfloat16 for Fp8Rows. row_nnz: as in fused_encode.
+    out_dtype: x's own, bfloat16 for Fp8Rows. row_nnz: as in fused_encode; not with "none".
     """
     if activation not in ACTIVATIONS:
         raise ValueError(f"fused_encode_fp8 supports {list(ACTIVATIONS)}, got {activation!r}")
     if activation == "jumprelu" and threshold is None:
         raise ValueError("jumprelu needs a threshold")
+    if activation == "none" and row_nnz is not None:
+        raise ValueError("row counts need relu or jumprelu")
     held = isinstance(x, Fp8Rows)
     if not isinstance(W, Fp8Rows):
         raise ValueError("W must be Fp8Rows, a row a feature: quantize_rows(W_enc.T)")

@@ -169,3 +169,20 @@ def test_c_abi_refuses_before_any_launch():
     refused(tok(bd=p, bdt=4), b"dtype")
     refused(tok(x=None), b"NULL")
     refused(tok(nbytes=100 * 260), b"workspace")
+
+
+@pytest.mark.parametrize("M,N", [(4, 10), (0, 10), (4, 0)])
+def test_counts_without_an_activation_are_refused(M, N):
+    """Bare pre-activations have no nonzeros to count: refused as sf_encode refuses it, before any launch."""
+    lib, p = _lib.load(), 4096  # (an address that is never used)
+
+    def tail(act):
+        return (p, 256, p, 4, None, 0, None, 0, p, 10, 1, p, M, N, 200, act, p, 1 << 20, None)
+
+    for call, x in ((lib.sf_encode_fp8_rows, (p, 256, p, 4)), (lib.sf_encode_fp8, (p, 200, 1, 1, None, 0))):
+        assert call(*x, *tail(_lib.ACT["none"])) == _lib.SF_EINVAL
+        assert b"row counts need relu or jumprelu" in lib.sf_last_error()
+    x, W, nnz = torch.randn(M, 200), host_rows(N, 200), torch.zeros(M, dtype=torch.int32)
+    for rows in (x, host_rows(M, 200)):
+        with pytest.raises(ValueError, match="row counts need relu or jumprelu"):
+            fused_encode_fp8(rows, W, activation="none", row_nnz=nnz)
