@@ -18,7 +18,7 @@ import torch
 
 from . import _lib
 from .kernels import dense_to_csr, fixed_width_to_dense, topk_rows
-from .kernels.fp8 import Fp8Rows, _vector, dequantize_rows, fused_encode_fp8, quantize_rows
+from .kernels.fp8 import Fp8Rows, _vector, dequantize_rows, fused_encode_fp8, quantize_rows, read_rows
 from .sae import ACTIVATIONS
 
 
@@ -64,9 +64,9 @@ class ActivationBuffer:
 
     def read(self, rows=None, *, out_dtype=torch.bfloat16):
         """Rows as out_dtype [n, d]: those of an int64 tensor of ids on the GPU (which are not checked: one
-        past the capacity reads as zeros), of a pair as write returns it, or, by default, all written."""
+        that no row has been written to reads as zeros), of a pair as write returns it, or, by default, all written."""
         if torch.is_tensor(rows):
-            return dequantize_rows(self.store, rows, shift=self.center, out_dtype=out_dtype)
+            return read_rows(self.store, self._filled, rows, 0, None, self.center, out_dtype)
         row0, count = (0, len(self)) if rows is None else rows
         if count < 0 or not 0 <= row0 < self.capacity or count > len(self) or (row0 + count > len(self) < self.capacity):
             raise ValueError(f"{count} rows from {row0} on are not among the {len(self)} written")

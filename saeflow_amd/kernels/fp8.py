@@ -164,7 +164,12 @@ def dequantize_rows(rows8, rows=None, *, row0=0, count=None, shift=None, out_dty
     """Rows read back, plus `shift` [d] if given (the sum in fp32, then rounded to out_dtype): those with
     the ids `rows` (int64, in any order; an id outside the store gives zeros), or `count` rows from row0 on,
     going on at row 0 behind the last (all of them by default)."""
-    R, d = rows8.q.shape[0], rows8.d
+    return read_rows(rows8, rows8.q.shape[0], rows, row0, count, shift, out_dtype)
+
+
+def read_rows(rows8, R, rows, row0, count, shift, out_dtype):
+    """dequantize_rows of a store of which only the first R rows have been written."""
+    d = rows8.d
     if rows is not None:
         if rows.dtype != torch.int64 or rows.dim() != 1:
             raise ValueError(f"rows must be a one-dimensional int64 tensor, got {rows.dtype} {list(rows.shape)}")
@@ -185,6 +190,8 @@ def dequantize_rows(rows8, rows=None, *, row0=0, count=None, shift=None, out_dty
     out_code = _lib.dtype_code(out, "out_dtype")
     if M == 0:
         return out
+    if R == 0:  # no id has a row
+        return out.zero_()
     with _lib.device(dev):
         rc = _lib.load().sf_dequantize_rows(*rows8._args(), R, ids, row0, at, code, M, d, out.data_ptr(), d, out_code,
                                             _lib.stream(dev))

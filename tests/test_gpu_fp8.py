@@ -544,3 +544,32 @@ def test_refusals():
             bad()
     with pytest.raises(TypeError):
         W[3]
+
+
+@pytest.mark.parametrize("centered", [False, True])
+def test_ids_of_rows_not_written_yet_read_as_zeros(centered):
+    """An id between the rows written and the capacity has no row: zeros, as for an id past the capacity,
+    whatever the memory behind it holds."""
+    center = torch.randn(130, device="cuda") if centered else None
+    buf = saeflow_amd.ActivationBuffer(100, 130, center=center)
+    buf.store.q.view(torch.uint8).fill_(0x7F)  # NaN codes
+    buf.store.scale.fill_(130)
+    ids = torch.tensor([69, 70, 0, 99, 100, -1, 5], device="cuda")
+    assert torch.equal(buf.read(ids, out_dtype=F32), torch.zeros(7, 130, device="cuda"))
+    assert buf.read(ids[:0]).shape == (0, 130)
+    for bad in (ids.int(), ids[None], ids.cpu()):
+        with pytest.raises(ValueError):
+            buf.read(bad)
+    x = torch.randn(130, 130, device="cuda")
+    held = dequantize_rows(quantize_rows(x, shift=center), shift=center, out_dtype=F32)
+    buf.write(x[:70])
+    want = held[ids.clamp(0, 69)]
+    want[[1, 3, 4, 5]] = 0
+    assert torch.equal(buf.read(ids, out_dtype=F32), want)
+    assert torch.equal(buf.read(out_dtype=F32), held[:70])
+    buf.write(x[70:100])  # full from here on
+    want = held[ids.clamp(0, 99)]
+    want[[4, 5]] = 0
+    assert torch.equal(buf.read(ids, out_dtype=F32), want)
+    buf.write(x[100:])
+    assert torch.equal(buf.read(ids, out_dtype=F32)[2], held[100])
