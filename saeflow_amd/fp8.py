@@ -35,7 +35,7 @@ class ActivationBuffer:
             raise ValueError(f"a buffer needs rows and a width, got {rows} x {d}")
         self.center = None if center is None else _vector(center.detach(), d, "center").clone()
         self.store = Fp8Rows.empty(rows, d, device)
-        _lib.require_gpu(("the buffer", self.store.q), ("center", self.center))
+        self._device = _lib.require_gpu(("the buffer", self.store.q), ("center", self.center))
         self._next, self._filled = 0, 0
 
     @property
@@ -51,12 +51,17 @@ class ActivationBuffer:
 
     def write(self, x):
         """Appends x [M, d], M <= capacity, over the oldest rows once the ring is full. Returns (first
-        row, M), which read takes."""
+        row, M), which read takes. Not while a graph is captured: the ring's place is kept on the host."""
         M = x.shape[0]
         if M > self.capacity:
             raise ValueError(f"{M} rows do not fit a buffer of {self.capacity}")
+        with _lib.device(self._device):
+            # (replays would write the same rows over and over, and rows only captured would count as written)
+            if torch._C._cuda_isCurrentStreamCapturing():
+                raise RuntimeError("ActivationBuffer.write cannot be captured in a graph; quantize_rows(out=, row0=) "
+                                   "writes to fixed rows")
         at = self._next
-        quantize_rows(x.detach(), shift=self.center, out=self.store, row0=at)
+        quantize_rows(x, shift=self.center, out=self.store, row0=at)
         self._next = (at + M) % self.capacity
         # in order from row 0 on, so the written rows are the first ones until the ring is full
         self._filled = min(self._filled + M, self.capacity)
@@ -64,7 +69,8 @@ class ActivationBuffer:
 
     def read(self, rows=None, *, out_dtype=torch.bfloat16):
         """Rows as out_dtype [n, d]: those of an int64 tensor of ids on the GPU (which are not checked: one
-        that no row has been written to reads as zeros), of a pair as write returns it, or, by default, all written."""
+        that no row has been written to reads as zeros), of a pair as write returns it, or, by default, all written.
+        Captured in a graph, a read knows the rows that were written by then."""
         if torch.is_tensor(rows):
             return read_rows(self.store, self._filled, rows, 0, None, self.center, out_dtype)
         row0, count = (0, len(self)) if rows is None else rows

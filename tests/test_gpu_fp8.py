@@ -573,3 +573,25 @@ def test_ids_of_rows_not_written_yet_read_as_zeros(centered):
     assert torch.equal(buf.read(ids, out_dtype=F32), want)
     buf.write(x[100:])
     assert torch.equal(buf.read(ids, out_dtype=F32)[2], held[100])
+
+
+def test_a_write_is_refused_while_a_graph_is_captured():
+    """The ring's place is the host's: replays would write the same rows over and over, and rows that were
+    only captured would count as written. Reading may be captured."""
+    buf = saeflow_amd.ActivationBuffer(50, 130)
+    x = torch.randn(60, 130, device="cuda")
+    held = dequantize_rows(quantize_rows(x), out_dtype=F32)
+    buf.write(x[:20])
+    ids = torch.arange(8, device="cuda")
+    buf.read(ids, out_dtype=F32)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        with pytest.raises(RuntimeError, match="captured"):
+            buf.write(x[20:30])
+        out = buf.read(ids, out_dtype=F32)
+    assert len(buf) == 20 and buf.write(x.requires_grad_()[20:60]) == (20, 40) and len(buf) == 50
+    for i in range(3):
+        ids.copy_(torch.randperm(20, device="cuda")[:8])
+        graph.replay()
+        assert torch.equal(out, buf.read(ids, out_dtype=F32))
+        assert torch.equal(out, torch.cat([held[50:60], held[10:20]])[ids])
