@@ -283,7 +283,9 @@ __global__ __launch_bounds__(TL::NT, TL::ST * TL::NS > 81920 ? (TL::NW + 3) / 4 
   if constexpr (NS > 5) issue(4, s4);
   for (int i = t; i < TN; i += NT) {  // (TN <= NT, or each thread's one feature)
     const int64_t n = n0 + i;
-    const float h = a.out_dt == SF_F32 ? 0.f : (a.out_dt == SF_BF16 ? 0x1p-126f : 0x1p-25f);
+    // keep-threshold: the largest value that rounds to zero in the result's type (subnormals of bf16 are kept, as
+    // PLAIN keeps them), or the feature's own
+    const float h = a.out_dt == SF_F32 ? 0.f : (a.out_dt == SF_BF16 ? 0x1p-134f : 0x1p-25f);
     float tv = h;
     if (n >= a.N) {
       tv = __builtin_inff();
@@ -454,7 +456,8 @@ __device__ __forceinline__ void dma4(__amdgpu_buffer_rsrc_t r, char* wave_base, 
 }
 
 // Three bf16 pieces of a fp32 value, whose sum it is (8 significant bits each, cut off, so that none passes the
-// value; a lone first piece for infinities and NaN), as two dwords.
+// value; a lone first piece for infinities and NaN; what lies below bf16's smallest subnormal 2^-133 is lost, which
+// concerns values below 2^-109), as two dwords.
 __device__ __forceinline__ sfenc::u32x2 pieces(float v) {
   const uint32_t u = __float_as_uint(v);
   const bool fine = fabsf(v) < __builtin_inff();
@@ -637,7 +640,7 @@ __global__ __launch_bounds__(256, 1) void gemm_f8_persist_kernel(F8Args a) {
     T.rn = (int)min((int64_t)BN, c->N - T.n0) - 1;
     return T;
   };
-  // Bias and keep-threshold (as gemm_kernel forms it) of feature t of a tile: raw bits, loaded while the
+  // Bias and keep-threshold (as gemm_f8_kernel forms it) of feature t of a tile: raw bits, loaded while the
   // tile before ends, and their values in LDS, read past the tile's first barrier.
   struct Raw {
     uint32_t bias, thr;
@@ -654,7 +657,7 @@ __global__ __launch_bounds__(256, 1) void gemm_f8_persist_kernel(F8Args a) {
     const auto c = cold();
     s_bias[slot][t] = bits_as_f32(r.bias, c->benc_dt);
     if constexpr (!PLAIN) {
-      constexpr float h = ODT == SF_F32 ? 0.f : (ODT == SF_BF16 ? 0x1p-126f : 0x1p-25f);
+      constexpr float h = ODT == SF_F32 ? 0.f : (ODT == SF_BF16 ? 0x1p-134f : 0x1p-25f);
       float tv = h;
       if (t > T.rn) {
         tv = __builtin_inff();

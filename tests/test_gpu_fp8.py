@@ -595,3 +595,26 @@ def test_a_write_is_refused_while_a_graph_is_captured():
         graph.replay()
         assert torch.equal(out, buf.read(ids, out_dtype=F32))
         assert torch.equal(out, torch.cat([held[50:60], held[10:20]])[ids])
+
+
+@pytest.mark.parametrize("out_dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("M", [1, 20, 300, 2048])
+def test_the_smallest_features_are_the_same_with_counts_and_without(M, out_dtype):
+    """A zero product plus a bias down to the smallest subnormal: what the result's type holds of it is stored and
+    counted, by every form alike."""
+    N = 16384
+    x, W = quantize_rows(torch.zeros(M, 200, device="cuda")), quantize_rows(torch.zeros(N, 200, device="cuda"))
+    b = torch.zeros(N, dtype=torch.float64)
+    b[:150] = 2.0 ** -torch.arange(150).double()
+    b[150:300] = 2.0 ** -torch.arange(150).double() * 1.25
+    b[300:450] = -b[:150]
+    b = b.float().cuda()
+    f = fused_encode_fp8(x, W, b, out_dtype=out_dtype)
+    held = b.double() == b.to(BF16).double()  # (the largest tiles take a bias in bf16 pieces)
+    assert torch.equal(f[:, held], b.clamp(min=0).to(out_dtype)[held].expand(M, -1))
+    for thr, act in ((None, "relu"), (torch.zeros(N, device="cuda"), "jumprelu"), (b.abs(), "jumprelu")):
+        nnz = torch.zeros(M, dtype=torch.int32, device="cuda")
+        got = fused_encode_fp8(x, W, b, thr, act, out_dtype=out_dtype, row_nnz=nnz)
+        want = torch.zeros_like(f) if thr is not None and thr.any() else f
+        assert torch.equal(got, want) and torch.equal(nnz, (want != 0).sum(1, dtype=torch.int32))
+        assert torch.equal(fused_encode_fp8(x, W, b, thr, act, out_dtype=out_dtype), want)
