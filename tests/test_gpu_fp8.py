@@ -618,3 +618,85 @@ def test_the_smallest_features_are_the_same_with_counts_and_without(M, out_dtype
         want = torch.zeros_like(f) if thr is not None and thr.any() else f
         assert torch.equal(got, want) and torch.equal(nnz, (want != 0).sum(1, dtype=torch.int32))
         assert torch.equal(fused_encode_fp8(x, W, b, thr, act, out_dtype=out_dtype), want)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("activation", ["relu", "jumprelu", "topk"])
+def test_sparse_features_of_large_products(activation, dtype):
+    """CSR out of the persistent tiles: 2300 tokens x 16200 features, rows without features and rows of NaN among
+    them, against the dense features of the same tiles and their nonzeros."""
+    sae = small_sae(activation, 640, 16200, dtype)
+    sae.b_enc.sub_(1.5)
+    x = torch.randn(2300, 640, device="cuda").to(dtype)
+    x[700:703] = sae.b_dec  # zeros once it is subtracted, and every bias below 0 drops them
+    sae.b_enc.clamp_(max=-0.5)
+    x[77, 5] = float("nan")
+    enc = saeflow_amd.Fp8Encoder.from_sae(sae)
+    f = enc.encode(x)
+    indptr, indices, values = enc.encode_sparse(x)
+    if activation == "topk":
+        pre = fused_encode_fp8(x, enc.W, enc.b_enc, b_dec=enc.b_dec)
+        v, i = topk_rows(pre, 16)
+        assert torch.equal(indptr, torch.arange(0, 16 * 2300 + 1, 16, device="cuda"))
+        assert torch.equal(indices.view(2300, 16), i) and torch.equal(values.nan_to_num(-7.0), v.nan_to_num(-7.0).flatten())
+        return
+    rows, cols = f.nonzero(as_tuple=True)
+    assert torch.equal(indptr[1:], (f != 0).sum(1).cumsum(0)) and indptr[0] == 0
+    assert torch.equal(indices, cols.int()) and torch.equal(values.nan_to_num(-7.0), f[rows, cols].nan_to_num(-7.0))
+    assert not f[700:703].any() and f[77].isnan().all() and f[0].any()
+
+
+@pytest.mark.parametrize("activation", ["relu", "jumprelu", "topk"])
+def test_encoder_without_tokens(activation):
+    enc = saeflow_amd.Fp8Encoder.from_sae(small_sae(activation))
+    x = torch.empty(0, 300, dtype=BF16, device="cuda")
+    for rows in (x, quantize_rows(x)):
+        assert enc.encode(rows).shape == (0, 2000)
+        indptr, indices, values = enc.encode_sparse(rows)
+        assert indptr.tolist() == [0] and indices.numel() == 0 and values.numel() == 0
+
+
+@pytest.mark.parametrize("times", [30, 3000])
+def test_product_of_rows_with_outlying_dimensions(times):
+    """Four dimensions `times` the others in size, biases that take most of what they add away again: the error
+    stays below 7 * 2^-13 of sum |x w| (of each eight products, seven lose at most 2^-13 of the largest), fp32
+    sums of K terms and one rounding."""
+    M, N, K = 300, 4096, 768
+    x = torch.randn(M, K, device="cuda")
+    x[:, [5, 130, 131, 700]] = times * (1 + 0.1 * x[:, [5, 130, 131, 700]])
+    x, W = quantize_rows(x), quantize_rows(torch.randn(N, K, device="cuda") / K ** 0.5)
+    xv, wv = (dequantize_rows(r, out_dtype=F32).double() for r in (x, W))
+    b = -(wv @ xv.mean(0)).float()
+    want, size = xv @ wv.T.contiguous() + b.double(), xv.abs() @ wv.abs().T.contiguous() + b.double().abs()
+    for dtype, u in ((F32, 0.0), (BF16, 2.0 ** -8), (F16, 2.0 ** -11)):
+        err = (fused_encode_fp8(x, W, b, activation="none", out_dtype=dtype).double() - want).abs()
+        sums = (K + 1) * 2.0 ** -23 + (7 * 2.0 ** -13 if u else 0.0)
+        assert (err <= sums * size * (1 + u) + u * want.abs() + 2.0 ** -24).all()
+
+
+def test_gradients_of_batches_from_the_buffer_are_those_of_the_values_read():
+    """Batches are the definition's values in 64 bits, bit for bit, and the gradients of a step on them are float64
+    autograd's at those values, to the tolerance of fp32 parameters (1e-4 of the largest, tests/test_gpu_backward.py)."""
+    from oracle import backward as obwd
+
+    sae = small_sae("relu", 200, 512, F32)
+    sae.requires_grad_(True)
+    data, b_dec = torch.randn(300, 200), sae.b_dec.detach().cpu()
+    buf = saeflow_amd.ActivationBuffer(256, 200, center=sae.b_dec)
+    buf.write(data[:200].cuda())
+    buf.write(data[200:].cuda())  # over rows 0 to 43
+    ids = torch.randperm(256)[:100]
+    x = buf.read(ids.cuda(), out_dtype=F32)
+    codes, scale = ofp8.quantize((torch.cat([data[256:], data[44:256]])[ids] - b_dec).numpy())
+    held = torch.from_numpy(codes * np.repeat(2.0 ** (scale.astype(np.float64) - 127), 128, 1)[:, :200]).float()
+    assert torch.equal(x.cpu(), held + b_dec)
+    x_hat, (indptr, indices, values) = saeflow_amd.forward_train(sae, x)
+    loss = (x_hat - x).pow(2).mean() + 0.01 * values.sum()
+    loss.backward()
+    G = (2 * (x_hat - x) / x.numel()).detach()
+    active = csr_to_dense(indptr, indices, values.detach(), 512).cpu() > 0
+    p = {name: getattr(sae, name).detach().cpu() for name in ("W_enc", "b_enc", "W_dec", "b_dec")}
+    want = obwd.grads(held + b_dec, p["W_enc"], p["b_enc"], p["W_dec"], p["b_dec"], active, G.cpu(), torch.full((100, 512), 0.01))
+    for name in p:
+        got = getattr(sae, name).grad.double().cpu()
+        torch.testing.assert_close(got, want[name], atol=1e-4 * float(want[name].abs().max()), rtol=1e-4, msg=name)
