@@ -136,9 +136,17 @@ constexpr int ONE_ROUND = 4;
 // 128x128 tiles 79; 2048 of d_in 4096 over 12289 106, 128x128 tiles 121).
 constexpr float UNALIGNED_TILE = 4.f;
 
-// Bytes of 16-bit results from which on 256x256 tiles store rows off whole lines past the caches too: 16000 tokens
-// over 12936 features (414 MB) 404 us so and 419 past the caches, over 16416 (525 MB) 571 and 494 (d_in 2304).
-constexpr double STREAM_FROM = 448e6;
+// Whether 256x256 tiles store 16-bit result rows off whole lines past the caches too. Time past the caches over time
+// through L2 (geometric means over 290 such shapes, d_in 64 to 4096, bf16):
+//   MB of results     250-448  448-530  530-600  600-750  750-1300
+//   d_in up to 128      1.42     1.39     1.40     1.35     1.24    (one K-step a tile)
+//   d_in 192 to 768     1.08     1.07     1.01     0.95     0.90
+//   d_in 1024 to 4096   1.02     0.99     0.93     0.91     0.85
+// The rule costs 1.2% over the better of both in the mean.
+bool stream_shared(int64_t M, int64_t N, int64_t K) {
+  const double bytes = (double)M * N * 2;
+  return K > BLOCK && bytes > (K < 1024 ? 600e6 : 448e6);
+}
 
 int pick_shape(int64_t M, int64_t N, int64_t K, int out_dt, bool unaligned) {
   const int nb = (int)blocks_of(K), wide = out_dt == SF_F32;
@@ -185,7 +193,7 @@ int product(const char* fn, const Tokens* tokens, const void* xq, int64_t sxq, c
   } else {
     const int shape = pick_shape(M, N, K, out_dt, som * sf_dtype_size(out_dt) % 16 != 0 || !aligned(out, 16));
     const Shape& h = SHAPES[out_dt == SF_F32][shape];
-    if (shape == 3 && out_dt != SF_F32 && (double)M * N * 2 > STREAM_FROM) a.stream = 1;
+    if (shape == 3 && out_dt != SF_F32 && stream_shared(M, N, K)) a.stream = 1;
     SF_REQUIRE(((M + h.tm - 1) / h.tm) * ((N + h.tn - 1) / h.tn) < (1ll << 23), "%s: too many tiles", fn);
     switch (shape) {
       case 0: e = launch_tile<F8x32>(a, s); break;

@@ -700,3 +700,15 @@ def test_gradients_of_batches_from_the_buffer_are_those_of_the_values_read():
     for name in p:
         got = getattr(sae, name).grad.double().cpu()
         torch.testing.assert_close(got, want[name], atol=1e-4 * float(want[name].abs().max()), rtol=1e-4, msg=name)
+
+
+@pytest.mark.parametrize("M,N,K,out_dtype", [(16384, 16391, 1100, BF16), (16384, 18501, 300, F16), (18500, 18501, 120, BF16),
+                                             (12000, 18500, 1030, F16)])
+def test_many_results_of_rows_off_whole_lines(M, N, K, out_dtype):
+    """Either kind of store, by d_in and the bytes of the results: whole numbers, whose sums (at most 9 * 1100) are
+    exact in fp32 and rounded once."""
+    g = torch.Generator(device="cuda").manual_seed(M + N + K)
+    x = torch.randint(-3, 4, (M, K), generator=g, device="cuda").float()
+    W = torch.randint(-3, 4, (N, K), generator=g, device="cuda").float()
+    got = fused_encode_fp8(quantize_rows(x), quantize_rows(W), activation="none", out_dtype=out_dtype)
+    assert torch.equal(got, (x @ W.T.contiguous()).to(out_dtype))
