@@ -73,10 +73,11 @@ class ActivationBuffer:
         Captured in a graph, a read knows the rows that were written by then."""
         if torch.is_tensor(rows):
             return read_rows(self.store, self._filled, rows, 0, None, self.center, out_dtype)
-        row0, count = (0, len(self)) if rows is None else rows
-        if count < 0 or not 0 <= row0 < self.capacity or count > len(self) or (row0 + count > len(self) < self.capacity):
-            raise ValueError(f"{count} rows from {row0} on are not among the {len(self)} written")
-        return dequantize_rows(self.store, row0=row0, count=count, shift=self.center, out_dtype=out_dtype)
+        R, filled = self.capacity, self._filled
+        row0, count = (0, filled) if rows is None else rows
+        if count < 0 or not 0 <= row0 < R or count > filled or (row0 + count > filled < R):
+            raise ValueError(f"{count} rows from {row0} on are not among the {filled} written")
+        return read_rows(self.store, R, None, row0, count, self.center, out_dtype)
 
     def rows(self, start, stop):
         """Written rows [start, stop) as they lie (a view): what Fp8Encoder and fused_encode_fp8 take."""
