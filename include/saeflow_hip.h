@@ -416,7 +416,10 @@ SF_API int sf_dequantize_rows(const void* q, int64_t sq, const void* scale, int6
 
 /*
  * sf_encode on 8-bit rows: out = act(x w^T + b_enc), x [M, K] and w [N, K] (a row a feature) as such
- * rows, fp32 sums. b_enc [N] or NULL, thr [N], activations, row_nnz (NULL with SF_ACT_NONE) and rounding as in sf_encode,
+ * rows. fp32 results are as good as fp32 sums. bf16 and fp16 results are summed in fp32 by the 8-bit
+ * matrix instruction, which drops, of each eight products, what lies below 2^-13 of the largest: at
+ * most 7 * 2^-13 of sum |x w| (5.5e-5 of the result in the root mean square for normal operands).
+ * b_enc [N] or NULL, thr [N], activations, row_nnz (NULL with SF_ACT_NONE) and rounding as in sf_encode,
  * but bf16 results of 2^-126 and less are stored and counted as they round (sf_encode stores zeros);
  * out [M, N], rows som elements apart.
  *   sf_encode_fp8_rows  x as 8-bit rows (of an activation cache). workspace: caller-owned, 16-B

@@ -111,11 +111,13 @@ struct Tokens {
 // Estimated time of a product in us with tiles of tm x tn: a fixed part, and for each round of tiles over
 // the CUs a part per block of K (`alone` times that with one workgroup a CU) and one per tile; at least
 // the bytes at the rate that the shape streams them. Fitted to 220 shapes of 1 to 4096 tokens, d_in 256 to
-// 4096, 4096 to 131072 features, in both result sizes: the pick is 1.1% (fp32 0.4%) slower than the best in
-// the mean, 23% at most. Where each of the first four wins at d_in 2304, d_sae 65536, bf16 (us in
-// order): 32 tokens 25 25 25 31 (d_sae 16384: 10 11 16 26), 128 tokens 43 30 27 32, 256 tokens 80 59 44 37, 4096
-// tokens 1175 867 690 530; fp32 results of 128 tokens 60 49 41 61, of 256 117 97 78 67, of 4096 1717 1424 1155
-// 1041.
+// 4096, 4096 to 131072 features, in both result sizes, before results went through L2 where lines are shared. Over 715
+// other shapes with the stores as they are (1 to 8192 tokens, d_in 120 to 4096, two of three with rows off 16 B) the pick is
+// 1.6% (fp32 0.6%) slower than the best in the mean, 30% at most (2175 tokens of d_in 256 over 58624 features: 256x256
+// 85 us, 128x128 67). Where each of the first four wins at d_in 2304, d_sae 65536, bf16 (us in
+// order): 32 tokens 24 25 25 32 (d_sae 16384: 11 11 16 26), 128 tokens 42 30 26 33, 256 tokens 79 53 42 37, 4096
+// tokens 1133 803 626 494; fp32 results of 128 tokens 59 46 40 60, of 256 109 87 73 66, of 4096 1714 1394 1104
+// 962.
 struct Shape {
   int tm, tn;
   float fixed, step, alone, tile, tail, tbs;
@@ -132,8 +134,9 @@ constexpr Shape SHAPES[2][5] = {
 // results only (d_in 4096, d_sae 12288, 256 tokens 18 us against 21 with 64 x 128; from two rounds on two
 // workgroups a CU win).
 constexpr int ONE_ROUND = 4;
-// What result rows off 16 B cost a 256x256 tile (bf16, stored past the caches: 4096 tokens of d_in 768 over 16391 features 92 us,
-// 128x128 tiles 79; 2048 of d_in 4096 over 12289 106, 128x128 tiles 121).
+// What result rows off 16 B cost a 256x256 tile (bf16: 4096 tokens of d_in 768 over 16391 features 92 us, 128x128 tiles
+// 73). Over 326 such shapes the pick is 1.3% slower than the best with 4 us, 2.0% with 3, 1.9% with 5, 4.2% with none (169
+// of fp32: 0.6, 0.5, 0.6, 1.7%).
 constexpr float UNALIGNED_TILE = 4.f;
 
 // Whether 256x256 tiles store 16-bit result rows off whole lines past the caches too. Time past the caches over time
