@@ -26,7 +26,7 @@
 extern "C" {
 #endif
 
-#define SF_ABI_VERSION 5
+#define SF_ABI_VERSION 6
 
 /* The library is built with hidden symbol visibility; exactly these entry points are exported. */
 #ifndef SF_API
@@ -438,6 +438,39 @@ SF_API int sf_encode_fp8(const void* x, int64_t sxm, int64_t sxk, int x_dt, cons
                          const void* wq, int64_t swq, const void* ws, int64_t sws, const void* b_enc, int benc_dt,
                          const void* thr, int thr_dt, void* out, int64_t som, int out_dt, int32_t* row_nnz, int64_t M,
                          int64_t N, int64_t K, int act, void* workspace, int64_t workspace_bytes, void* stream);
+
+/*
+ * Layer norm (no reference counterpart). Rows of D elements, 1 <= D <= 2^24, unit column stride and row
+ * strides in elements; any element-aligned addresses. Per row m: mean = sum x / D (summed in 64 bits), rstd =
+ * 1 / sqrt(sum (x - mean)^2 / D + eps), xh = (x - mean) rstd.
+ *
+ * sf_layer_norm: y = xh w + b, formed in fp32 and rounded once to y_dt. w, b [D] contiguous, either NULL; eps >= 0;
+ *   mean, rstd fp32 [M], either NULL. With q (16-B aligned) and scale also row m of an 8-bit store of x - mean
+ *   (the fp32 difference; layout and rounding of sf_quantize_rows).
+ * sf_layer_norm_backward: with qq = g w (g without w), c1 = sum qq / D, c2 = sum qq xh / D:
+ *     dx = rstd (qq - c1 - xh c2) + g_mean / D - g_rstd rstd^2 xh / D,   dw = sum_m g xh,   db = sum_m g.
+ *   The input is x with mean, or (x NULL) the 8-bit rows of x - mean that the forward pass left; rstd [M] fp32.
+ *   g_mean, g_rstd fp32 [M]: gradients of mean and rstd, either NULL. dx [M, D], dw, db [D]: any of them NULL.
+ *   Sums in fp32 in a fixed order. workspace: caller-owned, 4-B aligned, at least
+ *   sf_layer_norm_backward_workspace_size bytes; calls in flight at the same time must not share one.
+ * sf_denormalize: out = h / rstd + mean, rounded once to out_dt.
+ * sf_denormalize_backward: dh = g / rstd, dmean[m] = sum g, drstd[m] = -sum g h / rstd^2; any of the three NULL, and
+ *   h is read only for drstd.
+ */
+SF_API int sf_layer_norm(const void* x, int64_t sxm, int x_dt, const void* w, int w_dt, const void* b, int b_dt,
+                         float eps, int64_t M, int64_t D, void* y, int64_t sym, int y_dt, float* mean, float* rstd,
+                         void* q, int64_t sq, void* scale, int64_t ss, void* stream);
+SF_API int sf_layer_norm_backward_workspace_size(int64_t M, int64_t D, int64_t* bytes);
+SF_API int sf_layer_norm_backward(const void* g, int64_t sgm, int g_dt, const void* x, int64_t sxm, int x_dt,
+                                  const void* q, int64_t sq, const void* scale, int64_t ss, const float* mean,
+                                  const float* rstd, const void* w, int w_dt, const float* g_mean, const float* g_rstd,
+                                  int64_t M, int64_t D, void* dx, int64_t sdx, int dx_dt, void* dw, int dw_dt, void* db,
+                                  int db_dt, void* workspace, int64_t workspace_bytes, void* stream);
+SF_API int sf_denormalize(const void* h, int64_t shm, int h_dt, const float* mean, const float* rstd, int64_t M,
+                          int64_t D, void* out, int64_t som, int out_dt, void* stream);
+SF_API int sf_denormalize_backward(const void* g, int64_t sgm, int g_dt, const void* h, int64_t shm, int h_dt,
+                                   const float* rstd, int64_t M, int64_t D, void* dh, int64_t sdh, int dh_dt,
+                                   float* dmean, float* drstd, void* stream);
 
 #ifdef __cplusplus
 }

@@ -15,7 +15,7 @@ from pathlib import Path
 import torch
 
 LIB_PATH = Path(__file__).resolve().parent / "libsaeflow_hip.so"
-ABI_VERSION = 5
+ABI_VERSION = 6
 
 SF_OK, SF_EINVAL, SF_EHIP, SF_EUNSUPPORTED = 0, 1, 2, 3
 ACT = {"relu": 0, "jumprelu": 1, "none": 2}
@@ -72,6 +72,13 @@ SIGNATURES = {
     "sf_encode_fp8_workspace_size": (_I32, [_I64, _I64, _P]),
     "sf_encode_fp8": (_I32, [_P, _I64, _I64, _I32, _P, _I32, _P, _I64, _P, _I64, _P, _I32, _P, _I32, _P, _I64, _I32, _P,
                              _I64, _I64, _I64, _I32, _P, _I64, _P]),
+    "sf_layer_norm": (_I32, [_P, _I64, _I32, _P, _I32, _P, _I32, ctypes.c_float, _I64, _I64, _P, _I64, _I32, _P, _P,
+                             _P, _I64, _P, _I64, _P]),
+    "sf_layer_norm_backward_workspace_size": (_I32, [_I64, _I64, _P]),
+    "sf_layer_norm_backward": (_I32, [_P, _I64, _I32, _P, _I64, _I32, _P, _I64, _P, _I64, _P, _P, _P, _I32, _P, _P,
+                                      _I64, _I64, _P, _I64, _I32, _P, _I32, _P, _I32, _P, _I64, _P]),
+    "sf_denormalize": (_I32, [_P, _I64, _I32, _P, _P, _I64, _I64, _P, _I64, _I32, _P]),
+    "sf_denormalize_backward": (_I32, [_P, _I64, _I32, _P, _I64, _I32, _P, _I64, _I64, _P, _I64, _I32, _P, _P, _P]),
 }
 
 _lib = None
@@ -163,4 +170,12 @@ def fp8_workspace_bytes(M, K):
     """sf_encode_fp8_workspace_size, a function of its arguments alone."""
     nbytes = ctypes.c_int64()
     check(load().sf_encode_fp8_workspace_size(M, K, ctypes.byref(nbytes)))
+    return nbytes.value
+
+
+@functools.lru_cache(maxsize=256)
+def layer_norm_workspace_bytes(M, D):
+    """sf_layer_norm_backward_workspace_size, a function of its arguments alone."""
+    nbytes = ctypes.c_int64()
+    check(load().sf_layer_norm_backward_workspace_size(M, D, ctypes.byref(nbytes)))
     return nbytes.value

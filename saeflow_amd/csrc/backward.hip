@@ -24,6 +24,7 @@
 #include <type_traits>
 
 #include "common.h"
+#include "wave.h"
 
 namespace {
 
@@ -39,40 +40,6 @@ __device__ __forceinline__ void clamp_range(const int64_t* ptr, int64_t i, int64
   hi = ptr[i + 1];
   lo = lo < 0 ? 0 : (lo > n ? n : lo);
   hi = hi < lo ? lo : (hi > n ? n : hi);
-}
-
-// Sum of v over the wave, returned in every lane, with DPP moves (VALU) instead of LDS
-// permutes: xor-1 and xor-2 within quads, the half-row and row mirrors give each 16-lane row
-// its total, row_bcast:15 / row_bcast:31 carry row totals upward, lane 63 ends with the sum.
-template <int CTRL, int ROW_MASK>
-__device__ __forceinline__ float dpp_add(float v) {
-  return v + __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), CTRL, ROW_MASK, 0xF, false));
-}
-__device__ __forceinline__ float wave_sum(float v) {
-  v = dpp_add<0xB1, 0xF>(v);   // quad_perm [1,0,3,2]
-  v = dpp_add<0x4E, 0xF>(v);   // quad_perm [2,3,0,1]
-  v = dpp_add<0x141, 0xF>(v);  // row_half_mirror
-  v = dpp_add<0x140, 0xF>(v);  // row_mirror
-  v = dpp_add<0x142, 0xA>(v);  // row_bcast:15 into rows 1 and 3
-  v = dpp_add<0x143, 0xC>(v);  // row_bcast:31 into rows 2 and 3
-  return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), 63));
-}
-
-// Wave sums of 8 values at once: afterwards every lane l holds the total of v[(l >> 3) & 7].
-// A reduce-scatter: each of three exchanges (lanes 32, 16 and 8 apart) keeps half of the values
-// a lane still carries and adds its partner's copy of that half, then DPP moves sum the 8-lane
-// groups (quads, then the half-row mirror). 7 permutes and 10 adds instead of 8 full reductions.
-__device__ __forceinline__ float wave_sum8(const float (&v)[8], int lane) {
-  const bool b5 = lane & 32, b4 = lane & 16, b3 = lane & 8;
-  float w[4], x[2];
-#pragma unroll
-  for (int k = 0; k < 4; ++k) w[k] = (b5 ? v[k + 4] : v[k]) + __shfl_xor(b5 ? v[k] : v[k + 4], 32);
-#pragma unroll
-  for (int k = 0; k < 2; ++k) x[k] = (b4 ? w[k + 2] : w[k]) + __shfl_xor(b4 ? w[k] : w[k + 2], 16);
-  float y = (b3 ? x[1] : x[0]) + __shfl_xor(b3 ? x[0] : x[1], 8);
-  y = dpp_add<0xB1, 0xF>(y);   // quad_perm [1,0,3,2]
-  y = dpp_add<0x4E, 0xF>(y);   // quad_perm [2,3,0,1]
-  return dpp_add<0x141, 0xF>(y);  // row_half_mirror: the other quad of the 8-lane group
 }
 
 // EPC elements (one 16-B chunk) of row `rowp` starting at element c*EPC, as fp32. VEC: the

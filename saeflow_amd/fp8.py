@@ -19,6 +19,8 @@ import torch
 from . import _lib
 from .kernels import dense_to_csr, fixed_width_to_dense, topk_rows
 from .kernels.fp8 import Fp8Rows, _vector, dequantize_rows, fused_encode_fp8, quantize_rows, read_rows
+from .norm import layer_norm
+from .ops import INPUT_NORMS, input_norm, norm_eps
 from .sae import ACTIVATIONS
 
 
@@ -92,15 +94,20 @@ class Fp8Encoder:
 
     Tokens are quantised minus b_dec, in blocks of 128, on the way into the product. 8-bit rows (an
     ActivationBuffer's) are taken as they are: they hold x - center, `center` by default b_dec.
+    input_norm="layer_norm": tokens are normed first, as the SAE's are; 8-bit rows hold normed tokens then.
     """
 
-    def __init__(self, W_enc, b_enc, b_dec, threshold=None, activation="relu", k=None, *, center=None):
+    def __init__(self, W_enc, b_enc, b_dec, threshold=None, activation="relu", k=None, *, center=None, input_norm=None,
+                 norm_eps=1e-5):
         if activation not in ACTIVATIONS:
             raise ValueError(f"activation must be one of {ACTIVATIONS}, got {activation!r}")
         if activation == "jumprelu" and threshold is None:
             raise ValueError("jumprelu needs a threshold")
         if activation == "topk" and not k:
             raise ValueError("topk activation needs k")
+        if input_norm not in INPUT_NORMS:
+            raise ValueError(f"input_norm must be one of {INPUT_NORMS}, got {input_norm!r}")
+        self.input_norm, self.norm_eps = input_norm, norm_eps
         d_in, d_sae = W_enc.shape
         self.activation, self.k = activation, k
         self.b_enc = _vector(b_enc.detach(), d_sae, "b_enc").clone()
@@ -114,7 +121,8 @@ class Fp8Encoder:
     @classmethod
     def from_sae(cls, sae, *, center=None):
         """Of a saeflow_amd.SAE, or anything with its attributes."""
-        return cls(sae.W_enc, sae.b_enc, sae.b_dec, sae.threshold, sae.activation, sae.k, center=center)
+        return cls(sae.W_enc, sae.b_enc, sae.b_dec, sae.threshold, sae.activation, sae.k, center=center,
+                   input_norm=input_norm(sae), norm_eps=norm_eps(sae))
 
     def _moved_bias(self, center):
         """b_enc + W (center - b_dec) in fp32, W as it is held: the bias for rows that hold x - center."""
@@ -135,6 +143,8 @@ class Fp8Encoder:
         if isinstance(x, Fp8Rows):
             return fused_encode_fp8(x, self.W, self.rows_bias, self.threshold, activation, out_dtype=out_dtype,
                                     row_nnz=row_nnz)
+        if self.input_norm is not None:
+            x = layer_norm(x, eps=self.norm_eps)
         return fused_encode_fp8(x, self.W, self.b_enc, self.threshold, activation, b_dec=self.b_dec,
                                 out_dtype=out_dtype, row_nnz=row_nnz)
 

@@ -16,6 +16,7 @@ from types import SimpleNamespace
 import torch
 
 from .. import _lib
+from .fp8 import Fp8Rows, dequantize_rows
 
 
 def _rows(t, dtype):
@@ -51,20 +52,23 @@ def sparse_backward(x, W_enc, b_enc, W_dec, b_dec, csr, grad_x_hat=None, grad_va
     """Gradients of a loss L through the forward above, from g_xhat = dL/dx_hat [M, d_in] and
     optionally dL/df on the CSR values (grad_values [nnz], e.g. from a sparsity penalty).
 
+    x: the tokens, or 8-bit rows of x - b_dec (quantize_rows(x, shift=b_dec)) kept in their place: dW_enc
+    is then the sum over what the rows hold, and the other gradients do not depend on x.
     csr = (indptr, indices, values) as encode_sparse returned it for x. Returns a namespace
     with W_enc [d_in, d_sae], b_enc, W_dec [d_sae, d_in], b_dec (each in its parameter's
-    dtype), x (x's dtype; None unless need_grad_x) and pre (fp32 dL/dpre on the CSR entries).
+    dtype), x (x's dtype, fp32 for 8-bit rows; None unless need_grad_x) and pre (fp32 dL/dpre on the CSR entries).
     fp32 accumulation throughout, in a fixed order (repeated calls give identical bits). No
     threshold gradient: jumprelu's is zero almost everywhere. Nothing waits for the GPU.
     """
     indptr, indices, values = csr
     M, D = x.shape
+    held = isinstance(x, Fp8Rows)
     if W_enc.shape[0] != D or W_dec.shape != (W_enc.shape[1], D):
         raise ValueError(f"shape mismatch: x {tuple(x.shape)}, W_enc {tuple(W_enc.shape)}, W_dec {tuple(W_dec.shape)}")
     N = W_enc.shape[1]
     if W_enc.dtype != W_dec.dtype:
         raise ValueError(f"W_enc ({W_enc.dtype}) and W_dec ({W_dec.dtype}) must share a dtype")
-    dev = _lib.require_gpu(("x", x), ("W_enc", W_enc), ("b_enc", b_enc), ("W_dec", W_dec), ("b_dec", b_dec),
+    dev = _lib.require_gpu(("x", x.q if held else x), ("W_enc", W_enc), ("b_enc", b_enc), ("W_dec", W_dec), ("b_dec", b_dec),
                            ("indptr", indptr), ("indices", indices), ("values", values),
                            ("grad_x_hat", grad_x_hat), ("grad_values", grad_values))
     if indptr.numel() != M + 1:
@@ -85,9 +89,12 @@ def sparse_backward(x, W_enc, b_enc, W_dec, b_dec, csr, grad_x_hat=None, grad_va
             raise ValueError(f"grad_values has {gv.numel()} entries for nnz={nnz}")
         # per-feature sums over the CSC
         colptr, rows, pos = csr_transpose(indptr, indices, N)
-        xs = torch.empty(M, D, dtype=dt, device=dev)
-        _lib.check(lib.sf_shifted_input(_lib.ptr(x), x.stride(0), x.stride(1), _lib.dtype_code(x, "x"),
-                                        _lib.ptr(b_dec), _lib.dtype_code(b_dec, "b_dec"), M, D, code, _lib.ptr(xs), s))
+        if held:
+            xs = dequantize_rows(x, out_dtype=dt)
+        else:
+            xs = torch.empty(M, D, dtype=dt, device=dev)
+            _lib.check(lib.sf_shifted_input(_lib.ptr(x), x.stride(0), x.stride(1), _lib.dtype_code(x, "x"),
+                                            _lib.ptr(b_dec), _lib.dtype_code(b_dec, "b_dec"), M, D, code, _lib.ptr(xs), s))
         plan_i64 = torch.empty(3 * (N + 1), dtype=torch.int64, device=dev)
         max_items, max_slots, work_floats = ctypes.c_int64(), ctypes.c_int64(), ctypes.c_int64()
         _lib.check(lib.sf_backward_bounds(N, nnz, D, code, ctypes.byref(max_items), ctypes.byref(max_slots),
@@ -135,4 +142,4 @@ def sparse_backward(x, W_enc, b_enc, W_dec, b_dec, csr, grad_x_hat=None, grad_va
                                      nnz, _lib.ptr(W_encT), W_encT.stride(0), W_encT.stride(1), code, N, None, 0,
                                      _lib.ptr(dxs), D, 1, _lib.DTYPE[torch.float32], M, D, None, s))
     return SimpleNamespace(W_enc=d_wenc.to(W_enc.dtype), b_enc=d_benc.to(b_enc.dtype), W_dec=d_wdec,
-                           b_dec=d_bdec.to(b_dec.dtype), x=None if dxs is None else dxs.to(x.dtype), pre=g_pre)
+                           b_dec=d_bdec.to(b_dec.dtype), x=dxs if dxs is None or held else dxs.to(x.dtype), pre=g_pre)

@@ -7,6 +7,7 @@ see kernels/decode.py.
 
 import torch
 
+from . import norm
 from .kernels import (dense_to_csr, encode_gather, encode_rows, fixed_width_to_dense, fused_encode,
                       overflow_rows, rows_to_csr, rows_topk, scan_counts, sparse_decode, topk_gather, topk_rows)
 
@@ -19,6 +20,7 @@ ROW_PATHS = True   # False: always the dense path (the reference's structure)
 ROW_CAP = 1024     # candidates per row for encode_sparse (relu / jumprelu)
 TOPK_CAP = 4096    # candidates per row for TopK
 TOPK_MIN_FEATURES = 16384  # TopK takes the row-candidate path from this dictionary size on
+INPUT_NORMS = (None, "layer_norm")
 TOPK_REDO_BYTES = 1 << 31  # dense features of the overflowed rows redone per chunk (at least 256 rows)
 
 
@@ -102,8 +104,26 @@ def _encode_sparse_rows(sae, x):
     return indptr, indices, values
 
 
+def input_norm(sae):
+    """The SAE's input_norm, which a duck-typed one need not have: None or "layer_norm"."""
+    kind = getattr(sae, "input_norm", None)
+    if kind not in INPUT_NORMS:
+        raise ValueError(f"input_norm must be one of {INPUT_NORMS}, got {kind!r}")
+    return kind
+
+
+def norm_eps(sae):
+    return getattr(sae, "norm_eps", 1e-5)
+
+
+def normed_input(sae, x):
+    """What the encoder reads: x, or its rows normed (in x's type)."""
+    return x if input_norm(sae) is None else norm.layer_norm(x, eps=norm_eps(sae))
+
+
 def encode(sae, x):
     """The features of every token as a dense [M, d_sae] tensor (ops.py:19-26)."""
+    x = normed_input(sae, x)
     if sae.activation == "topk":
         values, indices = _topk(sae, x)
         return fixed_width_to_dense(indices, values, sae.W_enc.shape[1])
@@ -113,6 +133,10 @@ def encode(sae, x):
 def encode_sparse(sae, x):
     """The features of every token in the CSR contract, (indptr int64 [M+1], indices int32
     [nnz], values [nnz]) (ops.py:29-39)."""
+    return _encode_sparse(sae, normed_input(sae, x))
+
+
+def _encode_sparse(sae, x):
     M = x.shape[0]
     if sae.activation == "topk":
         # every row holds exactly k entries, so indptr is arange(0, M*k+1, k) and no scan or
@@ -128,10 +152,15 @@ def encode_sparse(sae, x):
 
 
 def decode_sparse(sae, csr):
-    """x_hat [M, d_in] = b_dec + the W_dec rows the CSR selects, weighted by its values (ops.py:42-44)."""
+    """x_hat [M, d_in] = b_dec + the W_dec rows the CSR selects, weighted by its values (ops.py:42-44).
+    With an input norm this reconstructs the normed tokens; saeflow_amd.denormalize carries it back."""
     return sparse_decode(*csr, sae.W_dec, sae.b_dec)
 
 
 def forward(sae, x):
-    """decode_sparse(encode_sparse(x)) (ops.py:47-49): no dense [M, d_sae] tensor reaches the decoder."""
-    return decode_sparse(sae, encode_sparse(sae, x))
+    """decode_sparse(encode_sparse(x)) (ops.py:47-49): no dense [M, d_sae] tensor reaches the decoder.
+    With an input norm the reconstruction is carried back to x's own space."""
+    if input_norm(sae) is None:
+        return decode_sparse(sae, _encode_sparse(sae, x))
+    z, mean, rstd = norm.layer_norm(x, eps=norm_eps(sae), return_stats=True)
+    return norm.denormalize(decode_sparse(sae, _encode_sparse(sae, z)), mean, rstd)

@@ -18,14 +18,22 @@ class SAE(nn.Module):
     Activations: "relu"; "jumprelu", which also zeroes features at or below their own
     `threshold`; "topk", which keeps each token's `k` largest ReLU features. The tensors carry
     SAELens's names and layouts (W_enc is [d_in, d_sae], W_dec is [d_sae, d_in]).
+
+    input_norm (not in the reference): None, or "layer_norm": the encoder reads layer_norm(x) (no weight, no bias,
+    `norm_eps`), decode reconstructs that, and calling the SAE carries the reconstruction back to x's own space with
+    the rows' means and deviations.
     """
 
-    def __init__(self, d_in, d_sae, activation="relu", k=None, device=None, dtype=torch.float32):
+    def __init__(self, d_in, d_sae, activation="relu", k=None, device=None, dtype=torch.float32, *, input_norm=None,
+                 norm_eps=1e-5):
         super().__init__()
         if activation not in ACTIVATIONS:
             raise ValueError(f"activation must be one of {ACTIVATIONS}, got {activation!r}")
         if activation == "topk" and not k:
             raise ValueError("topk activation needs k")
+        if input_norm not in (None, "layer_norm"):
+            raise ValueError(f"input_norm must be None or 'layer_norm', got {input_norm!r}")
+        self.input_norm, self.norm_eps = input_norm, norm_eps
         self.d_in, self.d_sae, self.activation, self.k = d_in, d_sae, activation, k
 
         W_dec = torch.randn(d_sae, d_in, device=device)
@@ -41,8 +49,9 @@ class SAE(nn.Module):
 
     def encode_pre(self, x):
         from .kernels import encode_pre
+        from .ops import normed_input
 
-        return encode_pre(x, self.W_enc, self.b_enc, self.b_dec)
+        return encode_pre(normed_input(self, x), self.W_enc, self.b_enc, self.b_dec)
 
     def encode(self, x):
         from .ops import encode
