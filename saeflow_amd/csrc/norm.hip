@@ -8,6 +8,7 @@
 //
 // All of it is bound by HBM: a row is read once and held in registers between the sums and the result.
 #include <algorithm>
+#include <type_traits>
 
 #include "fp8.h"
 #include "wave.h"
@@ -49,6 +50,46 @@ __device__ __forceinline__ Raw<ES> load_raw(const char* row, int64_t k0, int64_t
       }
   }
   return v;
+}
+// The same in two steps, for rows of at least eight elements, so that loads stay in flight without a branch: a
+// lane whose chunk runs past D loads the row's last eight elements, and shifts by `off` = k0 - (D - 8) elements
+// (zeros come in; eight or more: all zeros) once they are there.
+template <int ES>
+__device__ __forceinline__ Raw<ES> load_at(const char* row, uint32_t at) {  // (a uniform row, a lane's own offset)
+  Raw<ES> v;
+#pragma unroll
+  for (int i = 0; i < ES / 2; ++i) {
+    const u32x4 c = *(const u32x4_any*)(row + at + i * 16);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) v.r[4 * i + j] = c[j];
+  }
+  return v;
+}
+template <int ES>
+__device__ __forceinline__ Raw<ES> load_back(const char* row, int64_t k0, int64_t D) {
+  return load_at<ES>(row, (uint32_t)min(k0, D - 8) * ES);
+}
+template <int ES>
+__device__ __forceinline__ void shift_back(Raw<ES>& v, int off) {
+  constexpr int N = 2 * ES;
+  if constexpr (ES == 2) {  // an odd element first
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const uint32_t next = i + 1 < N ? v.r[i + 1] : 0;
+      v.r[i] = off & 1 ? (v.r[i] >> 16) | (next << 16) : v.r[i];
+    }
+  }
+#pragma unroll
+  for (int by = 1; by < N; by <<= 1) {  // then whole registers
+    const bool go = off & (ES == 2 ? 2 * by : by);
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const uint32_t from = i + by < N ? v.r[i + by] : 0;
+      v.r[i] = go ? from : v.r[i];
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < N; ++i) v.r[i] = off >= 8 ? 0 : v.r[i];
 }
 template <int ES>
 __device__ __forceinline__ float raw_elem(const Raw<ES>& v, int e, bool bf16) {
@@ -105,10 +146,42 @@ __device__ __forceinline__ void store8_any(char* row, int dt, int64_t k0, int64_
   }
 }
 
-__device__ __forceinline__ double wave_sum_f64(double v) {
+// the same through a buffer resource over a row, which drops what lies past its bounds (the row may begin anywhere)
+template <int DT>
+__device__ __forceinline__ void put8_rsrc(__amdgpu_buffer_rsrc_t rs, int k0, const float (&v)[8]) {
+  if constexpr (DT == SF_F32) {
 #pragma unroll
-  for (int off = 32; off > 0; off >>= 1) v += __shfl_xor(v, off);
-  return v;
+    for (int i = 0; i < 2; ++i)
+      __builtin_amdgcn_raw_buffer_store_b128(u32x4{__float_as_uint(v[4 * i]), __float_as_uint(v[4 * i + 1]),
+                                                   __float_as_uint(v[4 * i + 2]), __float_as_uint(v[4 * i + 3])},
+                                             rs, k0 * 4 + 16 * i, 0, 0);
+  } else {
+    u32x4 q;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) q[i] = f32_to_bits(v[2 * i], DT) | f32_to_bits(v[2 * i + 1], DT) << 16;
+    __builtin_amdgcn_raw_buffer_store_b128(q, rs, k0 * 2, 0, 0);
+  }
+}
+
+// Sum of v over the wave in 64 bits, in every lane (wave_sum's moves on both halves).
+template <int CTRL, int ROW_MASK>
+__device__ __forceinline__ double dpp_add_f64(double v) {
+  const uint64_t u = (uint64_t)__double_as_longlong(v);
+  const uint32_t lo = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)u, CTRL, ROW_MASK, 0xF, false);
+  const uint32_t hi = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)(u >> 32), CTRL, ROW_MASK, 0xF, false);
+  return v + __longlong_as_double((long long)((uint64_t)hi << 32 | lo));
+}
+__device__ __forceinline__ double wave_sum_f64(double v) {
+  v = dpp_add_f64<0xB1, 0xF>(v);
+  v = dpp_add_f64<0x4E, 0xF>(v);
+  v = dpp_add_f64<0x141, 0xF>(v);
+  v = dpp_add_f64<0x140, 0xF>(v);
+  v = dpp_add_f64<0x142, 0xA>(v);
+  v = dpp_add_f64<0x143, 0xC>(v);
+  const uint64_t u = (uint64_t)__double_as_longlong(v);
+  const uint32_t lo = (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)u, 63);
+  const uint32_t hi = (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)(u >> 32), 63);
+  return __longlong_as_double((long long)((uint64_t)hi << 32 | lo));
 }
 __device__ __forceinline__ float inverse_std(float sum_sq, float D, float eps) { return 1.0f / sqrtf(sum_sq / D + eps); }
 
@@ -120,6 +193,7 @@ struct FwdArgs {
   const void* b;
   int w_dt, b_dt;
   float eps;
+  double per_d;  // 1 / D
   int64_t M, D;
   char* y;
   int64_t sym;
@@ -156,6 +230,18 @@ __device__ __forceinline__ void put_y(const FwdArgs& a, int64_t m, int64_t k0, c
   store8_any(a.y + m * a.sym, a.y_dt, k0, a.D, y);
 }
 
+// sff8::quantize8 of finite elements: no look at each for NaN and infinity.
+__device__ __forceinline__ u32x2 quantize8_finite(float (&v)[8], uint32_t& byte) {
+  float top = 0.f;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) top = fmaxf(top, fabsf(v[e]));
+  byte = sff8::scale_byte(sff8::max16(__float_as_uint(top)));
+  const float inv = sff8::inverse_of(byte);
+#pragma unroll
+  for (int e = 0; e < 8; ++e) v[e] *= inv;
+  return u32x2{sff8::pack4(v[0], v[1], v[2], v[3]), sff8::pack4(v[4], v[5], v[6], v[7])};
+}
+
 // The same elements as codes: sixteen lanes hold a block, and all of a wave's lanes come here.
 __device__ __forceinline__ void put_codes(const FwdArgs& a, int64_t m, int64_t k0, const float (&d)[8]) {
   float v[8];
@@ -172,54 +258,124 @@ __device__ __forceinline__ void put_codes(const FwdArgs& a, int64_t m, int64_t k
   }
 }
 
-// A wave a row, U chunks of eight elements a lane. The mean's sum is held in 64 bits: it rounds to the same 32 bits
-// in whatever order it is formed, so the codes of x - mean are the same in every form of this kernel.
+// A wave a row, U = ceil(D / 512) chunks of eight elements a lane; y is of x's type. The mean's sum is held in 64 bits:
+// it rounds to the same 32 bits in whatever order it is formed, so the codes of x - mean are the same in every form of
+// this kernel. The wave's next row is under way while this one is worked on: rows leave by buffer stores, whose
+// bounds drop the lanes past the last whole chunk without a branch, and weight and bias are kept in LDS as fp32, so
+// that no wait for a row's loads waits for anything else. In LDS the lower four elements of all chunks lie before the
+// upper four: lanes read 16 B side by side.
 template <int DT, int U, bool HOLD>
 __global__ __launch_bounds__(256) void norm_kernel(FwdArgs a) {
-  constexpr int ES = DT == SF_F32 ? 4 : 2;
-  const int lane = threadIdx.x & 63;
-  const int64_t m = (int64_t)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  if (m >= a.M) return;
-  const char* row = a.x + m * a.sxm;
+  constexpr int ES = DT == SF_F32 ? 4 : 2, CH = U * 64;
+  constexpr bool bf = DT == SF_BF16;
+  __shared__ u32x4 s_par[4 * CH];  // weight's lower and upper halves, then bias's
+  const int lane = threadIdx.x & 63, D = (int)a.D;
+  const int last = ((U - 1) * 64 + lane) * 8, off = max(0, last - (D - 8));
+  const bool past = D < U * 512, affine = a.w || a.b;
+  int64_t m = (int64_t)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int64_t step = (int64_t)gridDim.x * 4;
   Raw<ES> raw[U];
+  auto load = [&](int64_t row) {
+    const char* p = a.x + min(row, a.M - 1) * a.sxm;  // (a wave past the last row loads that again)
 #pragma unroll
-  for (int i = 0; i < U; ++i) raw[i] = load_raw<ES>(row, (i * 64 + lane) * 8, a.D);
-  double sum = 0.0;
+    for (int i = 0; i < U; ++i) raw[i] = load_at<ES>(p, (uint32_t)(i + 1 < U ? (i * 64 + lane) * 8 : min(last, D - 8)) * ES);
+  };
+  load(m);
+  if (affine) {
+    for (int c = threadIdx.x; c < CH; c += 256) {
+      float w[8], b[8];
 #pragma unroll
-  for (int i = 0; i < U; ++i)
+      for (int e = 0; e < 8; ++e) {
+        w[e] = 1.f;
+        b[e] = 0.f;
+      }
+      if (a.w) load8_any(a.w, a.w_dt, c * 8, D, w);
+      if (a.b) load8_any(a.b, a.b_dt, c * 8, D, b);
 #pragma unroll
-    for (int e = 0; e < 8; ++e) sum += (double)raw_elem(raw[i], e, DT == SF_BF16);
-  const float mean = (float)(wave_sum_f64(sum) / (double)a.D);
-  float sq = 0.f;
-#pragma unroll
-  for (int i = 0; i < U; ++i)
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const float d = (i * 64 + lane) * 8 + e < a.D ? raw_elem(raw[i], e, DT == SF_BF16) - mean : 0.f;
-      sq = fmaf(d, d, sq);
+      for (int h = 0; h < 2; ++h) {
+        s_par[h * CH + c] = u32x4{__float_as_uint(w[4 * h]), __float_as_uint(w[4 * h + 1]), __float_as_uint(w[4 * h + 2]), __float_as_uint(w[4 * h + 3])};
+        s_par[(2 + h) * CH + c] = u32x4{__float_as_uint(b[4 * h]), __float_as_uint(b[4 * h + 1]), __float_as_uint(b[4 * h + 2]), __float_as_uint(b[4 * h + 3])};
+      }
     }
-  const float rstd = inverse_std(wave_sum(sq), (float)a.D, a.eps);
-  if (lane == 0) {
-    if (a.mean) a.mean[m] = mean;
-    if (a.rstd) a.rstd[m] = rstd;
+    __syncthreads();
   }
+  for (; m < a.M; m += step) {
+    if (past) shift_back(raw[U - 1], off);
+    float v[U][8];
+    double sum = 0.0;
 #pragma unroll
-  for (int i = 0; i < U; ++i) {
-    const int64_t k0 = (i * 64 + lane) * 8;
-    float d[8];
+    for (int i = 0; i < U; ++i)
 #pragma unroll
-    for (int e = 0; e < 8; ++e) d[e] = k0 + e < a.D ? raw_elem(raw[i], e, DT == SF_BF16) - mean : 0.f;
-    if (HOLD) put_codes(a, m, k0, d);
-    if (k0 < a.D) put_y(a, m, k0, d, rstd);
+      for (int e = 0; e < 8; ++e) {
+        v[i][e] = raw_elem(raw[i], e, bf);
+        sum += (double)v[i][e];
+      }
+    load(m + step);
+    const float mean = (float)(wave_sum_f64(sum) * a.per_d);
+    float sq = 0.f;
+#pragma unroll
+    for (int i = 0; i < U; ++i)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        v[i][e] -= mean;
+        if (i + 1 == U) v[i][e] = last + e < D ? v[i][e] : 0.f;
+        sq = fmaf(v[i][e], v[i][e], sq);
+      }
+    sq = wave_sum(sq);
+    const float rstd = inverse_std(sq, (float)D, a.eps);
+    if constexpr (HOLD) {
+      const bool finite = sq < __builtin_inff();  // so is every element: no NaN or infinity to look for
+      const __amdgpu_buffer_rsrc_t rq = __builtin_amdgcn_make_buffer_rsrc((void*)(a.q + m * a.sq), (short)0, (int)a.kp, (int)SF_RSRC_W3);
+      const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc((void*)(a.scale + m * a.ss), (short)0, 4 * U, (int)SF_RSRC_W3);
+#pragma unroll
+      for (int i = 0; i < U; ++i) {
+        float c[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) c[e] = v[i][e];
+        uint32_t byte;
+        const u32x2 codes = finite ? quantize8_finite(c, byte) : sff8::quantize8(c, byte);
+        __builtin_amdgcn_raw_buffer_store_b64(codes, rq, (i * 64 + lane) * 8, 0, 0);
+        // four blocks a chunk of 64 lanes: their bytes are one word of the row's scales (zero behind the last block)
+        const uint32_t word = (uint32_t)__builtin_amdgcn_readlane((int)byte, 0) | (uint32_t)__builtin_amdgcn_readlane((int)byte, 16) << 8 |
+                              (uint32_t)__builtin_amdgcn_readlane((int)byte, 32) << 16 | (uint32_t)__builtin_amdgcn_readlane((int)byte, 48) << 24;
+        __builtin_amdgcn_raw_buffer_store_b32(word, rs, lane == 0 ? 4 * i : 4 * U, 0, 0);
+      }
+    }
+    char* out = a.y + m * a.sym;
+    const __amdgpu_buffer_rsrc_t ry = __builtin_amdgcn_make_buffer_rsrc((void*)out, (short)0, (D & ~7) * ES, (int)SF_RSRC_W3);
+#pragma unroll
+    for (int i = 0; i < U; ++i) {
+      float y[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) y[e] = v[i][e] * rstd;
+      if (affine) {
+        const int c = i * 64 + lane;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const u32x4 w = s_par[h * CH + c], b = s_par[(2 + h) * CH + c];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) y[4 * h + e] = fmaf(y[4 * h + e], __uint_as_float(w[e]), __uint_as_float(b[e]));
+        }
+      }
+      put8_rsrc<DT>(ry, (i * 64 + lane) * 8, y);
+      if (i + 1 == U && (D & 7) && last < D && last + 8 > D) store8_any(out, DT, last, D, y);
+    }
+    if (lane == 0) {
+      if (a.mean) a.mean[m] = mean;
+      if (a.rstd) a.rstd[m] = rstd;
+    }
   }
 }
 
-// Sum over a block of 1024 threads, in every thread.
+// Sum over a row's NT threads, in every one of them: a wave, or a block of 1024.
+template <int NT>
+__device__ __forceinline__ double row_sum(double v, double*) { return wave_sum_f64(v); }
+template <int NT>
+__device__ __forceinline__ float row_sum(float v, float*) { return wave_sum(v); }
 template <class T>
 __device__ __forceinline__ T block_sum_1024(T v, T* s_w) {
   const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
-#pragma unroll
-  for (int off = 32; off > 0; off >>= 1) v += __shfl_xor(v, off);
+  v = row_sum<64>(v, s_w);
   __syncthreads();  // the last sum has been read
   if (lane == 0) s_w[w] = v;
   __syncthreads();
@@ -228,42 +384,50 @@ __device__ __forceinline__ T block_sum_1024(T v, T* s_w) {
   for (int i = 1; i < 16; ++i) s += s_w[i];
   return s;
 }
+template <>
+__device__ __forceinline__ double row_sum<1024>(double v, double* s) { return block_sum_1024(v, s); }
+template <>
+__device__ __forceinline__ float row_sum<1024>(float v, float* s) { return block_sum_1024(v, s); }
 
-// Rows that no wave can hold: a block a row, which is read three times (out of the caches after the first).
-template <int DT, bool HOLD>
-__global__ __launch_bounds__(1024) void norm_long_kernel(FwdArgs a) {
-  constexpr int ES = DT == SF_F32 ? 4 : 2;
+// Everything else, in three passes over the row, the last two out of the caches: a wave a row where types mix or rows
+// have less than eight elements, a block of 1024 a row where no wave holds it.
+template <int DT, bool HOLD, int NT>
+__global__ __launch_bounds__(NT == 64 ? 256 : 1024) void norm_any_kernel(FwdArgs a) {
+  constexpr int ES = DT == SF_F32 ? 4 : 2, ROWS = NT == 64 ? 4 : 1;
+  constexpr bool bf = DT == SF_BF16;
   __shared__ double s_d[16];
   __shared__ float s_f[16];
-  for (int64_t m = blockIdx.x; m < a.M; m += gridDim.x) {
+  const int t = threadIdx.x % NT;
+  const int64_t first = (int64_t)blockIdx.x * ROWS + (NT == 64 ? (int)__builtin_amdgcn_readfirstlane(threadIdx.x >> 6) : 0);
+  for (int64_t m = first; m < a.M; m += (int64_t)gridDim.x * ROWS) {
     const char* row = a.x + m * a.sxm;
     double sum = 0.0;
-    for (int64_t k0 = threadIdx.x * 8; k0 < a.D; k0 += 8192) {
+    for (int64_t k0 = t * 8; k0 < a.D; k0 += NT * 8) {
       const Raw<ES> r = load_raw<ES>(row, k0, a.D);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) sum += (double)raw_elem(r, e, DT == SF_BF16);
+      for (int e = 0; e < 8; ++e) sum += (double)raw_elem(r, e, bf);
     }
-    const float mean = (float)(block_sum_1024(sum, s_d) / (double)a.D);
+    const float mean = (float)(row_sum<NT>(sum, s_d) * a.per_d);
     float sq = 0.f;
-    for (int64_t k0 = threadIdx.x * 8; k0 < a.D; k0 += 8192) {
+    for (int64_t k0 = t * 8; k0 < a.D; k0 += NT * 8) {
       const Raw<ES> r = load_raw<ES>(row, k0, a.D);
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
-        const float d = k0 + e < a.D ? raw_elem(r, e, DT == SF_BF16) - mean : 0.f;
+        const float d = k0 + e < a.D ? raw_elem(r, e, bf) - mean : 0.f;
         sq = fmaf(d, d, sq);
       }
     }
-    const float rstd = inverse_std(block_sum_1024(sq, s_f), (float)a.D, a.eps);
-    if (threadIdx.x == 0) {
+    const float rstd = inverse_std(row_sum<NT>(sq, s_f), (float)a.D, a.eps);
+    if (t == 0) {
       if (a.mean) a.mean[m] = mean;
       if (a.rstd) a.rstd[m] = rstd;
     }
-    for (int64_t k = 0; k < a.kp; k += 8192) {  // (whole waves: the lanes of a block of codes stay together)
-      const int64_t k0 = k + threadIdx.x * 8;
+    for (int64_t k = 0; k < a.kp; k += NT * 8) {  // (whole waves: the lanes of a block of codes stay together)
+      const int64_t k0 = k + t * 8;
       const Raw<ES> r = load_raw<ES>(row, k0, a.D);
       float d[8];
 #pragma unroll
-      for (int e = 0; e < 8; ++e) d[e] = k0 + e < a.D ? raw_elem(r, e, DT == SF_BF16) - mean : 0.f;
+      for (int e = 0; e < 8; ++e) d[e] = k0 + e < a.D ? raw_elem(r, e, bf) - mean : 0.f;
       if (HOLD) put_codes(a, m, k0, d);
       if (k0 < a.D) put_y(a, m, k0, d, rstd);
     }
@@ -301,6 +465,11 @@ struct XRaw {
   static constexpr int ES = XT == SF_F32 ? 4 : 2;
   Raw<ES> v;
   __device__ __forceinline__ void load(const BwdArgs& a, int64_t m, int64_t k0) { v = load_raw<ES>(a.x + m * a.sxm, k0, a.D); }
+  __device__ __forceinline__ void load_back(const BwdArgs& a, int64_t m, int64_t k0) {
+    v = ::load_back<ES>(a.x + m * a.sxm, k0, a.D);
+  }
+  __device__ __forceinline__ void load_at(const BwdArgs& a, int64_t m, uint32_t k) { v = ::load_at<ES>(a.x + m * a.sxm, k * ES); }
+  __device__ __forceinline__ void shift_back(int off) { ::shift_back(v, off); }
   __device__ __forceinline__ void centred(float mean, float (&d)[8]) const {
 #pragma unroll
     for (int e = 0; e < 8; ++e) d[e] = raw_elem(v, e, XT == SF_BF16) - mean;
@@ -317,6 +486,18 @@ struct XRaw<X_FP8> {
       c = *(const u32x2*)(a.q + m * a.sq + k0);
       byte = a.scale[m * a.ss + k0 / sff8::BLOCK];
     }
+  }
+  __device__ __forceinline__ void load_at(const BwdArgs& a, int64_t m, uint32_t k) {
+    c = *(const u32x2*)(a.q + m * a.sq + k);
+    byte = (a.scale + m * a.ss)[k / sff8::BLOCK];
+  }
+  __device__ __forceinline__ void load_back(const BwdArgs& a, int64_t m, int64_t k0) {
+    const int64_t k = min(k0, (a.D - 1) & ~(int64_t)7);  // a lane past the row's end loads its last chunk
+    c = *(const u32x2*)(a.q + m * a.sq + k);
+    byte = a.scale[m * a.ss + k / sff8::BLOCK];
+  }
+  __device__ __forceinline__ void shift_back(int off) {
+    if (off >= 8) c = u32x2{0, 0};
   }
   __device__ __forceinline__ void centred(float, float (&d)[8]) const {
     const float f = sff8::scale_of(byte);
@@ -337,80 +518,115 @@ __device__ __forceinline__ void put_param(void* p, int dt, int64_t i, float v) {
   else ((u16*)p)[i] = (u16)f32_to_bits(v, dt);
 }
 
-// R rows at a time by a team of T = ceil(D / 512) waves, a lane holding the same eight columns of every row, so
+// A team's column sums: the parameters' gradients if its block is the only one, else its part of them.
+__device__ __forceinline__ void put_sums(const BwdArgs& a, int64_t k0, const float (&acc_w)[8], const float (&acc_b)[8]) {
+  if (gridDim.x == 1) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+      if (k0 + e < a.D) {
+        if (a.dw) put_param(a.dw, a.dw_dt, k0 + e, acc_w[e]);
+        if (a.db) put_param(a.db, a.db_dt, k0 + e, acc_b[e]);
+      }
+  } else if (k0 < a.D) {
+    char* p = (char*)(a.part + (int64_t)blockIdx.x * 2 * a.D);
+    store8_any(p, SF_F32, k0, a.D, acc_w);
+    store8_any(p + a.D * 4, SF_F32, k0, a.D, acc_b);
+  }
+}
+
+// R rows at a time by a team of T <= 8 waves, a lane holding the same U chunks of eight columns of every row, so
 // that the columns' sums stay in its registers over all rows of the block. A row's two sums go over the team
-// through LDS, those of R rows together (one barrier a batch, two buffers). Teams of one or two waves share a
-// block, which adds up its teams' column sums at the end.
-constexpr int R = 4;
-constexpr int MAX_T = 16;
-template <int XT, int GES, bool DX, bool PG>
-__global__ __launch_bounds__(1024) void norm_backward_kernel(BwdArgs a) {
-  __shared__ float s_sum[2][MAX_T][2 * R];
-  __shared__ float s_acc[PG ? 3 * 64 * 16 : 1];
+// through LDS, those of R rows together (one barrier a batch, two buffers), while the next batch's loads are under
+// way. Teams of one or two waves share a block, which adds up its teams' column sums at the end.
+constexpr int MAX_T = 8;
+template <int XT, int GT, int U>
+__global__ __launch_bounds__(64 * MAX_T) void norm_backward_kernel(BwdArgs a) {
+  constexpr int R = 4 / U, GES = GT == SF_F32 ? 4 : 2;
+  constexpr bool bf = GT == SF_BF16;
+  __shared__ float s_sum[2][MAX_T][8];
+  __shared__ float s_acc[U == 1 ? 3 * 64 * 16 : 1];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int team = wave / a.T, tw = wave - team * a.T;
-  const int64_t k0 = (tw * 64 + lane) * 8;
-  const bool live = k0 < a.D, bf = a.g_dt == SF_BF16;
-  float w[8];
-  if (a.w) {
-    load8_any(a.w, a.w_dt, k0, a.D, w);
-  } else {
+  int64_t k0[U];
+  int off[U];
+  float w[U][8], acc_w[U][8], acc_b[U][8];
+  const bool past = (tw + 1) * U * 512 > a.D;  // the wave holds the row's end
 #pragma unroll
-    for (int e = 0; e < 8; ++e) w[e] = 1.f;
+  for (int u = 0; u < U; ++u) {
+    k0[u] = ((tw * U + u) * 64 + lane) * 8;
+    off[u] = (int)max((int64_t)0, k0[u] - (a.D - 8));
+    if (a.w) {
+      load8_any(a.w, a.w_dt, k0[u], a.D, w[u]);
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) w[u][e] = 1.f;
+    }
+#pragma unroll
+    for (int e = 0; e < 8; ++e) acc_w[u][e] = acc_b[u][e] = 0.f;
   }
-  float acc_w[8] = {}, acc_b[8] = {};
   const int64_t batches = (a.M + R - 1) / R, step = (int64_t)gridDim.x * a.TB;
-  Raw<GES> g[R];
-  XRaw<XT> x[R];
+  Raw<GES> g[R][U];
+  XRaw<XT> x[R][U];
+  float stat_r[R], stat_m[R];
   auto load = [&](int64_t batch) {
 #pragma unroll
     for (int r = 0; r < R; ++r) {
       const int64_t m = min(batch * R + r, a.M - 1);  // rows past the last are loaded again and left out below
-      g[r] = load_raw<GES>(a.g + m * a.sgm, k0, a.D);
-      x[r].load(a, m, k0);
+      stat_r[r] = a.rstd[m];
+      stat_m[r] = XT == X_FP8 ? 0.f : a.mean[m];
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        g[r][u] = load_back<GES>(a.g + m * a.sgm, k0[u], a.D);
+        x[r][u].load_back(a, m, k0[u]);
+      }
     }
   };
   int64_t batch = (int64_t)blockIdx.x * a.TB + team;
   load(batch);
   int buf = 0;
   for (int64_t b0 = (int64_t)blockIdx.x * a.TB; b0 < batches; b0 += step, batch += step, buf ^= 1) {
-    Raw<GES> gc[R];
-    XRaw<XT> xc[R];
+    Raw<GES> gc[R][U];
+    XRaw<XT> xc[R][U];
 #pragma unroll
-    for (int r = 0; r < R; ++r) {
-      gc[r] = g[r];
-      xc[r] = x[r];
-    }
+    for (int r = 0; r < R; ++r)
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        gc[r][u] = g[r][u];
+        xc[r][u] = x[r][u];
+        if (past) {
+          shift_back(gc[r][u], off[u]);
+          xc[r][u].shift_back(off[u]);
+        }
+      }
     float rstd[R], mean[R];
 #pragma unroll
     for (int r = 0; r < R; ++r) {
-      const int64_t m = min(batch * R + r, a.M - 1);
-      rstd[r] = a.rstd[m];
-      mean[r] = XT == X_FP8 ? 0.f : a.mean[m];
+      rstd[r] = stat_r[r];
+      mean[r] = stat_m[r];
     }
     load(batch + step);
-    float s[2 * R];
+    float s[8];
+#pragma unroll
+    for (int r = 0; r < 4; ++r) s[2 * r] = s[2 * r + 1] = 0.f;
 #pragma unroll
     for (int r = 0; r < R; ++r) {
-      const bool in = batch * R + r < a.M;  // wave-uniform
-      s[2 * r] = s[2 * r + 1] = 0.f;
-      float d[8];
-      xc[r].centred(mean[r], d);
-      if (in) {
+      if (batch * R + r < a.M) {  // wave-uniform
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const float ge = raw_elem(gc[r], e, bf), xh = d[e] * rstd[r], q = ge * w[e];
-          if (PG) {
-            acc_w[e] = fmaf(ge, xh, acc_w[e]);
-            acc_b[e] += ge;
+        for (int u = 0; u < U; ++u) {
+          float d[8];
+          xc[r][u].centred(mean[r], d);
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            const float ge = raw_elem(gc[r][u], e, bf), xh = d[e] * rstd[r], q = ge * w[u][e];
+            acc_w[u][e] = fmaf(ge, xh, acc_w[u][e]);
+            acc_b[u][e] += ge;
+            s[2 * r] += q;
+            s[2 * r + 1] = fmaf(q, xh, s[2 * r + 1]);
           }
-          s[2 * r] += q;
-          s[2 * r + 1] = fmaf(q, xh, s[2 * r + 1]);
         }
       }
-      if (!live) s[2 * r] = s[2 * r + 1] = 0.f;
     }
-    if constexpr (DX) {
+    if (a.dx) {
       float tot = wave_sum8(s, lane);  // lane l: s[l >> 3]
       if (a.T > 1) {
         if ((lane & 7) == 0) s_sum[buf][wave][lane >> 3] = tot;
@@ -424,28 +640,33 @@ __global__ __launch_bounds__(1024) void norm_backward_kernel(BwdArgs a) {
         const int64_t m = batch * R + r;
         const float c1 = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(per), 16 * r));
         float c2 = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(per), 16 * r + 8));
-        if (m < a.M && live) {
+        if (m < a.M) {
           const float c0 = a.g_mean ? a.g_mean[m] / (float)a.D : 0.f;
           if (a.g_rstd) c2 += a.g_rstd[m] * rstd[r] / (float)a.D;
-          float d[8], o[8];
-          xc[r].centred(mean[r], d);
 #pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            const float q = raw_elem(gc[r], e, bf) * w[e];
-            o[e] = fmaf(rstd[r], q - c1 - d[e] * rstd[r] * c2, c0);
+          for (int u = 0; u < U; ++u) {
+            if (k0[u] >= a.D) continue;
+            float d[8], o[8];
+            xc[r][u].centred(mean[r], d);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+              const float q = raw_elem(gc[r][u], e, bf) * w[u][e];
+              o[e] = fmaf(rstd[r], q - c1 - d[e] * rstd[r] * c2, c0);
+            }
+            store8_any(a.dx + m * a.sdx, a.dx_dt, k0[u], a.D, o);
           }
-          store8_any(a.dx + m * a.sdx, a.dx_dt, k0, a.D, o);
         }
       }
     }
   }
-  if constexpr (PG) {
+  if (!a.dw && !a.db) return;
+  if constexpr (U == 1) {
     if (a.TB > 1) {  // at most 4 waves
       if (team > 0) {
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-          s_acc[(((team - 1) * a.T + tw) * 16 + e) * 64 + lane] = acc_w[e];
-          s_acc[(((team - 1) * a.T + tw) * 16 + 8 + e) * 64 + lane] = acc_b[e];
+          s_acc[(((team - 1) * a.T + tw) * 16 + e) * 64 + lane] = acc_w[0][e];
+          s_acc[(((team - 1) * a.T + tw) * 16 + 8 + e) * 64 + lane] = acc_b[0][e];
         }
       }
       __syncthreads();
@@ -453,24 +674,125 @@ __global__ __launch_bounds__(1024) void norm_backward_kernel(BwdArgs a) {
       for (int t = 0; t < a.TB - 1; ++t) {
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-          acc_w[e] += s_acc[((t * a.T + tw) * 16 + e) * 64 + lane];
-          acc_b[e] += s_acc[((t * a.T + tw) * 16 + 8 + e) * 64 + lane];
+          acc_w[0][e] += s_acc[((t * a.T + tw) * 16 + e) * 64 + lane];
+          acc_b[0][e] += s_acc[((t * a.T + tw) * 16 + 8 + e) * 64 + lane];
         }
       }
     }
-    if (gridDim.x == 1) {
+  }
 #pragma unroll
-      for (int e = 0; e < 8; ++e)
-        if (k0 + e < a.D) {
-          if (a.dw) put_param(a.dw, a.dw_dt, k0 + e, acc_w[e]);
-          if (a.db) put_param(a.db, a.db_dt, k0 + e, acc_b[e]);
-        }
-    } else if (live) {
-      char* p = (char*)(a.part + (int64_t)blockIdx.x * 2 * a.D);
-      store8_any(p, SF_F32, k0, a.D, acc_w);
-      store8_any(p + a.D * 4, SF_F32, k0, a.D, acc_b);
+  for (int u = 0; u < U; ++u) put_sums(a, k0[u], acc_w[u], acc_b[u]);
+}
+
+// The usual case of the above, straight through: x and dx of g's type (or x in 8 bits), up to 4096 elements. What
+// differs is what keeps the loads going. A row's result leaves by a buffer store, whose bounds drop the lanes past
+// the row's last whole chunk and rows past the last without a branch, so that waiting for the next row's loads does not
+// wait for the last row's stores. Elements are unpacked once, into the registers that both halves use, and the
+// sums are those of g (x - mean) and of its product with w: twelve vector instructions an element. One row at a time
+// keeps the registers at 80 (96 in fp32): two blocks of up to ten waves a CU.
+constexpr int FAST_WAVES = 10;
+template <int XT, int GT>
+__global__ __launch_bounds__(64 * FAST_WAVES, GT == SF_F32 ? 5 : 6) void norm_backward_fast_kernel(BwdArgs a) {
+  constexpr int ES = GT == SF_F32 ? 4 : 2;
+  constexpr bool bf = GT == SF_BF16;
+  __shared__ float s_sum[2][FAST_WAVES][2];
+  __shared__ float s_acc[(FAST_WAVES - 1) * 64 * 16];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int team = wave / a.T, tw = wave - team * a.T, D = (int)a.D;
+  const int k0 = (tw * 64 + lane) * 8, off = max(0, k0 - (D - 8));
+  const bool past = (tw + 1) * 512 > D;  // the wave holds the row's end
+  const uint32_t kg = (uint32_t)min(k0, D - 8), kx = XT == X_FP8 ? (uint32_t)min(k0, (D - 1) & ~7) : kg;
+  float w[8], acc_w[8], acc_b[8];
+  if (a.w) {
+    load8_any(a.w, a.w_dt, k0, D, w);
+  } else {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) w[e] = 1.f;
+  }
+#pragma unroll
+  for (int e = 0; e < 8; ++e) acc_w[e] = acc_b[e] = 0.f;
+  const int64_t step = (int64_t)gridDim.x * a.TB;
+  const float per_d = 1.0f / (float)D;
+  Raw<ES> g;
+  XRaw<XT> x;
+  float rstd_n, mean_n;
+  auto load = [&](int64_t row) {
+    const int64_t m = min(row, a.M - 1);  // a team past the last row loads that again, and leaves it out below
+    g = load_at<ES>(a.g + m * a.sgm, kg * ES);
+    x.load_at(a, m, kx);
+    rstd_n = a.rstd[m];
+    mean_n = XT == X_FP8 ? 0.f : a.mean[m];
+  };
+  int64_t m = (int64_t)blockIdx.x * a.TB + team;
+  load(m);
+  int buf = 0;
+  for (int64_t m0 = (int64_t)blockIdx.x * a.TB; m0 < a.M; m0 += step, m += step, buf ^= 1) {
+    const bool in = m < a.M;  // wave-uniform
+    const float rstd = rstd_n;
+    if (past) {
+      shift_back(g, off);
+      x.shift_back(off);
+    }
+    float ge[8], d[8], s1 = 0.f, s2 = 0.f;
+    x.centred(mean_n, d);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      ge[e] = in ? raw_elem(g, e, bf) : 0.f;
+      d[e] = in ? d[e] : 0.f;
+    }
+    load(m + step);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const float t = ge[e] * d[e];
+      acc_w[e] = fmaf(t, rstd, acc_w[e]);
+      acc_b[e] += ge[e];
+      s1 = fmaf(ge[e], w[e], s1);
+      s2 = fmaf(t, w[e], s2);
+    }
+    s1 = wave_sum(s1);
+    s2 = wave_sum(s2);
+    if (a.T > 1) {
+      if (lane == 0) {
+        s_sum[buf][wave][0] = s1;
+        s_sum[buf][wave][1] = s2;
+      }
+      __syncthreads();
+      s1 = s2 = 0.f;
+      for (int t = 0; t < a.T; ++t) {
+        s1 += s_sum[buf][team * a.T + t][0];
+        s2 += s_sum[buf][team * a.T + t][1];
+      }
+    }
+    const float k1 = -rstd * (s1 * per_d), k2 = -rstd * rstd * rstd * (s2 * per_d);
+    float o[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) o[e] = fmaf(d[e], k2, fmaf(ge[e] * w[e], rstd, k1));
+    char* out = a.dx + min(m, a.M - 1) * a.sdx;
+    const __amdgpu_buffer_rsrc_t rs =
+        __builtin_amdgcn_make_buffer_rsrc((void*)out, (short)0, in ? (D & ~7) * ES : 0, (int)SF_RSRC_W3);
+    put8_rsrc<GT>(rs, k0, o);
+    if (past && in && (D & 7) && k0 < D && k0 + 8 > D) store8_any(out, GT, k0, D, o);
+  }
+  if (!a.dw && !a.db) return;
+  if (a.TB > 1) {
+    if (team > 0) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        s_acc[((wave - a.T) * 16 + e) * 64 + lane] = acc_w[e];
+        s_acc[((wave - a.T) * 16 + 8 + e) * 64 + lane] = acc_b[e];
+      }
+    }
+    __syncthreads();
+    if (team > 0) return;
+    for (int t = tw; t < (a.TB - 1) * a.T; t += a.T) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        acc_w[e] += s_acc[(t * 16 + e) * 64 + lane];
+        acc_b[e] += s_acc[(t * 16 + 8 + e) * 64 + lane];
+      }
     }
   }
+  put_sums(a, k0, acc_w, acc_b);
 }
 
 // The parameters' gradients from the blocks' parts, in a fixed order: column c of [2][D] by 16 waves, wave i
@@ -495,11 +817,12 @@ __global__ __launch_bounds__(1024) void norm_params_kernel(const float* part, in
   }
 }
 
-// Rows longer than a team holds: dx by a block a row in two passes ...
-template <int XT, int GES>
+// Rows longer than a team holds, or shorter than eight elements: dx by a block a row in two passes ...
+template <int XT, int GT>
 __global__ __launch_bounds__(1024) void norm_backward_long_kernel(BwdArgs a) {
+  constexpr int GES = GT == SF_F32 ? 4 : 2;
+  constexpr bool bf = GT == SF_BF16;
   __shared__ float s_w[16];
-  const bool bf = a.g_dt == SF_BF16;
   for (int64_t m = blockIdx.x; m < a.M; m += gridDim.x) {
     const float rstd = a.rstd[m], mean = XT == X_FP8 ? 0.f : a.mean[m];
     float s1 = 0.f, s2 = 0.f;
@@ -538,11 +861,12 @@ __global__ __launch_bounds__(1024) void norm_backward_long_kernel(BwdArgs a) {
   }
 }
 // ... and the parameters' gradients by a pass over columns: block (x, y) sums 512 columns a wave over the y-th share of rows.
-template <int XT, int GES>
+template <int XT, int GT>
 __global__ __launch_bounds__(64) void norm_columns_kernel(BwdArgs a) {
   const int64_t k0 = ((int64_t)blockIdx.x * 64 + threadIdx.x) * 8;
   if (k0 >= a.D) return;
-  const bool bf = a.g_dt == SF_BF16;
+  constexpr int GES = GT == SF_F32 ? 4 : 2;
+  constexpr bool bf = GT == SF_BF16;
   float acc_w[8] = {}, acc_b[8] = {};
   for (int64_t m = blockIdx.y; m < a.M; m += gridDim.y) {
     const Raw<GES> g = load_raw<GES>(a.g + m * a.sgm, k0, a.D);
@@ -585,8 +909,9 @@ __device__ __forceinline__ void inverse_pair(float rstd, float& r, float& e) {
 }
 
 // out = h / rstd + mean, a wave a row.
-template <int ES>
-__global__ __launch_bounds__(256) void undo_kernel(UndoArgs a, int h_dt) {
+template <int HT>
+__global__ __launch_bounds__(256) void undo_kernel(UndoArgs a) {
+  constexpr int ES = HT == SF_F32 ? 4 : 2;
   const int lane = threadIdx.x & 63;
   for (int64_t m = (int64_t)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6); m < a.M; m += (int64_t)gridDim.x * 4) {
     float r, c;
@@ -597,7 +922,7 @@ __global__ __launch_bounds__(256) void undo_kernel(UndoArgs a, int h_dt) {
       float o[8];
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
-        const float v = raw_elem(h, e, h_dt == SF_BF16);
+        const float v = raw_elem(h, e, HT == SF_BF16);
         o[e] = fmaf(v, r, fmaf(v, c, mean));
       }
       store8_any(a.out + m * a.som, a.out_dt, k0, a.D, o);
@@ -606,8 +931,9 @@ __global__ __launch_bounds__(256) void undo_kernel(UndoArgs a, int h_dt) {
 }
 
 // dh = g / rstd (out), dmean = sum g, drstd = -sum g h / rstd^2, a wave a row.
-template <int GES, int HES>
-__global__ __launch_bounds__(256) void undo_backward_kernel(UndoArgs a, int g_dt, int h_dt) {
+template <int GT, int HT>
+__global__ __launch_bounds__(256) void undo_backward_kernel(UndoArgs a) {
+  constexpr int GES = GT == SF_F32 ? 4 : 2, HES = HT == SF_F32 ? 4 : 2;
   const int lane = threadIdx.x & 63;
   for (int64_t m = (int64_t)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6); m < a.M; m += (int64_t)gridDim.x * 4) {
     float r, c, s1 = 0.f, s2 = 0.f;
@@ -618,14 +944,14 @@ __global__ __launch_bounds__(256) void undo_backward_kernel(UndoArgs a, int g_dt
         const Raw<HES> h = load_raw<HES>(a.h + m * a.shm, k0, a.D);
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-          const float ge = raw_elem(g, e, g_dt == SF_BF16);
-          s2 = fmaf(ge, raw_elem(h, e, h_dt == SF_BF16), s2);
+          const float ge = raw_elem(g, e, GT == SF_BF16);
+          s2 = fmaf(ge, raw_elem(h, e, HT == SF_BF16), s2);
         }
       }
       float o[8];
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
-        const float ge = raw_elem(g, e, g_dt == SF_BF16);
+        const float ge = raw_elem(g, e, GT == SF_BF16);
         s1 += ge;
         o[e] = fmaf(ge, r, ge * c);
       }
@@ -645,7 +971,9 @@ __global__ __launch_bounds__(256) void undo_backward_kernel(UndoArgs a, int g_dt
 // ------------------------------------------------------------------ host
 constexpr int64_t MAX_M = (1ll << 31) - 1, MAX_D = 1 << 24;
 constexpr int64_t WAVE_D = 4096;          // the longest row a wave of norm_kernel holds
-constexpr int64_t TEAM_D = MAX_T * 512;   // the longest row a team of norm_backward_kernel holds
+constexpr int64_t FWD_BLOCKS = 1024;      // of four waves: four a CU
+constexpr int64_t TEAM_D = MAX_T * 2048;  // the longest row a team of norm_backward_kernel holds, four chunks a lane
+constexpr int64_t FAST_D = 4096;          // the longest of norm_backward_fast_kernel
 constexpr int64_t MOST_PARTS = 512;       // blocks of the backward pass: two a CU
 
 int check_matrix(const char* what, const void* p, int64_t stride, int dt, int64_t M, int64_t D) {
@@ -675,64 +1003,92 @@ int check_shape(int64_t M, int64_t D) {
 
 // Waves of a team, teams of a block and blocks of a backward pass.
 struct BwdPlan {
-  int T, TB;
+  int T, TB, U;
+  bool fast;
   int64_t blocks;
 };
-BwdPlan backward_plan(int64_t M, int64_t D) {
+BwdPlan backward_plan(int64_t M, int64_t D, bool plain) {
   BwdPlan p;
-  if (D > TEAM_D) {
-    p.T = p.TB = 0;
-    p.blocks = std::min<int64_t>(M, 64);
+  p.fast = plain && D >= 8 && D <= FAST_D;
+  if (D > TEAM_D || D < 8) {
+    p.T = p.TB = p.U = 0;
+    p.blocks = std::min<int64_t>(M, 64);  // parts of norm_columns_kernel
     return p;
   }
-  p.T = (int)((D + 511) / 512);
+  p.U = D <= MAX_T * 512 ? 1 : (D <= MAX_T * 1024 ? 2 : 4);
+  p.T = (int)((D + 512 * p.U - 1) / (512 * p.U));
   p.TB = p.T == 1 ? 4 : (p.T == 2 ? 2 : 1);
-  const int64_t batches = (M + R - 1) / R;
+  const int64_t R = p.fast ? 1 : 4 / p.U, batches = (M + R - 1) / R;
+  if (p.fast) p.TB = (int)std::max<int64_t>(1, std::min<int64_t>(FAST_WAVES / p.T, batches));
   p.blocks = std::min<int64_t>(MOST_PARTS, (batches + p.TB - 1) / p.TB);
   return p;
 }
 
 template <int DT, bool HOLD>
 int forward_typed(const FwdArgs& a, hipStream_t s) {
-  const dim3 grid((unsigned)((a.M + 3) / 4));
-#define SF_NORM(UV) hipLaunchKernelGGL((norm_kernel<DT, UV, HOLD>), grid, dim3(256), 0, s, a)
-  switch (a.D > WAVE_D ? 0 : (a.D + 511) / 512) {
-    case 1: SF_NORM(1); break;
-    case 2: SF_NORM(2); break;
-    case 3: SF_NORM(3); break;
-    case 4: SF_NORM(4); break;
-    case 5: SF_NORM(5); break;
-    case 6: SF_NORM(6); break;
-    case 7: SF_NORM(7); break;
-    case 8: SF_NORM(8); break;
-    default:
-      hipLaunchKernelGGL((norm_long_kernel<DT, HOLD>), dim3((unsigned)std::min<int64_t>(a.M, 1 << 16)), dim3(1024), 0, s, a);
-  }
+  const dim3 grid((unsigned)std::min<int64_t>((a.M + 3) / 4, FWD_BLOCKS));
+  if (a.D > WAVE_D) {
+    hipLaunchKernelGGL((norm_any_kernel<DT, HOLD, 1024>), dim3((unsigned)std::min<int64_t>(a.M, 1 << 16)), dim3(1024), 0, s, a);
+  } else if (a.D < 8 || a.y_dt != DT) {
+    hipLaunchKernelGGL((norm_any_kernel<DT, HOLD, 64>), dim3((unsigned)std::min<int64_t>((a.M + 3) / 4, 1 << 16)), dim3(256), 0, s, a);
+  } else {
+#define SF_NORM(UV) case UV: hipLaunchKernelGGL((norm_kernel<DT, UV, HOLD>), grid, dim3(256), 0, s, a); break
+    switch ((a.D + 511) / 512) {
+      SF_NORM(1);
+      SF_NORM(2);
+      SF_NORM(3);
+      SF_NORM(4);
+      SF_NORM(5);
+      SF_NORM(6);
+      SF_NORM(7);
+      SF_NORM(8);
+    }
 #undef SF_NORM
+  }
   SF_LAUNCH_CHECK("norm_kernel");
   return SF_OK;
 }
+template <int DT>
+int forward_of(const FwdArgs& a, hipStream_t s) {
+  return a.q ? forward_typed<DT, true>(a, s) : forward_typed<DT, false>(a, s);
+}
 
-template <int XT, int GES>
+template <int XT, int GT>
 int backward_typed(BwdArgs& a, const BwdPlan& p, hipStream_t s) {
   const bool pg = a.dw || a.db;
   if (p.T) {
     const dim3 grid((unsigned)p.blocks), block((unsigned)(64 * p.T * p.TB));
-    if (a.dx && pg) hipLaunchKernelGGL((norm_backward_kernel<XT, GES, true, true>), grid, block, 0, s, a);
-    else if (a.dx) hipLaunchKernelGGL((norm_backward_kernel<XT, GES, true, false>), grid, block, 0, s, a);
-    else hipLaunchKernelGGL((norm_backward_kernel<XT, GES, false, true>), grid, block, 0, s, a);
+    if constexpr (XT == GT || XT == X_FP8) {
+      if (p.fast) {
+        hipLaunchKernelGGL((norm_backward_fast_kernel<XT, GT>), grid, block, 0, s, a);
+        SF_LAUNCH_CHECK("norm_backward_fast_kernel");
+        return SF_OK;
+      }
+    }
+    if (p.U == 1) hipLaunchKernelGGL((norm_backward_kernel<XT, GT, 1>), grid, block, 0, s, a);
+    else if (p.U == 2) hipLaunchKernelGGL((norm_backward_kernel<XT, GT, 2>), grid, block, 0, s, a);
+    else hipLaunchKernelGGL((norm_backward_kernel<XT, GT, 4>), grid, block, 0, s, a);
     SF_LAUNCH_CHECK("norm_backward_kernel");
     return SF_OK;
   }
   if (a.dx) {
-    hipLaunchKernelGGL((norm_backward_long_kernel<XT, GES>), dim3((unsigned)std::min<int64_t>(a.M, 1 << 16)), dim3(1024), 0, s, a);
+    hipLaunchKernelGGL((norm_backward_long_kernel<XT, GT>), dim3((unsigned)std::min<int64_t>(a.M, 1 << 16)), dim3(1024), 0, s, a);
     SF_LAUNCH_CHECK("norm_backward_long_kernel");
   }
   if (pg) {
-    hipLaunchKernelGGL((norm_columns_kernel<XT, GES>), dim3((unsigned)((a.D + 511) / 512), (unsigned)p.blocks), dim3(64), 0, s, a);
+    hipLaunchKernelGGL((norm_columns_kernel<XT, GT>), dim3((unsigned)((a.D + 511) / 512), (unsigned)p.blocks), dim3(64), 0, s, a);
     SF_LAUNCH_CHECK("norm_columns_kernel");
   }
   return SF_OK;
+}
+
+template <int XT>
+int backward_of(BwdArgs& a, const BwdPlan& p, hipStream_t s) {
+  switch (a.g_dt) {
+    case SF_F32: return backward_typed<XT, SF_F32>(a, p, s);
+    case SF_BF16: return backward_typed<XT, SF_BF16>(a, p, s);
+    default: return backward_typed<XT, SF_F16>(a, p, s);
+  }
 }
 
 }  // namespace
@@ -753,14 +1109,15 @@ extern "C" int sf_layer_norm(const void* x, int64_t sxm, int x_dt, const void* w
   const int es = sf_dtype_size(x_dt);
   FwdArgs a;
   a.x = (const char*)x; a.sxm = sxm * es; a.w = w; a.b = b; a.w_dt = w_dt; a.b_dt = b_dt; a.eps = eps;
+  a.per_d = 1.0 / (double)D;
   a.M = M; a.D = D; a.y = (char*)y; a.sym = sym * sf_dtype_size(y_dt); a.y_dt = y_dt; a.mean = mean; a.rstd = rstd;
   a.q = (uint8_t*)q; a.sq = sq; a.scale = (uint8_t*)scale; a.ss = ss; a.kp = sff8::code_bytes(D);
   a.pad = (int)(sff8::scale_bytes(D) - sff8::blocks_of(D));
   hipStream_t s = (hipStream_t)stream;
   switch (x_dt) {
-    case SF_F32: return q ? forward_typed<SF_F32, true>(a, s) : forward_typed<SF_F32, false>(a, s);
-    case SF_BF16: return q ? forward_typed<SF_BF16, true>(a, s) : forward_typed<SF_BF16, false>(a, s);
-    default: return q ? forward_typed<SF_F16, true>(a, s) : forward_typed<SF_F16, false>(a, s);
+    case SF_F32: return forward_of<SF_F32>(a, s);
+    case SF_BF16: return forward_of<SF_BF16>(a, s);
+    default: return forward_of<SF_F16>(a, s);
   }
 }
 
@@ -768,7 +1125,7 @@ extern "C" int sf_layer_norm_backward_workspace_size(int64_t M, int64_t D, int64
   sf_clear_error();
   if (const int rc = check_shape(M, D)) return rc;
   SF_REQUIRE(bytes, "sf_layer_norm_backward_workspace_size: NULL result");
-  *bytes = backward_plan(M, D).blocks * 2 * D * (int64_t)sizeof(float);
+  *bytes = std::max(backward_plan(M, D, false).blocks, backward_plan(M, D, true).blocks) * 2 * D * (int64_t)sizeof(float);
   return SF_OK;
 }
 
@@ -783,8 +1140,8 @@ extern "C" int sf_layer_norm_backward(const void* g, int64_t sgm, int g_dt, cons
   SF_REQUIRE((!w || sf_valid_dtype(w_dt)) && (!dw || sf_valid_dtype(dw_dt)) && (!db || sf_valid_dtype(db_dt)),
              "unsupported dtype code");
   hipStream_t s = (hipStream_t)stream;
-  const BwdPlan p = backward_plan(M, D);
-  const bool pg = dw || db;
+  const bool pg = dw || db, plain = dx && dx_dt == g_dt && (!x || x_dt == g_dt) && !g_mean && !g_rstd;
+  const BwdPlan p = backward_plan(M, D, plain);
   if (M > 0) {
     if (const int rc = check_matrix("g", g, sgm, g_dt, M, D)) return rc;
     SF_REQUIRE((x != nullptr) != (q != nullptr), "the input is given as x or in 8 bits, not both");
@@ -808,14 +1165,12 @@ extern "C" int sf_layer_norm_backward(const void* g, int64_t sgm, int g_dt, cons
     a.mean = mean; a.rstd = rstd; a.w = w; a.w_dt = w_dt; a.g_mean = g_mean; a.g_rstd = g_rstd; a.M = M; a.D = D;
     a.dx = (char*)dx; a.sdx = dx ? sdx * sf_dtype_size(dx_dt) : 0; a.dx_dt = dx_dt;
     a.dw = dw; a.db = db; a.dw_dt = dw_dt; a.db_dt = db_dt; a.part = (float*)workspace; a.T = p.T; a.TB = p.TB;
-    const int xt = x ? x_dt : X_FP8;
-    const bool g4 = g_dt == SF_F32;
     int rc;
-    switch (xt) {
-      case SF_F32: rc = g4 ? backward_typed<SF_F32, 4>(a, p, s) : backward_typed<SF_F32, 2>(a, p, s); break;
-      case SF_BF16: rc = g4 ? backward_typed<SF_BF16, 4>(a, p, s) : backward_typed<SF_BF16, 2>(a, p, s); break;
-      case SF_F16: rc = g4 ? backward_typed<SF_F16, 4>(a, p, s) : backward_typed<SF_F16, 2>(a, p, s); break;
-      default: rc = g4 ? backward_typed<X_FP8, 4>(a, p, s) : backward_typed<X_FP8, 2>(a, p, s);
+    switch (x ? x_dt : X_FP8) {
+      case SF_F32: rc = backward_of<SF_F32>(a, p, s); break;
+      case SF_BF16: rc = backward_of<SF_BF16>(a, p, s); break;
+      case SF_F16: rc = backward_of<SF_F16>(a, p, s); break;
+      default: rc = backward_of<X_FP8>(a, p, s);
     }
     if (rc) return rc;
   }
@@ -839,8 +1194,12 @@ extern "C" int sf_denormalize(const void* h, int64_t shm, int h_dt, const float*
   a.h = (const char*)h; a.shm = shm * sf_dtype_size(h_dt); a.mean = mean; a.rstd = rstd; a.M = M; a.D = D;
   a.out = (char*)out; a.som = som * sf_dtype_size(out_dt); a.out_dt = out_dt;
   const dim3 grid((unsigned)std::min<int64_t>((M + 3) / 4, 1 << 20));
-  if (h_dt == SF_F32) hipLaunchKernelGGL(undo_kernel<4>, grid, dim3(256), 0, (hipStream_t)stream, a, h_dt);
-  else hipLaunchKernelGGL(undo_kernel<2>, grid, dim3(256), 0, (hipStream_t)stream, a, h_dt);
+  hipStream_t s = (hipStream_t)stream;
+  switch (h_dt) {
+    case SF_F32: hipLaunchKernelGGL(undo_kernel<SF_F32>, grid, dim3(256), 0, s, a); break;
+    case SF_BF16: hipLaunchKernelGGL(undo_kernel<SF_BF16>, grid, dim3(256), 0, s, a); break;
+    default: hipLaunchKernelGGL(undo_kernel<SF_F16>, grid, dim3(256), 0, s, a);
+  }
   SF_LAUNCH_CHECK("undo_kernel");
   return SF_OK;
 }
@@ -863,14 +1222,19 @@ extern "C" int sf_denormalize_backward(const void* g, int64_t sgm, int g_dt, con
   a.h = drstd ? (const char*)h : nullptr; a.shm = drstd ? shm * sf_dtype_size(h_dt) : 0;
   a.out = (char*)dh; a.som = dh ? sdh * sf_dtype_size(dh_dt) : 0; a.out_dt = dh_dt; a.dmean = dmean; a.drstd = drstd;
   const dim3 grid((unsigned)std::min<int64_t>((M + 3) / 4, 1 << 20));
-  const bool g4 = g_dt == SF_F32, h4 = drstd && h_dt == SF_F32;
   hipStream_t s = (hipStream_t)stream;
-  if (g4) {
-    if (h4) hipLaunchKernelGGL((undo_backward_kernel<4, 4>), grid, dim3(256), 0, s, a, g_dt, h_dt);
-    else hipLaunchKernelGGL((undo_backward_kernel<4, 2>), grid, dim3(256), 0, s, a, g_dt, h_dt);
-  } else {
-    if (h4) hipLaunchKernelGGL((undo_backward_kernel<2, 4>), grid, dim3(256), 0, s, a, g_dt, h_dt);
-    else hipLaunchKernelGGL((undo_backward_kernel<2, 2>), grid, dim3(256), 0, s, a, g_dt, h_dt);
+  auto typed = [&](auto g_tag) {
+    constexpr int GT = decltype(g_tag)::value;
+    switch (drstd ? h_dt : GT) {
+      case SF_F32: hipLaunchKernelGGL((undo_backward_kernel<GT, SF_F32>), grid, dim3(256), 0, s, a); break;
+      case SF_BF16: hipLaunchKernelGGL((undo_backward_kernel<GT, SF_BF16>), grid, dim3(256), 0, s, a); break;
+      default: hipLaunchKernelGGL((undo_backward_kernel<GT, SF_F16>), grid, dim3(256), 0, s, a);
+    }
+  };
+  switch (g_dt) {
+    case SF_F32: typed(std::integral_constant<int, SF_F32>{}); break;
+    case SF_BF16: typed(std::integral_constant<int, SF_BF16>{}); break;
+    default: typed(std::integral_constant<int, SF_F16>{});
   }
   SF_LAUNCH_CHECK("undo_backward_kernel");
   return SF_OK;

@@ -63,9 +63,16 @@ class Fp8Rows:
     @classmethod
     def empty(cls, rows, d, device="cuda"):
         """Room for `rows` rows, uninitialised."""
+        if rows < 0 or d < 1:
+            raise ValueError(f"no room to be made for {rows} rows of {d}")
         kp = _up(d, BLOCK)
-        return cls(torch.empty(rows, kp, dtype=torch.float8_e4m3fn, device=device),
-                   torch.empty(rows, _up(kp // BLOCK, 4), dtype=torch.uint8, device=device), d)
+        sp = _up(kp // BLOCK, 4)
+        q = torch.empty((rows, kp), dtype=torch.float8_e4m3fn, device=device)
+        made = object.__new__(cls)  # (of the right shapes: __init__'s checks would cost 1 us)
+        for name, value in (("q", q), ("scale", torch.empty((rows, sp), dtype=torch.uint8, device=q.device)), ("d", d),
+                            ("_strides", (kp, sp))):
+            object.__setattr__(made, name, value)
+        return made
 
     @classmethod
     def from_parts(cls, codes, scale):

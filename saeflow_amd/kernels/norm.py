@@ -6,6 +6,8 @@ The reference has no counterpart: its dictionaries read activations as they come
 
 The mean is summed in 64 bits, all else in 32; results are rounded once to their type. What the backward pass needs of
 x is x itself or, from layer_norm_held, x - mean as 8-bit rows (kernels.Fp8Rows), a little over a byte an element.
+
+A call on few rows is bound by the host (a launch takes 3 us, a tensor made 1 to 1.4), so the wrappers make few objects.
 """
 
 from types import SimpleNamespace
@@ -16,14 +18,21 @@ from .. import _lib
 from .encode import _vector
 from .fp8 import Fp8Rows
 
+_DTYPE = _lib.DTYPE
+
 
 def _matrix(t, name):
-    """t [M, D] with unit column stride (a copy only where it has another)."""
+    """t [M, D] with unit column stride (a copy only where it has another), M, D and the row stride."""
     if t.dim() != 2:
         raise ValueError(f"{name} must have two dimensions, got {list(t.shape)}")
-    if t.shape[1] < 1:
+    M, D = t.shape
+    if D < 1:
         raise ValueError(f"{name} has rows of no elements")
-    return t if t.stride(1) == 1 or t.shape[1] == 1 else t.contiguous()
+    row, col = t.stride()
+    if col != 1 and D > 1:
+        t = t.contiguous()
+        row = D
+    return t, M, D, row
 
 
 def _param(t, n, name):
@@ -31,37 +40,73 @@ def _param(t, n, name):
     if t is None:
         return None, None, 0
     t = _vector(t, n, name)
-    return t, t.data_ptr(), _lib.dtype_code(t, name)
+    code = _DTYPE.get(t.dtype)
+    return t, t.data_ptr(), _lib.dtype_code(t, name) if code is None else code
+
+
+def _code(t, name):
+    code = _DTYPE.get(t.dtype)
+    return _lib.dtype_code(t, name) if code is None else code
 
 
 def _row_stat(t, M, name):
-    if t.dtype != torch.float32 or t.dim() != 1 or t.numel() != M:
+    if t.dtype != torch.float32 or t.dim() != 1 or t.shape[0] != M:
         raise ValueError(f"{name} must be a float32 tensor of shape [{M}], got {t.dtype} {list(t.shape)}")
     return t.contiguous()
 
 
+def _gpu(first, *named):
+    """first's device number, which the other tensors (or None) have to share; require_gpu's errors."""
+    at = first.get_device()
+    if at >= 0:
+        for _, t in named:
+            if t is not None and t.get_device() != at:
+                break
+        else:
+            return at
+    _lib.require_gpu(("rows", first), *named)
+    raise ValueError("the tensors are on different devices")
+
+
+def _result(like, M, D, dtype):
+    """Room for [M, D], contiguous."""
+    return torch.empty_like(like) if like.dtype == dtype and like.is_contiguous() else like.new_empty((M, D), dtype=dtype)
+
+
+def _run(fn, at, *args):
+    """The C call on torch's current stream, with GPU `at` current."""
+    stream = torch._C._cuda_getCurrentRawStream(at)
+    if torch._C._cuda_getDevice() == at:
+        rc = fn(*args, stream)
+    else:
+        with torch.cuda.device(at):
+            rc = fn(*args, stream)
+    if rc:
+        _lib.check(rc)
+
+
 def _forward(x, weight, bias, eps, out_dtype, stats, hold):
-    x = _matrix(x, "x")
-    M, D = x.shape
+    x, M, D, row = _matrix(x, "x")
     if not eps >= 0.0:
         raise ValueError(f"eps must not be negative, got {eps}")
     w, w_ptr, w_code = _param(weight, D, "weight")
     b, b_ptr, b_code = _param(bias, D, "bias")
-    dev = _lib.require_gpu(("x", x), ("weight", w), ("bias", b))
-    x_code = _lib.dtype_code(x, "x")
-    y = torch.empty((M, D), dtype=out_dtype or x.dtype, device=dev)
-    y_code = _lib.dtype_code(y, "out_dtype")
-    both = torch.empty((2, M), dtype=torch.float32, device=dev) if stats else None
-    held = Fp8Rows.empty(M, D, dev) if hold else None
+    at = _gpu(x, ("weight", w), ("bias", b))
+    x_code = _code(x, "x")
+    y = _result(x, M, D, out_dtype or x.dtype)
+    y_code = _code(y, "out_dtype")
+    both, mean, rstd = None, None, None
+    if stats:
+        both = x.new_empty((2, M), dtype=torch.float32)
+        mean = both.data_ptr()
+        rstd = mean + 4 * M
+    held, q = None, (None, 0, None, 0)
+    if hold:
+        held = Fp8Rows.empty(M, D, x.device)
+        q = held._args()
     if M:
-        at = None if both is None else both.data_ptr()
-        q = held._args() if hold else (None, 0, None, 0)
-        with _lib.device(dev):
-            rc = _lib.load().sf_layer_norm(x.data_ptr(), x.stride(0), x_code, w_ptr, w_code, b_ptr, b_code, eps, M, D,
-                                           y.data_ptr(), D, y_code, at, None if at is None else at + 4 * M, *q,
-                                           _lib.stream(dev))
-        if rc:
-            _lib.check(rc)
+        _run(_lib.load().sf_layer_norm, at, x.data_ptr(), row, x_code, w_ptr, w_code, b_ptr, b_code, eps, M, D,
+             y.data_ptr(), D, y_code, mean, rstd, *q)
     return y, held, both
 
 
@@ -69,14 +114,14 @@ def layer_norm(x, weight=None, bias=None, eps=1e-5, *, out_dtype=None):
     """(y, mean, rstd) of the rows of x [M, D] in fp32, bf16 or fp16: y in out_dtype (x's own by default), mean and
     rstd float32 [M]. weight and bias [D], either None, in any of the three types."""
     y, _, stats = _forward(x, weight, bias, eps, out_dtype, True, False)
-    return y, stats[0], stats[1]
+    return y, *stats.unbind()
 
 
 def layer_norm_held(x, weight=None, bias=None, eps=1e-5, *, out_dtype=None):
     """(y, held, mean, rstd): layer_norm that also leaves x - mean in 8 bits (Fp8Rows), written in the same pass,
     which layer_norm_backward takes in place of x."""
     y, held, stats = _forward(x, weight, bias, eps, out_dtype, True, True)
-    return y, held, stats[0], stats[1]
+    return y, held, *stats.unbind()
 
 
 def layer_norm_backward(grad_y, x, mean, rstd, weight=None, bias=None, *, need_grad_x=True, grad_mean=None,
@@ -89,87 +134,86 @@ def layer_norm_backward(grad_y, x, mean, rstd, weight=None, bias=None, *, need_g
       used. out_dtype: of the gradient of x; x's own by default, grad_y's for Fp8Rows.
     fp32 sums in a fixed order: repeated calls give identical bits. Nothing waits for the GPU.
     """
-    g = _matrix(grad_y, "grad_y")
-    M, D = g.shape
+    g, M, D, g_row = _matrix(grad_y, "grad_y")
     held = isinstance(x, Fp8Rows)
     if tuple(x.shape) != (M, D):
         raise ValueError(f"grad_y has shape {[M, D]}, x {list(x.shape)}")
-    if not held:
-        x = _matrix(x, "x")
+    if held:
+        mean = mean_ptr = None
+        x_args, first = (None, 0, 0, *x._args()), x.q
+    else:
+        x, _, _, x_row = _matrix(x, "x")
+        mean = _row_stat(mean, M, "mean")
+        mean_ptr = mean.data_ptr()
+        x_args, first = (x.data_ptr(), x_row, _code(x, "x"), None, 0, None, 0), x
     rstd = _row_stat(rstd, M, "rstd")
-    mean = None if held else _row_stat(mean, M, "mean")
-    grad_mean = None if grad_mean is None else _row_stat(grad_mean, M, "grad_mean")
-    grad_rstd = None if grad_rstd is None else _row_stat(grad_rstd, M, "grad_rstd")
+    gm = gr = gm_ptr = gr_ptr = None
+    if grad_mean is not None:
+        gm = _row_stat(grad_mean, M, "grad_mean")
+        gm_ptr = gm.data_ptr()
+    if grad_rstd is not None:
+        gr = _row_stat(grad_rstd, M, "grad_rstd")
+        gr_ptr = gr.data_ptr()
     w, w_ptr, w_code = _param(weight, D, "weight")
-    if bias is not None and (bias.dim() != 1 or bias.numel() != D):
-        raise ValueError(f"bias must have shape [{D}], got {list(bias.shape)}")
-    dev = _lib.require_gpu(("grad_y", g), ("x", x.q if held else x), ("mean", mean), ("rstd", rstd), ("weight", w),
-                           ("bias", bias), ("grad_mean", grad_mean), ("grad_rstd", grad_rstd))
-    g_code = _lib.dtype_code(g, "grad_y")
-    x_args = (None, 0, 0, *x._args()) if held else (x.data_ptr(), x.stride(0), _lib.dtype_code(x, "x"), None, 0, None, 0)
-    dx = dx_ptr = dw = dw_ptr = db = db_ptr = None
-    dx_code = db_code = 0
+    b, _, b_code = _param(bias, D, "bias")
+    at = _gpu(g, ("x", first), ("mean", mean), ("rstd", rstd), ("weight", w), ("bias", b), ("grad_mean", gm),
+              ("grad_rstd", gr))
+    g_code = _code(g, "grad_y")
+    dx = dx_ptr = dw = dw_ptr = db = db_ptr = ws = ws_ptr = None
+    dx_code = nbytes = 0
     if need_grad_x:
-        dx = torch.empty((M, D), dtype=out_dtype or (g.dtype if held else x.dtype), device=dev)
-        dx_ptr, dx_code = dx.data_ptr(), _lib.dtype_code(dx, "out_dtype")
+        dx = _result(g if held else x, M, D, out_dtype or (g if held else x).dtype)
+        dx_ptr, dx_code = dx.data_ptr(), _code(dx, "out_dtype")
     if w is not None:
-        dw = torch.empty(D, dtype=w.dtype, device=dev)
+        dw = torch.empty_like(w)
         dw_ptr = dw.data_ptr()
-    if bias is not None:
-        db = torch.empty(D, dtype=bias.dtype, device=dev)
-        db_ptr, db_code = db.data_ptr(), _lib.dtype_code(db, "bias")
-    with _lib.device(dev):
-        ws = None
-        if dw is not None or db is not None:
-            ws = torch.empty(_lib.layer_norm_workspace_bytes(M, D), dtype=torch.uint8, device=dev)
-        rc = _lib.load().sf_layer_norm_backward(
-            g.data_ptr(), g.stride(0), g_code, *x_args, _lib.ptr(mean), rstd.data_ptr(), w_ptr, w_code,
-            _lib.ptr(grad_mean), _lib.ptr(grad_rstd), M, D, dx_ptr, D, dx_code, dw_ptr, w_code, db_ptr, db_code,
-            _lib.ptr(ws), 0 if ws is None else ws.numel(), _lib.stream(dev))
-    if rc:
-        _lib.check(rc)
+    if b is not None:
+        db = torch.empty_like(b)
+        db_ptr = db.data_ptr()
+    if dw is not None or db is not None:
+        nbytes = _lib.layer_norm_workspace_bytes(M, D)
+        if nbytes:
+            ws = g.new_empty(nbytes, dtype=torch.uint8)
+            ws_ptr = ws.data_ptr()
+    _run(_lib.load().sf_layer_norm_backward, at, g.data_ptr(), g_row, g_code, *x_args, mean_ptr, rstd.data_ptr(),
+         w_ptr, w_code, gm_ptr, gr_ptr, M, D, dx_ptr, D, dx_code, dw_ptr, w_code, db_ptr, b_code, ws_ptr, nbytes)
     return SimpleNamespace(x=dx, weight=dw, bias=db)
 
 
 def denormalize(h, mean, rstd, *, out_dtype=None):
     """h / rstd + mean per row of h [M, D]: layer_norm (without weight and bias) undone, which carries a reconstruction
     of normed rows back to the rows' own space. In fp32, rounded once to out_dtype (h's own by default)."""
-    h = _matrix(h, "h")
-    M, D = h.shape
+    h, M, D, row = _matrix(h, "h")
     mean, rstd = _row_stat(mean, M, "mean"), _row_stat(rstd, M, "rstd")
-    dev = _lib.require_gpu(("h", h), ("mean", mean), ("rstd", rstd))
-    h_code = _lib.dtype_code(h, "h")
-    out = torch.empty((M, D), dtype=out_dtype or h.dtype, device=dev)
-    out_code = _lib.dtype_code(out, "out_dtype")
-    with _lib.device(dev):
-        rc = _lib.load().sf_denormalize(h.data_ptr(), h.stride(0), h_code, mean.data_ptr(), rstd.data_ptr(), M, D,
-                                        out.data_ptr(), D, out_code, _lib.stream(dev))
-    if rc:
-        _lib.check(rc)
+    at = _gpu(h, ("mean", mean), ("rstd", rstd))
+    h_code = _code(h, "h")
+    out = _result(h, M, D, out_dtype or h.dtype)
+    _run(_lib.load().sf_denormalize, at, h.data_ptr(), row, h_code, mean.data_ptr(), rstd.data_ptr(), M, D,
+         out.data_ptr(), D, _code(out, "out_dtype"))
     return out
 
 
 def denormalize_backward(grad, h, rstd, *, need_grad_stats=True, out_dtype=None):
     """(dh, dmean, drstd) of denormalize from grad [M, D]: dh in out_dtype (h's own by default), the other two float32
     [M], or None without need_grad_stats (then h is not read and may be None, dh in grad's type by default)."""
-    g = _matrix(grad, "grad")
-    M, D = g.shape
+    g, M, D, g_row = _matrix(grad, "grad")
     if h is None and need_grad_stats:
         raise ValueError("the gradients of mean and rstd need h")
-    h = None if h is None else _matrix(h, "h")
-    if h is not None and tuple(h.shape) != (M, D):
-        raise ValueError(f"grad has shape {[M, D]}, h {list(h.shape)}")
+    h_args = (None, 0, 0)
+    if h is not None:
+        if tuple(h.shape) != (M, D):
+            raise ValueError(f"grad has shape {[M, D]}, h {list(h.shape)}")
+        h, _, _, h_row = _matrix(h, "h")
+        h_args = (h.data_ptr(), h_row, _code(h, "h"))
     rstd = _row_stat(rstd, M, "rstd")
-    dev = _lib.require_gpu(("grad", g), ("h", h), ("rstd", rstd))
-    g_code = _lib.dtype_code(g, "grad")
-    h_args = (None, 0, 0) if h is None else (h.data_ptr(), h.stride(0), _lib.dtype_code(h, "h"))
-    dh = torch.empty((M, D), dtype=out_dtype or (g if h is None else h).dtype, device=dev)
-    dh_code = _lib.dtype_code(dh, "out_dtype")
-    stats = torch.empty((2, M), dtype=torch.float32, device=dev) if need_grad_stats else None
-    at = None if stats is None else stats.data_ptr()
-    with _lib.device(dev):
-        rc = _lib.load().sf_denormalize_backward(g.data_ptr(), g.stride(0), g_code, *h_args, rstd.data_ptr(), M, D,
-                                                 dh.data_ptr(), D, dh_code, at, None if at is None else at + 4 * M, _lib.stream(dev))
-    if rc:
-        _lib.check(rc)
-    return (dh, None, None) if stats is None else (dh, stats[0], stats[1])
+    at = _gpu(g, ("h", h), ("rstd", rstd))
+    g_code = _code(g, "grad")
+    dh = _result(g, M, D, out_dtype or (g if h is None else h).dtype)
+    stats = dmean = drstd = None
+    if need_grad_stats:
+        stats = g.new_empty((2, M), dtype=torch.float32)
+        dmean = stats.data_ptr()
+        drstd = dmean + 4 * M
+    _run(_lib.load().sf_denormalize_backward, at, g.data_ptr(), g_row, g_code, *h_args, rstd.data_ptr(), M, D,
+         dh.data_ptr(), D, _code(dh, "out_dtype"), dmean, drstd)
+    return (dh, None, None) if stats is None else (dh, *stats.unbind())
