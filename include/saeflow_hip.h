@@ -372,6 +372,16 @@ SF_API int sf_backward_columns(const int64_t* colptr, const int32_t* csc_row, co
                         int64_t nnz, float* g_pre, void* d_wdec, void* d_wenc, float* d_benc,
                         float* partials, float* work, int64_t work_floats, void* stream);
 
+/* sf_backward_columns with x' as 8-bit rows (sf_quantize_rows of x - b_dec; see "Rows in 8 bits") in place of xs, of any
+ * D; everything else as there. No reference counterpart. */
+SF_API int sf_backward_columns_held(const int64_t* colptr, const int32_t* csc_row, const int32_t* csc_pos,
+                        const int64_t* plan_i64, const int32_t* item_col, const int32_t* multi_col,
+                        const int32_t* slot_item, int64_t max_items, int64_t max_slots, const void* values,
+                        int val_dt, const void* g_val, int gval_dt, const void* w_dec, int64_t sw, const void* xq,
+                        int64_t sxq, const void* xscale, int64_t sxs, const void* g_xhat, int64_t sg, int dt,
+                        int64_t N, int64_t M, int64_t D, int64_t nnz, float* g_pre, void* d_wdec, void* d_wenc,
+                        float* d_benc, float* partials, float* work, int64_t work_floats, void* stream);
+
 /* dst [C, R] (contiguous) = transpose of src [R, C] (row stride ss), dtype dt. skip_ptr: NULL,
  * or int64 [R+1] offsets (a CSC colptr) under which a source row r with skip_ptr[r+1] ==
  * skip_ptr[r] reads as zeros and is not accessed (rows of unused features). */

@@ -24,6 +24,7 @@
 #include <type_traits>
 
 #include "common.h"
+#include "fp8.h"
 #include "wave.h"
 
 namespace {
@@ -470,6 +471,10 @@ struct ColArgs {
   float* d_benc;  // [N]
   float* part;    // [slots, 2, D] fp32, then [slots] fp32 for b_enc
   int64_t n_slots;
+  const uint8_t* xq;  // x' as 8-bit rows in place of xs (fp8.h): codes of stride sxq, scale bytes of stride sxs
+  int64_t sxq;
+  const uint8_t* xscale;
+  int64_t sxs;
   const int4* rec;  // [n_items] what a wave needs of each work item (item_records_kernel), or NULL
 };
 
@@ -583,6 +588,58 @@ __device__ __forceinline__ float chunk_dot(const u32x4& x, const u32x4& y) {
   return d;
 }
 
+enum Held { HELD_NO = 0, HELD_NEAR = 1, HELD_FAR = 2 };
+
+// x' held in 8 bits: a lane's EPC codes of a row, and the word with the scale bytes of the row's slab (a slab of 64
+// chunks is four blocks of 128 in 16-bit types, two in fp32, so its bytes never cross a word). The words of 64
+// entries are one load of a lane each, as their rows are; a gathered row is then half (fp32: a quarter) of what x' in its own
+// type takes from L2. Rows are padded to whole blocks, so a chunk that holds one element of a row can be read.
+template <int DT>
+struct HeldChunk {
+  static constexpr int EPC = DT == SF_F32 ? 4 : 8;
+  typename std::conditional<DT == SF_F32, uint32_t, sff8::u32x2>::type q;
+  // the codes from k on of a wave-uniform row: HELD_NEAR at a byte offset of 32 bits, which entries() has ready,
+  // HELD_FAR (4 GB of codes and more) by its number
+  template <int HELD>
+  __device__ __forceinline__ void load(const ColArgs& a, __amdgpu_buffer_rsrc_t rs, int at, uint32_t k) {
+    if constexpr (HELD == HELD_FAR) q = *(const decltype(q)*)(a.xq + (int64_t)at * a.sxq + k);
+    else if constexpr (DT == SF_F32) q = (uint32_t)__builtin_amdgcn_raw_buffer_load_b32(rs, (int)k, at, 0);
+    else q = __builtin_bit_cast(sff8::u32x2, __builtin_amdgcn_raw_buffer_load_b64(rs, (int)k, at, 0));
+  }
+  // What the walk over a wave's 64 entries reads of each with readlane: where its row lies, its scale word and its
+  // scalar. Lanes without an entry take the last one's row with a scalar of zero, so the walk needs no bounds.
+  template <int HELD>
+  static __device__ __forceinline__ void entries(const ColArgs& a, int slab, int kn, int lane, int& my_row, uint32_t& my_word) {
+    my_row = lane < kn ? my_row : __builtin_amdgcn_readlane(my_row, max(kn - 1, 0));
+    my_word = word(a, my_row, slab);
+    if constexpr (HELD == HELD_NEAR) my_row = (int)((uint32_t)my_row * (uint32_t)a.sxq);
+  }
+  // where in the slab's word a lane's scale byte lies
+  static __device__ __forceinline__ int shift(int slab, int lane) {
+    return DT == SF_F32 ? ((slab & 1) * 2 + (lane >> 5)) * 8 : (lane >> 4) * 8;
+  }
+  static __device__ __forceinline__ uint32_t word(const ColArgs& a, int row, int slab) {
+    return *(const uint32_t*)(a.xscale + (int64_t)row * a.sxs + (DT == SF_F32 ? (slab >> 1) * 4 : slab * 4));
+  }
+  // acc += s * element; the conversion multiplies by the power of two (v_cvt_scalef32_pk_f32_fp8, which takes the
+  // exponent of its scale: bits byte << 23)
+  __device__ __forceinline__ void add(float s, uint32_t word, int shift, float (&acc)[EPC]) const {
+    const float two = __uint_as_float(((word >> shift) & 0xffu) << 23);
+#pragma unroll
+    for (int i = 0; i < EPC / 4; ++i) {
+      uint32_t c;
+      if constexpr (DT == SF_F32) c = q;
+      else c = q[i];
+      const sff8::f32x2 lo = __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(c, two, false);
+      const sff8::f32x2 hi = __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(c, two, true);
+      acc[4 * i] = fmaf(s, lo[0], acc[4 * i]);
+      acc[4 * i + 1] = fmaf(s, lo[1], acc[4 * i + 1]);
+      acc[4 * i + 2] = fmaf(s, hi[0], acc[4 * i + 2]);
+      acc[4 * i + 3] = fmaf(s, hi[1], acc[4 * i + 3]);
+    }
+  }
+};
+
 // Final row chunk of a one-chunk column, or this chunk's fp32 partial (half 0: dW_dec, 1: dW_enc^T).
 template <int DT, bool VEC>
 __device__ __forceinline__ void put_rows(const ColArgs& a, const Item& it, char* out, int half, int64_t c,
@@ -619,7 +676,8 @@ __device__ __forceinline__ void put_rows(const ColArgs& a, const Item& it, char*
 // chunk instead of branching around the load, their sums are never stored and their phase-A
 // dot shares are zeroed (a load past the buffer's end, as with D = 0, returns zeros). U rows
 // in flight. Surplus waves (the grid may be sized by a bound of the item count) return at once.
-template <int DT, bool VEC, int U, bool DEC, int G, bool LIST>
+// HELD (phase B): x' comes as 8-bit rows. (With G = 1 a wave has one item, and no end to look for among its entries.)
+template <int DT, bool VEC, int U, bool DEC, int G, bool LIST, int HELD = HELD_NO>
 __global__ __launch_bounds__(256) void backward_units_kernel(ColArgs a, int nslab, int slab_major) {
   constexpr int ES = DT == SF_F32 ? 4 : 2, EPC = 16 / ES;
   static_assert(!DEC || U == 8, "phase A reduces 8 entries at once");
@@ -677,9 +735,11 @@ __global__ __launch_bounds__(256) void backward_units_kernel(ColArgs a, int nsla
   const int64_t nch = (a.D + EPC - 1) / EPC, c = slab * 64 + lane;
   const bool cin = c < nch;
   const uint32_t coff = (uint32_t)(min(c, max(nch - 1, (int64_t)0)) * 16);  // the lane's chunk, kept inside the row
-  const char* src = DEC ? a.g_xhat : a.xs;
-  const int64_t st_bytes = (DEC ? a.sg : a.sx) * ES;
-  const int64_t span = a.M > 0 ? (a.M - 1) * st_bytes + a.D * ES : 0;  // < 4 GB on the VEC path
+  static_assert(!HELD || (VEC && !DEC), "held rows are gathered by phase B");
+  const int held_shift = HeldChunk<DT>::shift((int)slab, lane);
+  const char* src = DEC ? a.g_xhat : (HELD ? (const char*)a.xq : a.xs);
+  const int64_t st_bytes = HELD ? a.sxq : (DEC ? a.sg : a.sx) * ES;
+  const int64_t span = HELD ? a.M * a.sxq : a.M > 0 ? (a.M - 1) * st_bytes + a.D * ES : 0;  // < 4 GB on the VEC path
   const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc((void*)src, (short)0, (int)(uint32_t)span,
                                                                      (int)BUF_W3);
   u32x4 wq[G];       // phase A, VEC: the items' W_dec[j] chunks (raw)
@@ -745,22 +805,27 @@ __global__ __launch_bounds__(256) void backward_units_kernel(ColArgs a, int nsla
       my_s = a.g_csc[ke];
     }
     const bool ok = lane < kn && r >= 0 && r < a.M;  // always in range, for a transpose made by sf_csr_transpose
-    const int my_row = ok ? r : 0;
+    int my_row = ok ? r : 0;
     my_s = ok ? my_s : 0.f;
+    uint32_t my_word = 0;
+    if constexpr (HELD) HeldChunk<DT>::template entries<HELD>(a, (int)slab, kn, lane, my_row, my_word);
     for (int kk = 0; kk < kn; kk += U) {
       int rows[U];
       float sv[U];
 #pragma unroll
       for (int u = 0; u < U; ++u) {
-        const int sl = min(kk + u, kn - 1);
+        const int sl = HELD ? kk + u : min(kk + u, kn - 1);
         rows[u] = __builtin_amdgcn_readlane(my_row, sl);
-        sv[u] = kk + u < kn ? __int_as_float(__builtin_amdgcn_readlane(__float_as_int(my_s), sl)) : 0.f;
+        sv[u] = HELD || kk + u < kn ? __int_as_float(__builtin_amdgcn_readlane(__float_as_int(my_s), sl)) : 0.f;
       }
       u32x4 r[U];       // VEC: raw chunks
       float v[U][EPC];  // otherwise: elements
+      HeldChunk<DT> h[U];
 #pragma unroll
       for (int u = 0; u < U; ++u) {
-        if constexpr (VEC) {
+        if constexpr (HELD) {
+          h[u].template load<HELD>(a, rs, rows[u], coff / 16 * EPC);
+        } else if constexpr (VEC) {
           r[u] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(
                                                rs, (int)coff, (int)((uint32_t)rows[u] * (uint32_t)st_bytes), 0));
         } else if (cin) {
@@ -774,7 +839,7 @@ __global__ __launch_bounds__(256) void backward_units_kernel(ColArgs a, int nsla
 #pragma unroll
       for (int u = 0; u < U; ++u) {
         const bool live = kk + u < kn;  // wave-uniform
-        if (live && k0 + kk + u >= q_end[0]) flush();
+        if (G > 1 && live && k0 + kk + u >= q_end[0]) flush();
         if constexpr (DEC) {
           if constexpr (VEC) {
             pd[u] = cin ? chunk_dot<DT>(r[u], wq[0]) : 0.f;
@@ -786,8 +851,12 @@ __global__ __launch_bounds__(256) void backward_units_kernel(ColArgs a, int nsla
         } else if (slab == 0) {
           bsum += sv[u];
         }
+        if constexpr (HELD) {
+          h[u].add(sv[u], (uint32_t)__builtin_amdgcn_readlane((int)my_word, kk + u), held_shift, acc);
+        } else {
 #pragma unroll
-        for (int e = 0; e < EPC; ++e) acc[e] = fmaf(sv[u], VEC ? chunk_elem<DT>(r[u], e) : v[u][e], acc[e]);
+          for (int e = 0; e < EPC; ++e) acc[e] = fmaf(sv[u], VEC ? chunk_elem<DT>(r[u], e) : v[u][e], acc[e]);
+        }
       }
       if constexpr (DEC) {
         const float sd = wave_sum8(pd, lane);  // entry kk + (lane >> 3)
@@ -884,10 +953,11 @@ __device__ __forceinline__ int64_t readlane_i64(int64_t v, int l) {
 // an edge tile or unaligned output). The column bounds and the first 64 entries of each walk
 // are loaded once for all slabs. VEC gathers as backward_units_kernel does.
 constexpr int TJ = 64, TILE_WAVES = 16, TILE_CPW = TJ / TILE_WAVES, TILE_THREADS = 64 * TILE_WAVES;
-template <int DT, bool VEC>
+// HELD: x' comes as 8-bit rows, of any D.
+template <int DT, bool VEC, int HELD = HELD_NO>
 __global__ __launch_bounds__(TILE_THREADS, VEC ? 8 : 4) void enc_tile_kernel(ColArgs a, int nslab, int slabs,
                                                                                    int out_vec, int dec_vec) {
-  constexpr int ES = DT == SF_F32 ? 4 : 2, EPC = 16 / ES, SD = 64 * EPC, U = 4;  // U: 64 VGPRs for 32 waves a CU
+  constexpr int ES = DT == SF_F32 ? 4 : 2, EPC = 16 / ES, SD = 64 * EPC, U = HELD ? 8 : 4;  // U: 64 VGPRs for 32 waves a CU
   typedef typename std::conditional<ES == 4, uint32_t, u16>::type T;
   __shared__ u32x4 tile[TJ * 64];
   auto lds_chunk = [&](int r, int k) -> u32x4& { return tile[r * 64 + (k ^ (r / EPC))]; };
@@ -944,9 +1014,10 @@ __global__ __launch_bounds__(TILE_THREADS, VEC ? 8 : 4) void enc_tile_kernel(Col
   int row0;
   float s0;
   entry(0, min(64, L), row0, s0);
-  const int64_t st_bytes = a.sx * ES;
-  const int64_t span = a.M > 0 ? (a.M - 1) * st_bytes + a.D * ES : 0;  // < 4 GB on the VEC path
-  const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc((void*)a.xs, (short)0, (int)(uint32_t)span,
+  const int64_t st_bytes = HELD ? a.sxq : a.sx * ES;
+  // < 4 GB on the VEC path (and of codes with HELD_NEAR)
+  const int64_t span = a.M > 0 ? (HELD ? a.M * a.sxq : (a.M - 1) * st_bytes + a.D * ES) : 0;
+  const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc((void*)(HELD ? (const char*)a.xq : a.xs), (short)0, (int)(uint32_t)span,
                                                                      (int)BUF_W3);
   const bool full_cols = out_vec && j0 + TJ <= a.N;
   // grid y: the block's slabs
@@ -955,6 +1026,7 @@ __global__ __launch_bounds__(TILE_THREADS, VEC ? 8 : 4) void enc_tile_kernel(Col
     const int64_t c = (int64_t)slab * 64 + lane;
     const bool cin = c < nch;
     const uint32_t coff = (uint32_t)(min(c, max(nch - 1, (int64_t)0)) * 16);
+    const int held_shift = HeldChunk<DT>::shift(slab, lane);
     // rows without light entries, and the queue of the others (column, end of its entries)
     int e_q[TILE_CPW], e_end[TILE_CPW], nq = 0;
 #pragma unroll
@@ -1015,20 +1087,25 @@ __global__ __launch_bounds__(TILE_THREADS, VEC ? 8 : 4) void enc_tile_kernel(Col
       int my_row = row0;
       float my_s = s0;
       if (k0 > 0) entry(k0, kn, my_row, my_s);
+      uint32_t my_word = 0;
+      if constexpr (HELD) HeldChunk<DT>::template entries<HELD>(a, slab, kn, lane, my_row, my_word);
       for (int kk = 0; kk < kn; kk += U) {
         int rows[U];
         float sv[U];
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-          const int sl = min(kk + u, kn - 1);
+          const int sl = HELD ? kk + u : min(kk + u, kn - 1);
           rows[u] = __builtin_amdgcn_readlane(my_row, sl);
-          sv[u] = kk + u < kn ? __int_as_float(__builtin_amdgcn_readlane(__float_as_int(my_s), sl)) : 0.f;
+          sv[u] = HELD || kk + u < kn ? __int_as_float(__builtin_amdgcn_readlane(__float_as_int(my_s), sl)) : 0.f;
         }
         u32x4 r[U];
         float v[U][EPC];
+        HeldChunk<DT> h[U];
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-          if constexpr (VEC) {
+          if constexpr (HELD) {
+            h[u].template load<HELD>(a, rs, rows[u], coff / 16 * EPC);
+          } else if constexpr (VEC) {
             r[u] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(
                                                  rs, (int)coff, (int)((uint32_t)rows[u] * (uint32_t)st_bytes), 0));
           } else if (cin) {
@@ -1042,8 +1119,12 @@ __global__ __launch_bounds__(TILE_THREADS, VEC ? 8 : 4) void enc_tile_kernel(Col
         for (int u = 0; u < U; ++u) {
           if (kk + u < kn && k0 + kk + u >= e_end[0]) flush();  // wave-uniform
           bsum += sv[u];
+          if constexpr (HELD) {
+            h[u].add(sv[u], (uint32_t)__builtin_amdgcn_readlane((int)my_word, kk + u), held_shift, acc);
+          } else {
 #pragma unroll
-          for (int e = 0; e < EPC; ++e) acc[e] = fmaf(sv[u], VEC ? chunk_elem<DT>(r[u], e) : v[u][e], acc[e]);
+            for (int e = 0; e < EPC; ++e) acc[e] = fmaf(sv[u], VEC ? chunk_elem<DT>(r[u], e) : v[u][e], acc[e]);
+          }
         }
       }
     }
@@ -1412,7 +1493,9 @@ constexpr int64_t GRID_BLOCKS = 2048;  // blocks of the grid-stride backward ker
 // (d_sae 2^20, 4096 tokens, L0 128) four are (phase A 1.27 -> 0.77 ms, phase B 0.84 -> 0.55).
 constexpr int units_per_wave(int64_t nnz, int64_t N) { return nnz < 4 * N ? 4 : 1; }
 
-template <int DT, bool VEC, bool DEC, int G>
+bool held_near(const ColArgs& a) { return a.M * a.sxq < (1LL << 32); }
+
+template <int DT, bool VEC, bool DEC, int G, int HELD = HELD_NO>
 void launch_units_g(const ColArgs& a, int64_t nslab, hipStream_t s) {
   const int64_t nb = (((DEC ? a.n_items : a.n_slots) + G - 1) / G + WPB - 1) / WPB;  // a bound
   if (nb == 0) return;
@@ -1422,7 +1505,7 @@ void launch_units_g(const ColArgs& a, int64_t nslab, hipStream_t s) {
   // 752); with 4 it is even to 1% slower, with 0.5 (2^20 features) 13% slower, as a feature's W_dec
   // and dW_dec rows then stream in 1-KB pieces.
   const int slab_major = !DEC || (G == 1 && a.nnz >= 8 * a.N);
-  hipLaunchKernelGGL((backward_units_kernel<DT, VEC, 8, DEC, G, !DEC>), dim3((unsigned)((nb * nslab + 7) / 8 * 8)),
+  hipLaunchKernelGGL((backward_units_kernel<DT, VEC, HELD ? 16 : 8, DEC, G, !DEC, HELD>), dim3((unsigned)((nb * nslab + 7) / 8 * 8)),
                      dim3(256), 0, s, a, (int)nslab, slab_major);
 }
 
@@ -1450,12 +1533,25 @@ void launch_tile(const ColArgs& a, bool vec, int out_vec, int dec_vec, int64_t n
   const int64_t split = std::min(nslab, std::max<int64_t>(1, (TILE_BLOCKS + tiles - 1) / tiles));
   const int slabs = (int)((nslab + split - 1) / split);
   const dim3 grid((unsigned)((tiles + 31) / 32 * 32), (unsigned)((nslab + slabs - 1) / slabs));
-  if (vec) hipLaunchKernelGGL((enc_tile_kernel<DT, true>), grid, dim3(TILE_THREADS), 0, s, a, (int)nslab, slabs, out_vec, dec_vec);
+  if (a.xq && held_near(a)) hipLaunchKernelGGL((enc_tile_kernel<DT, true, HELD_NEAR>), grid, dim3(TILE_THREADS), 0, s, a, (int)nslab, slabs, out_vec, dec_vec);
+  else if (a.xq) hipLaunchKernelGGL((enc_tile_kernel<DT, true, HELD_FAR>), grid, dim3(TILE_THREADS), 0, s, a, (int)nslab, slabs, out_vec, dec_vec);
+  else if (vec) hipLaunchKernelGGL((enc_tile_kernel<DT, true>), grid, dim3(TILE_THREADS), 0, s, a, (int)nslab, slabs, out_vec, dec_vec);
   else hipLaunchKernelGGL((enc_tile_kernel<DT, false>), grid, dim3(TILE_THREADS), 0, s, a, (int)nslab, slabs, out_vec, dec_vec);
 }
 
 template <bool DEC>
 void launch_units_dt(const ColArgs& a, int dt, bool vec, int64_t nslab, hipStream_t s) {
+  if constexpr (!DEC) {
+    auto held = [&](auto tag) {
+      constexpr int H = decltype(tag)::value;
+      switch (dt) {
+        case SF_BF16: launch_units_g<SF_BF16, true, false, 1, H>(a, nslab, s); break;
+        case SF_F16: launch_units_g<SF_F16, true, false, 1, H>(a, nslab, s); break;
+        default: launch_units_g<SF_F32, true, false, 1, H>(a, nslab, s); break;
+      }
+    };
+    if (a.xq) return held_near(a) ? held(std::integral_constant<int, HELD_NEAR>{}) : held(std::integral_constant<int, HELD_FAR>{});
+  }
   switch (dt) {
     case SF_BF16: vec ? launch_units<SF_BF16, true, DEC>(a, nslab, s) : launch_units<SF_BF16, false, DEC>(a, nslab, s); break;
     case SF_F16: vec ? launch_units<SF_F16, true, DEC>(a, nslab, s) : launch_units<SF_F16, false, DEC>(a, nslab, s); break;
@@ -1621,11 +1717,21 @@ extern "C" int sf_shifted_input(const void* x, int64_t sxm, int64_t sxk, int x_d
   return SF_OK;
 }
 
-extern "C" int sf_backward_columns(const int64_t* colptr, const int32_t* csc_row, const int32_t* csc_pos,
+namespace {
+// The input of dW_enc: x' in the parameters' type, or as 8-bit rows.
+struct Input {
+  const void* xs;
+  int64_t sx;
+  const void* xq;
+  int64_t sxq;
+  const void* xscale;
+  int64_t sxs;
+};
+int backward_columns(const int64_t* colptr, const int32_t* csc_row, const int32_t* csc_pos,
                                    const int64_t* plan_i64, const int32_t* item_col, const int32_t* multi_col,
                                    const int32_t* slot_item, int64_t max_items, int64_t max_slots, const void* values, int val_dt,
-                                   const void* g_val, int gval_dt, const void* w_dec, int64_t sw, const void* xs,
-                                   int64_t sx, const void* g_xhat, int64_t sg, int dt, int64_t N, int64_t M, int64_t D,
+                                   const void* g_val, int gval_dt, const void* w_dec, int64_t sw, const Input& in,
+                                   const void* g_xhat, int64_t sg, int dt, int64_t N, int64_t M, int64_t D,
                                    int64_t nnz, float* g_pre, void* d_wdec, void* d_wenc, float* d_benc,
                                    float* partials, float* work, int64_t work_floats, void* stream) {
   sf_clear_error();
@@ -1643,7 +1749,7 @@ extern "C" int sf_backward_columns(const int64_t* colptr, const int32_t* csc_row
                "sf_backward_columns: too many work items");
     SF_REQUIRE(colptr && plan_i64 && item_col && multi_col && slot_item && (D == 0 || d_wenc) && d_wdec && d_benc,
                "sf_backward_columns: NULL buffer");
-    SF_REQUIRE(nnz == 0 || (csc_row && csc_pos && values && work && partials && (D == 0 || (w_dec && xs && g_xhat))),
+    SF_REQUIRE(nnz == 0 || (csc_row && csc_pos && values && work && partials && (D == 0 || (w_dec && (in.xs || in.xq) && g_xhat))),
                "sf_backward_columns: NULL buffer");
     SF_REQUIRE(work_floats >= (nslab + 1) * nnz, "sf_backward_columns: work of %lld floats, need %lld",
                (long long)work_floats, (long long)((nslab + 1) * nnz));
@@ -1662,13 +1768,14 @@ extern "C" int sf_backward_columns(const int64_t* colptr, const int32_t* csc_row
   a.colptr = colptr; a.csc_row = csc_row; a.csc_pos = csc_pos; a.item_off = item_off; a.part_off = slot_off;
   a.item_col = item_col; a.slot_item = slot_item; a.n_items = max_items; a.values = values; a.val_dt = val_dt;
   a.g_val = g_val; a.gval_dt = gval_dt; a.w_dec = (const char*)w_dec; a.sw = sw;
-  a.xs = (const char*)xs; a.sx = sx; a.g_xhat = (const char*)g_xhat; a.sg = sg;
+  a.xs = (const char*)in.xs; a.sx = in.sx; a.xq = (const uint8_t*)in.xq; a.sxq = in.sxq;
+  a.xscale = (const uint8_t*)in.xscale; a.sxs = in.sxs; a.g_xhat = (const char*)g_xhat; a.sg = sg;
   a.N = N; a.M = M; a.D = D; a.nnz = nnz;
   a.dots = work; a.g_csc = work ? work + nslab * nnz : nullptr; a.g_pre = g_pre;
   a.d_wdec = (char*)d_wdec; a.d_wenc = (char*)d_wenc; a.d_benc = d_benc;
   a.part = partials; a.n_slots = max_slots;
-  const int64_t span_x = M > 0 ? ((M - 1) * sx + D) * es : 0, span_g = M > 0 ? ((M - 1) * sg + D) * es : 0;
-  const bool vec = D % (16 / es) == 0 && aligned16(xs, sx, es) && aligned16(g_xhat, sg, es) &&
+  const int64_t span_x = M > 0 && in.xs ? ((M - 1) * in.sx + D) * es : 0, span_g = M > 0 ? ((M - 1) * sg + D) * es : 0;
+  const bool vec = D % (16 / es) == 0 && (in.xq || aligned16(in.xs, in.sx, es)) && aligned16(g_xhat, sg, es) &&
                    aligned16(w_dec, sw, es) && aligned16(d_wdec, D, es) &&
                    span_x < (1LL << 32) && span_g < (1LL << 32);  // the per-row gathers are buffer loads
   // the records sit in d_wenc, which enc_tile_kernel overwrites once the units are done with them
@@ -1711,6 +1818,41 @@ extern "C" int sf_backward_columns(const int64_t* colptr, const int32_t* csc_row
     SF_LAUNCH_CHECK("enc_tile_kernel");
   }
   return SF_OK;
+}
+}  // namespace
+
+extern "C" int sf_backward_columns(const int64_t* colptr, const int32_t* csc_row, const int32_t* csc_pos,
+                                   const int64_t* plan_i64, const int32_t* item_col, const int32_t* multi_col,
+                                   const int32_t* slot_item, int64_t max_items, int64_t max_slots, const void* values, int val_dt,
+                                   const void* g_val, int gval_dt, const void* w_dec, int64_t sw, const void* xs,
+                                   int64_t sx, const void* g_xhat, int64_t sg, int dt, int64_t N, int64_t M, int64_t D,
+                                   int64_t nnz, float* g_pre, void* d_wdec, void* d_wenc, float* d_benc,
+                                   float* partials, float* work, int64_t work_floats, void* stream) {
+  return backward_columns(colptr, csc_row, csc_pos, plan_i64, item_col, multi_col, slot_item, max_items, max_slots, values,
+                          val_dt, g_val, gval_dt, w_dec, sw, Input{xs, sx, nullptr, 0, nullptr, 0}, g_xhat, sg, dt, N, M, D,
+                          nnz, g_pre, d_wdec, d_wenc, d_benc, partials, work, work_floats, stream);
+}
+
+extern "C" int sf_backward_columns_held(const int64_t* colptr, const int32_t* csc_row, const int32_t* csc_pos,
+                                        const int64_t* plan_i64, const int32_t* item_col, const int32_t* multi_col,
+                                        const int32_t* slot_item, int64_t max_items, int64_t max_slots,
+                                        const void* values, int val_dt, const void* g_val, int gval_dt,
+                                        const void* w_dec, int64_t sw, const void* xq, int64_t sxq, const void* xscale,
+                                        int64_t sxs, const void* g_xhat, int64_t sg, int dt, int64_t N, int64_t M,
+                                        int64_t D, int64_t nnz, float* g_pre, void* d_wdec, void* d_wenc,
+                                        float* d_benc, float* partials, float* work, int64_t work_floats,
+                                        void* stream) {
+  sf_clear_error();
+  if (M > 0 && D > 0) {
+    SF_REQUIRE(xq && xscale, "sf_backward_columns_held: NULL codes or scales");
+    SF_REQUIRE((uintptr_t)xq % 16 == 0 && sxq % 16 == 0, "sf_backward_columns_held: rows of codes must be 16-B aligned");
+    SF_REQUIRE((uintptr_t)xscale % 4 == 0 && sxs % 4 == 0, "sf_backward_columns_held: rows of scales must be 4-B aligned");
+    SF_REQUIRE(sxq >= sff8::code_bytes(D) && sxs >= sff8::scale_bytes(D),
+               "sf_backward_columns_held: rows of 8 bits are too short for %lld elements", (long long)D);
+  }
+  return backward_columns(colptr, csc_row, csc_pos, plan_i64, item_col, multi_col, slot_item, max_items, max_slots, values,
+                          val_dt, g_val, gval_dt, w_dec, sw, Input{nullptr, 0, xq, sxq, xscale, sxs}, g_xhat, sg, dt, N, M, D,
+                          nnz, g_pre, d_wdec, d_wenc, d_benc, partials, work, work_floats, stream);
 }
 
 extern "C" int sf_transpose(const void* src, int64_t R, int64_t C, int64_t ss, int dt, const int64_t* skip_ptr,

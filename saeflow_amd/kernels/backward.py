@@ -16,7 +16,7 @@ from types import SimpleNamespace
 import torch
 
 from .. import _lib
-from .fp8 import Fp8Rows, dequantize_rows
+from .fp8 import Fp8Rows
 
 
 def _rows(t, dtype):
@@ -89,12 +89,13 @@ def sparse_backward(x, W_enc, b_enc, W_dec, b_dec, csr, grad_x_hat=None, grad_va
             raise ValueError(f"grad_values has {gv.numel()} entries for nnz={nnz}")
         # per-feature sums over the CSC
         colptr, rows, pos = csr_transpose(indptr, indices, N)
-        if held:
-            xs = dequantize_rows(x, out_dtype=dt)
+        if held:  # gathered as they lie
+            columns, x_args = lib.sf_backward_columns_held, x._args()
         else:
             xs = torch.empty(M, D, dtype=dt, device=dev)
             _lib.check(lib.sf_shifted_input(_lib.ptr(x), x.stride(0), x.stride(1), _lib.dtype_code(x, "x"),
                                             _lib.ptr(b_dec), _lib.dtype_code(b_dec, "b_dec"), M, D, code, _lib.ptr(xs), s))
+            columns, x_args = lib.sf_backward_columns, (_lib.ptr(xs), D)
         plan_i64 = torch.empty(3 * (N + 1), dtype=torch.int64, device=dev)
         max_items, max_slots, work_floats = ctypes.c_int64(), ctypes.c_int64(), ctypes.c_int64()
         _lib.check(lib.sf_backward_bounds(N, nnz, D, code, ctypes.byref(max_items), ctypes.byref(max_slots),
@@ -112,15 +113,14 @@ def sparse_backward(x, W_enc, b_enc, W_dec, b_dec, csr, grad_x_hat=None, grad_va
         work = torch.empty(work_floats.value, dtype=torch.float32, device=dev)
         # the grid is sized by the bound of the work-item count (surplus waves return at once), so
         # nothing here waits for the GPU
-        _lib.check(lib.sf_backward_columns(_lib.ptr(colptr), _lib.ptr(rows), _lib.ptr(pos), _lib.ptr(plan_i64),
-                                           _lib.ptr(item_col), _lib.ptr(multi_col), _lib.ptr(slot_item),
-                                           max_items.value, max_slots.value,
-                                           _lib.ptr(values), _lib.dtype_code(values, "values"), _lib.ptr(gv),
-                                           0 if gv is None else _lib.dtype_code(gv, "grad_values"), _lib.ptr(Wd),
-                                           Wd.stride(0), _lib.ptr(xs), D, _lib.ptr(g), g.stride(0), code, N, M, D,
-                                           nnz, _lib.ptr(g_pre), _lib.ptr(d_wdec), _lib.ptr(d_wenc),
-                                           _lib.ptr(d_benc), _lib.ptr(partials), _lib.ptr(work), work.numel(), s))
-        del partials, xs, work
+        _lib.check(columns(_lib.ptr(colptr), _lib.ptr(rows), _lib.ptr(pos), _lib.ptr(plan_i64), _lib.ptr(item_col),
+                           _lib.ptr(multi_col), _lib.ptr(slot_item), max_items.value, max_slots.value, _lib.ptr(values),
+                           _lib.dtype_code(values, "values"), _lib.ptr(gv),
+                           0 if gv is None else _lib.dtype_code(gv, "grad_values"), _lib.ptr(Wd), Wd.stride(0), *x_args,
+                           _lib.ptr(g), g.stride(0), code, N, M, D, nnz, _lib.ptr(g_pre), _lib.ptr(d_wdec),
+                           _lib.ptr(d_wenc), _lib.ptr(d_benc), _lib.ptr(partials), _lib.ptr(work), work.numel(), s))
+        del partials, work
+        xs = None  # (its memory is free for what follows)
         # db_dec = sum_m g_xhat[m] - sum_m dx'[m], and sum_m dx'[m] = W_enc db_enc
         d_bdec = torch.empty(D, dtype=torch.float32, device=dev)
         ws = torch.empty(min(256, max(M, 1)) * D, dtype=torch.float32, device=dev)
