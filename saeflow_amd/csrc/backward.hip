@@ -1491,7 +1491,11 @@ constexpr int64_t GRID_BLOCKS = 2048;  // blocks of the grid-stride backward ker
 // entries per feature (d_sae 65536, 16384 tokens, L0 64) one item per wave is fastest (four:
 // phase A 0.74 -> 0.88 ms, phase B 0.69 -> 0.77: the queue's registers cost occupancy); at 0.5
 // (d_sae 2^20, 4096 tokens, L0 128) four are (phase A 1.27 -> 0.77 ms, phase B 0.84 -> 0.55).
-constexpr int units_per_wave(int64_t nnz, int64_t N) { return nnz < 4 * N ? 4 : 1; }
+// With few waves one item each is faster all the same, as a long column's items, which follow each other, then run side by
+// side (us, one item a wave -> four: fp16 d_in 1000, d_sae 10007, 1000 tokens, 20 K waves of one item 41 -> 63, 100
+// tokens, 7 K 9.7 -> 11.5; bf16 2304, 32768, 200 tokens, 58 K 37 -> 31; 65536, 1000 tokens, 184 K 80 -> 57; fp32 768,
+// 24576, 500 tokens, 74 K 31 -> 34).
+int units_per_wave(int64_t nnz, int64_t N, int64_t waves) { return nnz < 4 * N && waves >= 40000 ? 4 : 1; }
 
 bool held_near(const ColArgs& a) { return a.M * a.sxq < (1LL << 32); }
 
@@ -1513,7 +1517,7 @@ void launch_units_g(const ColArgs& a, int64_t nslab, hipStream_t s) {
 template <int DT, bool VEC, bool DEC>
 void launch_units(const ColArgs& a, int64_t nslab, hipStream_t s) {
   if constexpr (DEC) {
-    if (units_per_wave(a.nnz, a.N) == 4) {
+    if (units_per_wave(a.nnz, a.N, a.n_items * nslab) == 4) {
       launch_units_g<DT, VEC, DEC, 4>(a, nslab, s);
       return;
     }

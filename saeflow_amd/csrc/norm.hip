@@ -768,10 +768,11 @@ __global__ __launch_bounds__(64 * FAST_WAVES, GT == SF_F32 ? 5 : 6) void norm_ba
 #pragma unroll
     for (int e = 0; e < 8; ++e) o[e] = fmaf(d[e], k2, fmaf(ge[e] * w[e], rstd, k1));
     char* out = a.dx + min(m, a.M - 1) * a.sdx;
+    const bool put = in && a.dx;  // without dx its bounds drop all of it: a branch would have loads wait for stores
     const __amdgpu_buffer_rsrc_t rs =
-        __builtin_amdgcn_make_buffer_rsrc((void*)out, (short)0, in ? (D & ~7) * ES : 0, (int)SF_RSRC_W3);
+        __builtin_amdgcn_make_buffer_rsrc((void*)out, (short)0, put ? (D & ~7) * ES : 0, (int)SF_RSRC_W3);
     put8_rsrc<GT>(rs, k0, o);
-    if (past && in && (D & 7) && k0 < D && k0 + 8 > D) store8_any(out, GT, k0, D, o);
+    if (past && put && (D & 7) && k0 < D && k0 + 8 > D) store8_any(out, GT, k0, D, o);
   }
   if (!a.dw && !a.db) return;
   if (a.TB > 1) {
@@ -1140,7 +1141,7 @@ extern "C" int sf_layer_norm_backward(const void* g, int64_t sgm, int g_dt, cons
   SF_REQUIRE((!w || sf_valid_dtype(w_dt)) && (!dw || sf_valid_dtype(dw_dt)) && (!db || sf_valid_dtype(db_dt)),
              "unsupported dtype code");
   hipStream_t s = (hipStream_t)stream;
-  const bool pg = dw || db, plain = dx && dx_dt == g_dt && (!x || x_dt == g_dt) && !g_mean && !g_rstd;
+  const bool pg = dw || db, plain = (!dx || dx_dt == g_dt) && (!x || x_dt == g_dt) && !g_mean && !g_rstd;
   const BwdPlan p = backward_plan(M, D, plain);
   if (M > 0) {
     if (const int rc = check_matrix("g", g, sgm, g_dt, M, D)) return rc;
