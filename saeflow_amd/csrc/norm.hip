@@ -264,21 +264,27 @@ __device__ __forceinline__ void put_codes(const FwdArgs& a, int64_t m, int64_t k
 // bounds drop the lanes past the last whole chunk without a branch, and weight and bias are kept in LDS as fp32, so
 // that no wait for a row's loads waits for anything else. In LDS the lower four elements of all chunks lie before the
 // upper four: lanes read 16 B side by side.
-template <int DT, int U, bool HOLD>
+// W: waves of a row, one up to 4096 elements and a block's four up to 8192, which then exchange their sums through LDS.
+template <int DT, int U, bool HOLD, int W>
 __global__ __launch_bounds__(256) void norm_kernel(FwdArgs a) {
-  constexpr int ES = DT == SF_F32 ? 4 : 2, CH = U * 64;
+  constexpr int ES = DT == SF_F32 ? 4 : 2, CH = W * U * 64, ROWS = 4 / W;
   constexpr bool bf = DT == SF_BF16;
   __shared__ u32x4 s_par[4 * CH];  // weight's lower and upper halves, then bias's
-  const int lane = threadIdx.x & 63, D = (int)a.D;
-  const int last = ((U - 1) * 64 + lane) * 8, off = max(0, last - (D - 8));
-  const bool past = D < U * 512, affine = a.w || a.b;
-  int64_t m = (int64_t)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int64_t step = (int64_t)gridDim.x * 4;
+  __shared__ double s_sum[W > 1 ? 2 : 1][4];
+  __shared__ float s_sq[W > 1 ? 2 : 1][4];
+  const int lane = threadIdx.x & 63, D = (int)a.D, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int c0 = W > 1 ? wave * U : 0;  // the wave's first chunk of 64 lanes
+  const bool affine = a.w || a.b;
+  auto at = [&](int i) { return ((c0 + i) * 64 + lane) * 8; };
+  // only a wave's last chunk, or any of a row's last wave, can run past the row's end
+  auto past = [&](int i) { return (W > 1 || i + 1 == U) && (c0 + i + 1) * 512 > D; };
+  int64_t m = (int64_t)blockIdx.x * ROWS + (W > 1 ? 0 : wave);
+  const int64_t step = (int64_t)gridDim.x * ROWS;
   Raw<ES> raw[U];
   auto load = [&](int64_t row) {
     const char* p = a.x + min(row, a.M - 1) * a.sxm;  // (a wave past the last row loads that again)
 #pragma unroll
-    for (int i = 0; i < U; ++i) raw[i] = load_at<ES>(p, (uint32_t)(i + 1 < U ? (i * 64 + lane) * 8 : min(last, D - 8)) * ES);
+    for (int i = 0; i < U; ++i) raw[i] = load_at<ES>(p, (uint32_t)(W > 1 || i + 1 == U ? min(at(i), D - 8) : at(i)) * ES);
   };
   load(m);
   if (affine) {
@@ -299,34 +305,48 @@ __global__ __launch_bounds__(256) void norm_kernel(FwdArgs a) {
     }
     __syncthreads();
   }
-  for (; m < a.M; m += step) {
-    if (past) shift_back(raw[U - 1], off);
+  int buf = 0;
+  for (; m < a.M; m += step, buf ^= 1) {
     float v[U][8];
     double sum = 0.0;
 #pragma unroll
-    for (int i = 0; i < U; ++i)
+    for (int i = 0; i < U; ++i) {
+      if (past(i)) shift_back(raw[i], max(0, at(i) - (D - 8)));
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
         v[i][e] = raw_elem(raw[i], e, bf);
         sum += (double)v[i][e];
       }
+    }
     load(m + step);
-    const float mean = (float)(wave_sum_f64(sum) * a.per_d);
+    sum = wave_sum_f64(sum);
+    if constexpr (W > 1) {
+      if (lane == 0) s_sum[buf][wave] = sum;
+      __syncthreads();
+      sum = (s_sum[buf][0] + s_sum[buf][1]) + (s_sum[buf][2] + s_sum[buf][3]);
+    }
+    const float mean = (float)(sum * a.per_d);
     float sq = 0.f;
 #pragma unroll
     for (int i = 0; i < U; ++i)
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
         v[i][e] -= mean;
-        if (i + 1 == U) v[i][e] = last + e < D ? v[i][e] : 0.f;
+        if (W > 1 || i + 1 == U) v[i][e] = at(i) + e < D ? v[i][e] : 0.f;
         sq = fmaf(v[i][e], v[i][e], sq);
       }
     sq = wave_sum(sq);
+    if constexpr (W > 1) {
+      if (lane == 0) s_sq[buf][wave] = sq;
+      __syncthreads();
+      sq = (s_sq[buf][0] + s_sq[buf][1]) + (s_sq[buf][2] + s_sq[buf][3]);
+    }
     const float rstd = inverse_std(sq, (float)D, a.eps);
     if constexpr (HOLD) {
       const bool finite = sq < __builtin_inff();  // so is every element: no NaN or infinity to look for
+      const int words = (D + 511) / 512 * 4;
       const __amdgpu_buffer_rsrc_t rq = __builtin_amdgcn_make_buffer_rsrc((void*)(a.q + m * a.sq), (short)0, (int)a.kp, (int)SF_RSRC_W3);
-      const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc((void*)(a.scale + m * a.ss), (short)0, 4 * U, (int)SF_RSRC_W3);
+      const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc((void*)(a.scale + m * a.ss), (short)0, words, (int)SF_RSRC_W3);
 #pragma unroll
       for (int i = 0; i < U; ++i) {
         float c[8];
@@ -334,11 +354,11 @@ __global__ __launch_bounds__(256) void norm_kernel(FwdArgs a) {
         for (int e = 0; e < 8; ++e) c[e] = v[i][e];
         uint32_t byte;
         const u32x2 codes = finite ? quantize8_finite(c, byte) : sff8::quantize8(c, byte);
-        __builtin_amdgcn_raw_buffer_store_b64(codes, rq, (i * 64 + lane) * 8, 0, 0);
+        __builtin_amdgcn_raw_buffer_store_b64(codes, rq, at(i), 0, 0);
         // four blocks a chunk of 64 lanes: their bytes are one word of the row's scales (zero behind the last block)
         const uint32_t word = (uint32_t)__builtin_amdgcn_readlane((int)byte, 0) | (uint32_t)__builtin_amdgcn_readlane((int)byte, 16) << 8 |
                               (uint32_t)__builtin_amdgcn_readlane((int)byte, 32) << 16 | (uint32_t)__builtin_amdgcn_readlane((int)byte, 48) << 24;
-        __builtin_amdgcn_raw_buffer_store_b32(word, rs, lane == 0 ? 4 * i : 4 * U, 0, 0);
+        __builtin_amdgcn_raw_buffer_store_b32(word, rs, lane == 0 ? 4 * (c0 + i) : words, 0, 0);
       }
     }
     char* out = a.y + m * a.sym;
@@ -349,7 +369,7 @@ __global__ __launch_bounds__(256) void norm_kernel(FwdArgs a) {
 #pragma unroll
       for (int e = 0; e < 8; ++e) y[e] = v[i][e] * rstd;
       if (affine) {
-        const int c = i * 64 + lane;
+        const int c = (c0 + i) * 64 + lane;
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
           const u32x4 w = s_par[h * CH + c], b = s_par[(2 + h) * CH + c];
@@ -357,10 +377,10 @@ __global__ __launch_bounds__(256) void norm_kernel(FwdArgs a) {
           for (int e = 0; e < 4; ++e) y[4 * h + e] = fmaf(y[4 * h + e], __uint_as_float(w[e]), __uint_as_float(b[e]));
         }
       }
-      put8_rsrc<DT>(ry, (i * 64 + lane) * 8, y);
-      if (i + 1 == U && (D & 7) && last < D && last + 8 > D) store8_any(out, DT, last, D, y);
+      put8_rsrc<DT>(ry, at(i), y);
+      if (past(i) && (D & 7) && at(i) < D && at(i) + 8 > D) store8_any(out, DT, at(i), D, y);
     }
-    if (lane == 0) {
+    if (lane == 0 && c0 == 0) {
       if (a.mean) a.mean[m] = mean;
       if (a.rstd) a.rstd[m] = rstd;
     }
@@ -972,6 +992,7 @@ __global__ __launch_bounds__(256) void undo_backward_kernel(UndoArgs a) {
 // ------------------------------------------------------------------ host
 constexpr int64_t MAX_M = (1ll << 31) - 1, MAX_D = 1 << 24;
 constexpr int64_t WAVE_D = 4096;          // the longest row a wave of norm_kernel holds
+constexpr int64_t ROW_D = 8192;           // the longest its block holds
 constexpr int64_t FWD_BLOCKS = 1024;      // of four waves: four a CU
 constexpr int64_t TEAM_D = MAX_T * 2048;  // the longest row a team of norm_backward_kernel holds, four chunks a lane
 constexpr int64_t FAST_D = 4096;          // the longest of norm_backward_fast_kernel
@@ -1027,22 +1048,25 @@ BwdPlan backward_plan(int64_t M, int64_t D, bool plain) {
 
 template <int DT, bool HOLD>
 int forward_typed(const FwdArgs& a, hipStream_t s) {
-  const dim3 grid((unsigned)std::min<int64_t>((a.M + 3) / 4, FWD_BLOCKS));
-  if (a.D > WAVE_D) {
+  if (a.D > ROW_D) {
     hipLaunchKernelGGL((norm_any_kernel<DT, HOLD, 1024>), dim3((unsigned)std::min<int64_t>(a.M, 1 << 16)), dim3(1024), 0, s, a);
   } else if (a.D < 8 || a.y_dt != DT) {
     hipLaunchKernelGGL((norm_any_kernel<DT, HOLD, 64>), dim3((unsigned)std::min<int64_t>((a.M + 3) / 4, 1 << 16)), dim3(256), 0, s, a);
   } else {
-#define SF_NORM(UV) case UV: hipLaunchKernelGGL((norm_kernel<DT, UV, HOLD>), grid, dim3(256), 0, s, a); break
-    switch ((a.D + 511) / 512) {
-      SF_NORM(1);
-      SF_NORM(2);
-      SF_NORM(3);
-      SF_NORM(4);
-      SF_NORM(5);
-      SF_NORM(6);
-      SF_NORM(7);
-      SF_NORM(8);
+    const int waves = a.D <= WAVE_D ? 1 : 4;
+    const dim3 grid((unsigned)std::min<int64_t>((a.M * waves + 3) / 4, FWD_BLOCKS));
+#define SF_NORM(UV, WV) case 100 * WV + UV: hipLaunchKernelGGL((norm_kernel<DT, UV, HOLD, WV>), grid, dim3(256), 0, s, a); break
+    switch (100 * waves + (int)((a.D + 512 * waves - 1) / (512 * waves))) {
+      SF_NORM(1, 1);
+      SF_NORM(2, 1);
+      SF_NORM(3, 1);
+      SF_NORM(4, 1);
+      SF_NORM(5, 1);
+      SF_NORM(6, 1);
+      SF_NORM(7, 1);
+      SF_NORM(8, 1);
+      SF_NORM(3, 4);
+      SF_NORM(4, 4);
     }
 #undef SF_NORM
   }

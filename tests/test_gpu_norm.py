@@ -24,7 +24,7 @@ pytestmark = pytest.mark.gpu
 U = 2.0 ** -24
 DTYPES = [torch.float32, torch.bfloat16, torch.float16]
 # one element, inside a chunk, chunk and block edges, a wave, teams of waves, the longest row of a wave, of a team, longer
-WIDTHS = [1, 2, 7, 8, 9, 64, 100, 127, 129, 511, 512, 513, 768, 1000, 1003, 1537, 2304, 4095, 4096, 4097, 8192, 8200, 20001]
+WIDTHS = [1, 2, 7, 8, 9, 64, 100, 127, 129, 511, 512, 513, 768, 1000, 1003, 1537, 2304, 4095, 4096, 4097, 6144, 8191, 8192, 8200, 20001]
 
 
 def half(dtype):
