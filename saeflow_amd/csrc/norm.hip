@@ -479,7 +479,7 @@ struct BwdArgs {
   int T, TB;    // waves of a row's team, teams of a block
 };
 
-// Eight elements of x - mean in the form they come in.
+// Eight elements of a row in the form they come in.
 template <int XT>
 struct XRaw {
   static constexpr int ES = XT == SF_F32 ? 4 : 2;
@@ -490,9 +490,10 @@ struct XRaw {
   }
   __device__ __forceinline__ void load_at(const BwdArgs& a, int64_t m, uint32_t k) { v = ::load_at<ES>(a.x + m * a.sxm, k * ES); }
   __device__ __forceinline__ void shift_back(int off) { ::shift_back(v, off); }
-  __device__ __forceinline__ void centred(float mean, float (&d)[8]) const {
+  // xh
+  __device__ __forceinline__ void normed(float mean, float rstd, float (&xh)[8]) const {
 #pragma unroll
-    for (int e = 0; e < 8; ++e) d[e] = raw_elem(v, e, XT == SF_BF16) - mean;
+    for (int e = 0; e < 8; ++e) xh[e] = (raw_elem(v, e, XT == SF_BF16) - mean) * rstd;
   }
 };
 template <>
@@ -519,16 +520,16 @@ struct XRaw<X_FP8> {
   __device__ __forceinline__ void shift_back(int off) {
     if (off >= 8) c = u32x2{0, 0};
   }
-  __device__ __forceinline__ void centred(float, float (&d)[8]) const {
-    const float f = sff8::scale_of(byte);
+  __device__ __forceinline__ void normed(float, float rstd, float (&xh)[8]) const {
+    const float f = sff8::scale_of(byte) * rstd;
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
       const sff8::f32x2 lo = __builtin_amdgcn_cvt_pk_f32_fp8((int)c[i], false);
       const sff8::f32x2 hi = __builtin_amdgcn_cvt_pk_f32_fp8((int)c[i], true);
-      d[4 * i] = lo[0] * f;
-      d[4 * i + 1] = lo[1] * f;
-      d[4 * i + 2] = hi[0] * f;
-      d[4 * i + 3] = hi[1] * f;
+      xh[4 * i] = lo[0] * f;
+      xh[4 * i + 1] = lo[1] * f;
+      xh[4 * i + 2] = hi[0] * f;
+      xh[4 * i + 3] = hi[1] * f;
     }
   }
 };
@@ -633,15 +634,15 @@ __global__ __launch_bounds__(64 * MAX_T) void norm_backward_kernel(BwdArgs a) {
       if (batch * R + r < a.M) {  // wave-uniform
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-          float d[8];
-          xc[r][u].centred(mean[r], d);
+          float xh[8];
+          xc[r][u].normed(mean[r], rstd[r], xh);
 #pragma unroll
           for (int e = 0; e < 8; ++e) {
-            const float ge = raw_elem(gc[r][u], e, bf), xh = d[e] * rstd[r], q = ge * w[u][e];
-            acc_w[u][e] = fmaf(ge, xh, acc_w[u][e]);
+            const float ge = raw_elem(gc[r][u], e, bf), q = ge * w[u][e];
+            acc_w[u][e] = fmaf(ge, xh[e], acc_w[u][e]);
             acc_b[u][e] += ge;
             s[2 * r] += q;
-            s[2 * r + 1] = fmaf(q, xh, s[2 * r + 1]);
+            s[2 * r + 1] = fmaf(q, xh[e], s[2 * r + 1]);
           }
         }
       }
@@ -666,12 +667,12 @@ __global__ __launch_bounds__(64 * MAX_T) void norm_backward_kernel(BwdArgs a) {
 #pragma unroll
           for (int u = 0; u < U; ++u) {
             if (k0[u] >= a.D) continue;
-            float d[8], o[8];
-            xc[r][u].centred(mean[r], d);
+            float xh[8], o[8];
+            xc[r][u].normed(mean[r], rstd[r], xh);
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
               const float q = raw_elem(gc[r][u], e, bf) * w[u][e];
-              o[e] = fmaf(rstd[r], q - c1 - d[e] * rstd[r] * c2, c0);
+              o[e] = fmaf(rstd[r], q - c1 - xh[e] * c2, c0);
             }
             store8_any(a.dx + m * a.sdx, a.dx_dt, k0[u], a.D, o);
           }
@@ -707,8 +708,8 @@ __global__ __launch_bounds__(64 * MAX_T) void norm_backward_kernel(BwdArgs a) {
 // The usual case of the above, straight through: x and dx of g's type (or x in 8 bits), up to 4096 elements. What
 // differs is what keeps the loads going. A row's result leaves by a buffer store, whose bounds drop the lanes past
 // the row's last whole chunk and rows past the last without a branch, so that waiting for the next row's loads does not
-// wait for the last row's stores. Elements are unpacked once, into the registers that both halves use, and the
-// sums are those of g (x - mean) and of its product with w: twelve vector instructions an element. One row at a time
+// wait for the last row's stores. Elements are unpacked once, into the registers that both halves use, and g xh is formed
+// once for both sums it is in: thirteen vector instructions an element. One row at a time
 // keeps the registers at 80 (96 in fp32): two blocks of up to ten waves a CU.
 constexpr int FAST_WAVES = 10;
 template <int XT, int GT>
@@ -735,36 +736,39 @@ __global__ __launch_bounds__(64 * FAST_WAVES, GT == SF_F32 ? 5 : 6) void norm_ba
   const float per_d = 1.0f / (float)D;
   Raw<ES> g;
   XRaw<XT> x;
-  float rstd_n, mean_n;
+  float rstd_n, mean_n, gm_n, gr_n;
+  const float *g_mean = a.g_mean ? a.g_mean : a.rstd, *g_rstd = a.g_rstd ? a.g_rstd : a.rstd;  // (loads without a branch)
   auto load = [&](int64_t row) {
     const int64_t m = min(row, a.M - 1);  // a team past the last row loads that again, and leaves it out below
     g = load_at<ES>(a.g + m * a.sgm, kg * ES);
     x.load_at(a, m, kx);
     rstd_n = a.rstd[m];
     mean_n = XT == X_FP8 ? 0.f : a.mean[m];
+    gm_n = g_mean[m];
+    gr_n = g_rstd[m];
   };
   int64_t m = (int64_t)blockIdx.x * a.TB + team;
   load(m);
   int buf = 0;
   for (int64_t m0 = (int64_t)blockIdx.x * a.TB; m0 < a.M; m0 += step, m += step, buf ^= 1) {
     const bool in = m < a.M;  // wave-uniform
-    const float rstd = rstd_n;
+    const float rstd = rstd_n, gm = a.g_mean ? gm_n : 0.f, gr = a.g_rstd ? gr_n : 0.f;
     if (past) {
       shift_back(g, off);
       x.shift_back(off);
     }
-    float ge[8], d[8], s1 = 0.f, s2 = 0.f;
-    x.centred(mean_n, d);
+    float ge[8], xh[8], s1 = 0.f, s2 = 0.f;
+    x.normed(mean_n, rstd, xh);
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
       ge[e] = in ? raw_elem(g, e, bf) : 0.f;
-      d[e] = in ? d[e] : 0.f;
+      xh[e] = in ? xh[e] : 0.f;
     }
     load(m + step);
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
-      const float t = ge[e] * d[e];
-      acc_w[e] = fmaf(t, rstd, acc_w[e]);
+      const float t = ge[e] * xh[e];
+      acc_w[e] += t;
       acc_b[e] += ge[e];
       s1 = fmaf(ge[e], w[e], s1);
       s2 = fmaf(t, w[e], s2);
@@ -783,10 +787,10 @@ __global__ __launch_bounds__(64 * FAST_WAVES, GT == SF_F32 ? 5 : 6) void norm_ba
         s2 += s_sum[buf][team * a.T + t][1];
       }
     }
-    const float k1 = -rstd * (s1 * per_d), k2 = -rstd * rstd * rstd * (s2 * per_d);
+    const float k1 = fmaf(gm, per_d, -rstd * (s1 * per_d)), k2 = -rstd * fmaf(gr * rstd, per_d, s2 * per_d);
     float o[8];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) o[e] = fmaf(d[e], k2, fmaf(ge[e] * w[e], rstd, k1));
+    for (int e = 0; e < 8; ++e) o[e] = fmaf(xh[e], k2, fmaf(ge[e] * w[e], rstd, k1));
     char* out = a.dx + min(m, a.M - 1) * a.sdx;
     const bool put = in && a.dx;  // without dx its bounds drop all of it: a branch would have loads wait for stores
     const __amdgpu_buffer_rsrc_t rs =
@@ -859,22 +863,22 @@ __global__ __launch_bounds__(1024) void norm_backward_long_kernel(BwdArgs a) {
         const Raw<GES> g = load_raw<GES>(a.g + m * a.sgm, k0, a.D);
         XRaw<XT> x;
         x.load(a, m, k0);
-        float w[8], d[8], o[8];
+        float w[8], xh[8], o[8];
         if (a.w) {
           load8_any(a.w, a.w_dt, k0, a.D, w);
         } else {
 #pragma unroll
           for (int e = 0; e < 8; ++e) w[e] = 1.f;
         }
-        x.centred(mean, d);
+        x.normed(mean, rstd, xh);
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-          const float q = raw_elem(g, e, bf) * w[e], xh = d[e] * rstd;
+          const float q = raw_elem(g, e, bf) * w[e];
           if (pass == 0 && k0 + e < a.D) {
             s1 += q;
-            s2 = fmaf(q, xh, s2);
+            s2 = fmaf(q, xh[e], s2);
           }
-          o[e] = fmaf(rstd, q - c1 - xh * c2, c0);
+          o[e] = fmaf(rstd, q - c1 - xh[e] * c2, c0);
         }
         if (pass == 1) store8_any(a.dx + m * a.sdx, a.dx_dt, k0, a.D, o);
       }
@@ -893,13 +897,12 @@ __global__ __launch_bounds__(64) void norm_columns_kernel(BwdArgs a) {
     const Raw<GES> g = load_raw<GES>(a.g + m * a.sgm, k0, a.D);
     XRaw<XT> x;
     x.load(a, m, k0);
-    float d[8];
-    x.centred(XT == X_FP8 ? 0.f : a.mean[m], d);
-    const float rstd = a.rstd[m];
+    float xh[8];
+    x.normed(XT == X_FP8 ? 0.f : a.mean[m], a.rstd[m], xh);
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
       const float ge = raw_elem(g, e, bf);
-      acc_w[e] = fmaf(ge, d[e] * rstd, acc_w[e]);
+      acc_w[e] = fmaf(ge, xh[e], acc_w[e]);
       acc_b[e] += ge;
     }
   }
@@ -994,7 +997,7 @@ constexpr int64_t MAX_M = (1ll << 31) - 1, MAX_D = 1 << 24;
 constexpr int64_t WAVE_D = 4096;          // the longest row a wave of norm_kernel holds
 constexpr int64_t ROW_D = 8192;           // the longest its block holds
 constexpr int64_t FWD_BLOCKS = 1024;      // of four waves: four a CU
-constexpr int64_t TEAM_D = MAX_T * 2048;  // the longest row a team of norm_backward_kernel holds, four chunks a lane
+constexpr int64_t TEAM_D = MAX_T * 1024;  // the longest row a team of norm_backward_kernel holds, two chunks a lane
 constexpr int64_t FAST_D = 4096;          // the longest of norm_backward_fast_kernel
 constexpr int64_t MOST_PARTS = 512;       // blocks of the backward pass: two a CU
 
@@ -1037,7 +1040,7 @@ BwdPlan backward_plan(int64_t M, int64_t D, bool plain) {
     p.blocks = std::min<int64_t>(M, 64);  // parts of norm_columns_kernel
     return p;
   }
-  p.U = D <= MAX_T * 512 ? 1 : (D <= MAX_T * 1024 ? 2 : 4);
+  p.U = D <= MAX_T * 512 ? 1 : 2;
   p.T = (int)((D + 512 * p.U - 1) / (512 * p.U));
   p.TB = p.T == 1 ? 4 : (p.T == 2 ? 2 : 1);
   const int64_t R = p.fast ? 1 : 4 / p.U, batches = (M + R - 1) / R;
@@ -1045,6 +1048,9 @@ BwdPlan backward_plan(int64_t M, int64_t D, bool plain) {
   p.blocks = std::min<int64_t>(MOST_PARTS, (batches + p.TB - 1) / p.TB);
   return p;
 }
+
+// The parameters' sums go through parts unless a single block has them all.
+int64_t part_bytes(const BwdPlan& p, int64_t D) { return p.T == 0 || p.blocks > 1 ? p.blocks * 2 * D * (int64_t)sizeof(float) : 0; }
 
 template <int DT, bool HOLD>
 int forward_typed(const FwdArgs& a, hipStream_t s) {
@@ -1091,8 +1097,7 @@ int backward_typed(BwdArgs& a, const BwdPlan& p, hipStream_t s) {
       }
     }
     if (p.U == 1) hipLaunchKernelGGL((norm_backward_kernel<XT, GT, 1>), grid, block, 0, s, a);
-    else if (p.U == 2) hipLaunchKernelGGL((norm_backward_kernel<XT, GT, 2>), grid, block, 0, s, a);
-    else hipLaunchKernelGGL((norm_backward_kernel<XT, GT, 4>), grid, block, 0, s, a);
+    else hipLaunchKernelGGL((norm_backward_kernel<XT, GT, 2>), grid, block, 0, s, a);
     SF_LAUNCH_CHECK("norm_backward_kernel");
     return SF_OK;
   }
@@ -1150,7 +1155,7 @@ extern "C" int sf_layer_norm_backward_workspace_size(int64_t M, int64_t D, int64
   sf_clear_error();
   if (const int rc = check_shape(M, D)) return rc;
   SF_REQUIRE(bytes, "sf_layer_norm_backward_workspace_size: NULL result");
-  *bytes = std::max(backward_plan(M, D, false).blocks, backward_plan(M, D, true).blocks) * 2 * D * (int64_t)sizeof(float);
+  *bytes = std::max(part_bytes(backward_plan(M, D, false), D), part_bytes(backward_plan(M, D, true), D));
   return SF_OK;
 }
 
@@ -1165,7 +1170,7 @@ extern "C" int sf_layer_norm_backward(const void* g, int64_t sgm, int g_dt, cons
   SF_REQUIRE((!w || sf_valid_dtype(w_dt)) && (!dw || sf_valid_dtype(dw_dt)) && (!db || sf_valid_dtype(db_dt)),
              "unsupported dtype code");
   hipStream_t s = (hipStream_t)stream;
-  const bool pg = dw || db, plain = (!dx || dx_dt == g_dt) && (!x || x_dt == g_dt) && !g_mean && !g_rstd;
+  const bool pg = dw || db, plain = (!dx || dx_dt == g_dt) && (!x || x_dt == g_dt);
   const BwdPlan p = backward_plan(M, D, plain);
   if (M > 0) {
     if (const int rc = check_matrix("g", g, sgm, g_dt, M, D)) return rc;
@@ -1179,7 +1184,7 @@ extern "C" int sf_layer_norm_backward(const void* g, int64_t sgm, int g_dt, cons
     SF_REQUIRE(rstd, "rstd must not be NULL");
     if (dx)
       if (const int rc = check_result("dx", dx, sdx, dx_dt, M, D)) return rc;
-    const int64_t need = pg && (p.T == 0 || p.blocks > 1) ? p.blocks * 2 * D * 4 : 0;
+    const int64_t need = pg ? part_bytes(p, D) : 0;
     SF_REQUIRE(need == 0 || (workspace && workspace_bytes >= need && (uintptr_t)workspace % 4 == 0),
                "workspace of %lld bytes, need %lld", (long long)workspace_bytes, (long long)need);
     if (!dx && !pg) return SF_OK;

@@ -302,3 +302,79 @@ def test_rows_that_are_not_numbers_reach_only_their_features():
     rest[3, on] = 0
     assert torch.isfinite(rest).all()
     assert torch.equal(dequantize_rows(quantize_rows(xg, shift=bd))[8].isnan().any().cpu(), torch.tensor(False))
+
+
+def test_sparse_backward_from_held_rows_four_items_a_wave():
+    """Over 40000 work items of less than four entries each, as on wide dictionaries."""
+    M, D, N = 2500, 72, 45100
+    g = torch.Generator().manual_seed(5)
+    cols = torch.stack([torch.randperm(N, generator=g)[:24].sort().values for _ in range(M)])
+    indptr, indices = torch.arange(0, 24 * M + 1, 24), cols.flatten().int()
+    values = torch.rand(24 * M, generator=g) + 0.1
+    n = lambda *s: torch.randn(*s, generator=g)  # noqa: E731
+    x, W_enc, W_dec, G = n(M, D), n(D, N) / D ** 0.5, n(N, D) / D ** 0.5, 0.1 * n(M, D)
+    b_enc, b_dec = torch.zeros(N), torch.zeros(D)
+    xg, We, be, Wd, bd, ip, ix, va, Gg = cuda(x, W_enc, b_enc, W_dec, b_dec, indptr, indices, values, G)
+    held = quantize_rows(xg)
+    got = sparse_backward(held, We, be, Wd, bd, (ip, ix, va), Gg)
+    rows, j = torch.arange(M).repeat_interleave(24), indices.long()
+    p = (G.double()[rows] * W_dec.double()[j]).sum(1)
+    pa = (G.double()[rows].abs() * W_dec.double()[j].abs()).sum(1)
+    v = held_values(held)[rows]
+    want = torch.zeros(N, D, dtype=torch.float64).index_add_(0, j, p[:, None] * v)
+    size = torch.zeros(N, D, dtype=torch.float64).index_add_(0, j, pa[:, None] * v.abs())
+    within(got.W_enc, want.T, U * (D / 64 + 24 + 16) * size.T, "dW_enc")
+    wd = torch.zeros(N, D, dtype=torch.float64).index_add_(0, j, values.double()[:, None] * G.double()[rows])
+    wa = torch.zeros(N, D, dtype=torch.float64).index_add_(0, j, values.double()[:, None] * G.double()[rows].abs())
+    within(got.W_dec, wd, U * 16 * wa, "dW_dec")
+
+
+@pytest.mark.parametrize("dtype,top", [(torch.float16, 65504.0), (torch.float32, 1e36), (torch.float32, 1e-37), (torch.bfloat16, 1e-38)])
+def test_held_rows_at_the_ends_of_their_range(dtype, top):
+    """Tokens near a type's largest number (whose code may stand for more than fp16 holds) and near the smallest."""
+    M, D, N = 12, 256, 64
+    x, W_enc, b_enc, W_dec, b_dec, csr, f, G, _ = problem(M, D, N, dtype, l0=10)
+    x = (torch.rand(M, D) * 2 - 1) * top
+    x[:, 0] = top
+    x[3, 130:] = 0
+    x = x.to(dtype)
+    b_dec = torch.zeros_like(b_dec)
+    scale = 1e-4 if top > 1 else 1e4  # of the gradients, so that results are ordinary numbers of their type
+    G = (G * scale).to(dtype)
+    xg, We, be, Wd, bd, ip, ix, va, Gg = cuda(x, W_enc, b_enc, W_dec, b_dec, *csr, G)
+    held = quantize_rows(xg, shift=bd)
+    got = sparse_backward(held, We, be, Wd, bd, (ip, ix, va), Gg, need_grad_x=False)
+    v, p = held_values(held), (G.double() @ W_dec.double().T) * (f != 0)
+    pa = (G.double().abs() @ W_dec.double().abs().T) * (f != 0)
+    want = v.T @ p
+    n = (f != 0).sum(0).double()
+    tol = U * (n + 8) * (v.abs().T @ p.abs()) + U * (D / 64 + 24) * (v.abs().T @ pa) + M * 2.0 ** -149
+    within(got.W_enc, want, 1.01 * half(dtype) * want.abs() + tiny(dtype) + 1.01 * tol, "dW_enc")
+    assert torch.isfinite(got.W_enc).all() and (want != 0).any()
+
+
+def test_held_rows_past_four_gigabytes():
+    M, D, N = 1_870_000, 2304, 64  # 4.3 GB of codes
+    dt = torch.bfloat16
+    at = torch.tensor([0, 1, 934_999, M - 2, M - 1])
+    g = torch.Generator().manual_seed(3)
+    n = lambda *s: torch.randn(*s, generator=g)  # noqa: E731
+    xs, Gs = n(5, D).to(dt), (0.1 * n(5, D)).to(dt)
+    W_enc, W_dec = (n(D, N) / 48).to(dt), (n(N, D) / 48).to(dt)
+    cols = torch.stack([torch.randperm(N, generator=g)[:40].sort().values for _ in range(5)])
+    counts = torch.zeros(M, dtype=torch.int64)
+    counts[at] = 40
+    indptr = torch.cat([torch.zeros(1, dtype=torch.int64), counts.cumsum(0)])
+    values = (torch.rand(200, generator=g) + 0.1).to(dt)
+    x, G = torch.zeros(M, D, dtype=dt, device="cuda"), torch.zeros(M, D, dtype=dt, device="cuda")
+    x[at.cuda()], G[at.cuda()] = xs.cuda(), Gs.cuda()
+    held = quantize_rows(x)
+    del x
+    We, Wd, be, bd = W_enc.cuda(), W_dec.cuda(), torch.zeros(N, dtype=dt, device="cuda"), torch.zeros(D, dtype=dt, device="cuda")
+    got = sparse_backward(held, We, be, Wd, bd, (indptr.cuda(), cols.flatten().int().cuda(), values.cuda()), G, need_grad_x=False)
+    on = torch.zeros(5, N, dtype=torch.float64).scatter_(1, cols, 1.0)
+    v = torch.cat([held_values(held[i:i + 1]) for i in at.tolist()])
+    p, pa = (Gs.double() @ W_dec.double().T) * on, (Gs.double().abs() @ W_dec.double().abs().T) * on
+    want = v.T @ p
+    tol = U * 16 * (v.abs().T @ p.abs()) + U * (D / 64 + 24) * (v.abs().T @ pa)
+    within(got.W_enc, want, 1.01 * half(dt) * want.abs() + tiny(dt) + 1.01 * tol, "dW_enc")

@@ -455,3 +455,30 @@ def test_graph_replays_match_eager():
         torch.cuda.synchronize()
         for i, (a, c, e) in enumerate(zip(want, outs, outs2)):
             assert torch.equal(a, c) and torch.equal(a, e), (seed, i)
+
+
+@pytest.mark.parametrize("D", [40, 1000, 8500])
+@pytest.mark.parametrize("size", [1e-18, 1e15])
+def test_rows_of_any_size(size, D):
+    """Deviations whose cubes leave fp32 (gradients of the rows go with 1 / size)."""
+    x, w, b, g = make(9, D, torch.float32)
+    x = x * size
+    xg, wg, bg, gg = cuda(x, w, b, g)
+    y, held, mean, rstd = kernels.layer_norm_held(xg, wg, bg, eps=0.0)
+    check_forward(x, w, b, y, mean, rstd, eps=0.0)
+    check_held(x, held)
+    _, mean64, rstd64, _ = onorm.forward(x, eps=0.0)
+    check_backward(g, x.double() - mean64[:, None], rstd64, w, b, kernels.layer_norm_backward(gg, xg, mean, rstd, wg, bg), mean64)
+    check_backward(g, held_values(held), rstd.cpu(), w, b, kernels.layer_norm_backward(gg, held, None, rstd, wg, bg), mean64, exact_input=True)
+
+
+@pytest.mark.parametrize("D", [96, 1003, 2304, 5000])
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_gradients_of_mean_and_rstd_from_held_rows(D, dtype):
+    x, w, b, g = make(23, D, dtype)
+    gm, gs = torch.randn(23), torch.randn(23)
+    xg, wg, bg, gg, gmg, gsg = cuda(x, w, b, g, gm, gs)
+    _, held, mean, rstd = kernels.layer_norm_held(xg, wg, bg)
+    for a, c in ((gmg, gsg), (gmg, None), (None, gsg)):
+        gr = kernels.layer_norm_backward(gg, held, None, rstd, wg, bg, grad_mean=a, grad_rstd=c)
+        check_backward(g, held_values(held), rstd.cpu(), w, b, gr, mean, a, c, exact_input=True)
