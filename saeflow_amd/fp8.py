@@ -17,9 +17,8 @@ trained SAE's encoder on the 8-bit matrix cores, to tokens or to the buffer's ro
 import torch
 
 from . import _lib
-from .kernels import dense_to_csr, fixed_width_to_dense, topk_rows
+from .kernels import dense_to_csr, fixed_width_to_dense, layer_norm, topk_rows
 from .kernels.fp8 import Fp8Rows, _vector, dequantize_rows, fused_encode_fp8, quantize_rows, read_rows
-from .norm import layer_norm
 from .ops import INPUT_NORMS, input_norm, norm_eps
 from .sae import ACTIVATIONS
 
@@ -144,7 +143,7 @@ class Fp8Encoder:
             return fused_encode_fp8(x, self.W, self.rows_bias, self.threshold, activation, out_dtype=out_dtype,
                                     row_nnz=row_nnz)
         if self.input_norm is not None:
-            x = layer_norm(x, eps=self.norm_eps)
+            x = layer_norm(x, eps=self.norm_eps)[0]
         return fused_encode_fp8(x, self.W, self.b_enc, self.threshold, activation, b_dec=self.b_dec,
                                 out_dtype=out_dtype, row_nnz=row_nnz)
 

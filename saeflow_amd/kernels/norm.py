@@ -50,6 +50,8 @@ def _code(t, name):
 
 
 def _row_stat(t, M, name):
+    if t is None:
+        raise ValueError(f"{name} is needed")
     if t.dtype != torch.float32 or t.dim() != 1 or t.shape[0] != M:
         raise ValueError(f"{name} must be a float32 tensor of shape [{M}], got {t.dtype} {list(t.shape)}")
     return t.contiguous()
@@ -124,10 +126,11 @@ def layer_norm_held(x, weight=None, bias=None, eps=1e-5, *, out_dtype=None):
     return y, held, *stats.unbind()
 
 
-def layer_norm_backward(grad_y, x, mean, rstd, weight=None, bias=None, *, need_grad_x=True, grad_mean=None,
-                        grad_rstd=None, out_dtype=None):
+def layer_norm_backward(grad_y, x, mean, rstd, weight=None, bias=None, *, need_grad_x=True, need_grad_weight=True,
+                        grad_mean=None, grad_rstd=None, out_dtype=None):
     """Gradients of a loss through layer_norm, from grad_y = dL/dy [M, D]: a namespace of x [M, D], weight and bias
-    (each in its parameter's type, None for one that is not given), x None without need_grad_x.
+    (each in its parameter's type, None for one that is not given), x None without need_grad_x, weight without
+    need_grad_weight.
 
     x: what layer_norm was given, or the Fp8Rows of layer_norm_held (then mean is not read and may be None).
     grad_mean, grad_rstd: float32 [M], gradients of the mean and rstd that the forward pass returned, if they were
@@ -164,7 +167,7 @@ def layer_norm_backward(grad_y, x, mean, rstd, weight=None, bias=None, *, need_g
     if need_grad_x:
         dx = _result(g if held else x, M, D, out_dtype or (g if held else x).dtype)
         dx_ptr, dx_code = dx.data_ptr(), _code(dx, "out_dtype")
-    if w is not None:
+    if w is not None and need_grad_weight:
         dw = torch.empty_like(w)
         dw_ptr = dw.data_ptr()
     if b is not None:

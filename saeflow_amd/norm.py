@@ -49,8 +49,8 @@ class LayerNormFunction(torch.autograd.Function):
         if g_y is None:
             g_y = torch.zeros((rstd.shape[0], ctx.d), dtype=ctx.x_dtype, device=rstd.device)
         gr = _k.layer_norm_backward(g_y, x, mean, rstd, weight, bias if need[2] else None, need_grad_x=need[0],
-                                    grad_mean=g_mean, grad_rstd=g_rstd, out_dtype=ctx.x_dtype)
-        return gr.x, gr.weight if need[1] else None, gr.bias, None, None
+                                    need_grad_weight=need[1], grad_mean=g_mean, grad_rstd=g_rstd, out_dtype=ctx.x_dtype)
+        return gr.x, gr.weight, gr.bias, None, None
 
 
 class DenormalizeFunction(torch.autograd.Function):
@@ -77,11 +77,12 @@ def layer_norm(x, weight=None, bias=None, eps=1e-5, *, hold=None, return_stats=F
     float32 [...]. Differentiable with respect to x, weight and bias (and through mean and rstd).
 
     hold: None, or torch.float8_e4m3fn: the backward pass keeps x - mean in 8 bits (a power-of-two scale for each
-      block of 128) in place of x. Each element is then off by at most 2^-4 of itself in the gradients; y is not touched.
+      block of 128) in place of x: for the gradients each element is off by at most 2^-4 of itself, or 2^-10 of its
+      block's scale; y is not touched.
     """
     held = check_hold(hold)
-    if x.dim() < 1:
-        raise ValueError("x needs a dimension to be normed over")
+    if x.dim() < 1 or x.shape[-1] < 1:
+        raise ValueError(f"x needs a dimension to be normed over, got {list(x.shape)}")
     lead = x.shape[:-1]
     rows = x if x.dim() == 2 else x.reshape(-1, x.shape[-1])
     if torch.is_grad_enabled() and (x.requires_grad or (weight is not None and weight.requires_grad)
@@ -100,7 +101,7 @@ def layer_norm(x, weight=None, bias=None, eps=1e-5, *, hold=None, return_stats=F
 def denormalize(h, mean, rstd):
     """h / rstd + mean over the rows of h [..., D], mean and rstd float32 [...] as layer_norm returned them, in h's type.
     Differentiable with respect to all three."""
-    if h.dim() < 1 or mean.shape != h.shape[:-1] or rstd.shape != h.shape[:-1]:
+    if h.dim() < 1 or h.shape[-1] < 1 or mean.shape != h.shape[:-1] or rstd.shape != h.shape[:-1]:
         raise ValueError(f"h {list(h.shape)} needs mean and rstd of its rows, got {list(mean.shape)} and {list(rstd.shape)}")
     rows, m, r = (h, mean, rstd) if h.dim() == 2 else (h.reshape(-1, h.shape[-1]), mean.reshape(-1), rstd.reshape(-1))
     if torch.is_grad_enabled() and (h.requires_grad or mean.requires_grad or rstd.requires_grad):

@@ -7,9 +7,8 @@ see kernels/decode.py.
 
 import torch
 
-from . import norm
-from .kernels import (dense_to_csr, encode_gather, encode_rows, fixed_width_to_dense, fused_encode,
-                      overflow_rows, rows_to_csr, rows_topk, scan_counts, sparse_decode, topk_gather, topk_rows)
+from .kernels import (dense_to_csr, denormalize, encode_gather, encode_rows, fixed_width_to_dense, fused_encode,
+                      layer_norm, overflow_rows, rows_to_csr, rows_topk, scan_counts, sparse_decode, topk_gather, topk_rows)
 
 # Row-candidate paths: the fused encode appends each row's selected features to a per-row list
 # instead of writing the dense [M, d_sae] features, which the reference writes and reads back
@@ -118,7 +117,7 @@ def norm_eps(sae):
 
 def normed_input(sae, x):
     """What the encoder reads: x, or its rows normed (in x's type)."""
-    return x if input_norm(sae) is None else norm.layer_norm(x, eps=norm_eps(sae))
+    return x if input_norm(sae) is None else layer_norm(x, eps=norm_eps(sae))[0]
 
 
 def encode(sae, x):
@@ -162,5 +161,5 @@ def forward(sae, x):
     With an input norm the reconstruction is carried back to x's own space."""
     if input_norm(sae) is None:
         return decode_sparse(sae, _encode_sparse(sae, x))
-    z, mean, rstd = norm.layer_norm(x, eps=norm_eps(sae), return_stats=True)
-    return norm.denormalize(decode_sparse(sae, _encode_sparse(sae, z)), mean, rstd)
+    z, mean, rstd = layer_norm(x, eps=norm_eps(sae))
+    return denormalize(decode_sparse(sae, _encode_sparse(sae, z)), mean, rstd)

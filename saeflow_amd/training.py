@@ -64,8 +64,9 @@ def forward_train(sae, x, *, hold=None):
     respect to x, W_enc, b_enc, W_dec and b_dec (and through `values`).
 
     hold: None, or torch.float8_e4m3fn: what the backward pass needs of the activations is kept in 8 bits (x - b_dec,
-      and x - mean of an input norm) in place of x, so dW_enc sums elements that are off by at most 2^-4 of themselves;
-      the features, x_hat and the other parameters' gradients are not touched."""
+      and x - mean of an input norm, each element off by at most 2^-4 of itself or 2^-10 of its block's scale) in
+      place of x. dW_enc sums those, and the gradient of x goes through an input norm by them; the features, x_hat and
+      the other gradients are not touched."""
     held = norm.check_hold(hold)
     normed = ops.input_norm(sae) is not None
     if normed:

@@ -378,3 +378,25 @@ def test_held_rows_past_four_gigabytes():
     want = v.T @ p
     tol = U * 16 * (v.abs().T @ p.abs()) + U * (D / 64 + 24) * (v.abs().T @ pa)
     within(got.W_enc, want, 1.01 * half(dt) * want.abs() + tiny(dt) + 1.01 * tol, "dW_enc")
+
+
+def test_an_sae_called_outside_of_training_gives_no_gradient():
+    """As without an input norm: what sae(x) returns is not part of a graph, not even through the rows' means."""
+    for norm in (None, "layer_norm"):
+        sae = make_sae(64, 128, "relu", torch.float32, norm)
+        x = torch.randn(8, 64, device="cuda", requires_grad=True)
+        assert sae(x).grad_fn is None and sae.encode(x).grad_fn is None and sae.encode_pre(x).grad_fn is None
+        assert Fp8Encoder.from_sae(sae).encode(x).grad_fn is None
+
+
+def test_a_frozen_norm_ahead_of_a_trained_one():
+    """Gradients of x alone through a layer norm whose parameters are fixed."""
+    x = torch.randn(40, 96, device="cuda", requires_grad=True)
+    w, b = torch.randn(96, device="cuda"), torch.randn(96, device="cuda")
+    G = torch.randn(40, 96, device="cuda")
+    layer_norm(x, w, b).backward(G)
+    with torch.no_grad():
+        _, mean, rstd = kernels.layer_norm(x, w, b)
+        gr = kernels.layer_norm_backward(G, x, mean, rstd, w, b, need_grad_weight=False)
+    assert gr.weight is None and torch.equal(x.grad, gr.x)
+    assert torch.equal(gr.bias, kernels.layer_norm_backward(G, x.detach(), mean, rstd, w, b).bias)

@@ -94,6 +94,10 @@ def test_shapes_and_values_are_refused():
                         (lambda: kernels.denormalize(x, s, torch.zeros(3)), "rstd"),
                         (lambda: kernels.denormalize_backward(x, None, s), "need h"),
                         (lambda: kernels.denormalize_backward(x, torch.zeros(4, 9), s), "h"),
+                        (lambda: kernels.layer_norm_backward(x, x, None, s), "mean"),
+                        (lambda: kernels.layer_norm_backward(x, x, s, None), "rstd"),
+                        (lambda: saeflow_amd.layer_norm(torch.zeros(3, 0)), "dimension"),
+                        (lambda: saeflow_amd.denormalize(torch.zeros(3, 0), torch.zeros(3), torch.zeros(3)), "mean and rstd"),
                         (lambda: saeflow_amd.layer_norm(x, hold=torch.int8), "hold"),
                         (lambda: saeflow_amd.layer_norm(torch.tensor(1.0)), "dimension"),
                         (lambda: saeflow_amd.denormalize(x, torch.zeros(4, 1), s), "needs mean and rstd"),
