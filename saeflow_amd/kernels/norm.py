@@ -176,7 +176,7 @@ def layer_norm_backward(grad_y, x, mean, rstd, weight=None, bias=None, *, need_g
     if dw is not None or db is not None:
         nbytes = _lib.layer_norm_workspace_bytes(M, D)
         if nbytes:
-            ws = g.new_empty(nbytes, dtype=torch.uint8)
+            ws = rstd.new_empty(nbytes // 4)
             ws_ptr = ws.data_ptr()
     _run(_lib.load().sf_layer_norm_backward, at, g.data_ptr(), g_row, g_code, *x_args, mean_ptr, rstd.data_ptr(),
          w_ptr, w_code, gm_ptr, gr_ptr, M, D, dx_ptr, D, dx_code, dw_ptr, w_code, db_ptr, b_code, ws_ptr, nbytes)

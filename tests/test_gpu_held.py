@@ -353,8 +353,9 @@ def test_held_rows_at_the_ends_of_their_range(dtype, top):
     assert torch.isfinite(got.W_enc).all() and (want != 0).any()
 
 
-def test_held_rows_past_four_gigabytes():
-    M, D, N = 1_870_000, 2304, 64  # 4.3 GB of codes
+@pytest.mark.parametrize("M", [1_100_000, 1_870_000])  # 2.5 and 4.3 GB of codes
+def test_held_rows_past_two_and_four_gigabytes(M):
+    D, N = 2304, 64
     dt = torch.bfloat16
     at = torch.tensor([0, 1, 934_999, M - 2, M - 1])
     g = torch.Generator().manual_seed(3)
@@ -400,3 +401,43 @@ def test_a_frozen_norm_ahead_of_a_trained_one():
         gr = kernels.layer_norm_backward(G, x, mean, rstd, w, b, need_grad_weight=False)
     assert gr.weight is None and torch.equal(x.grad, gr.x)
     assert torch.equal(gr.bias, kernels.layer_norm_backward(G, x.detach(), mean, rstd, w, b).bias)
+
+
+def test_no_tokens_and_tokens_without_features():
+    sae = make_sae(48, 96, "relu", torch.float32, "layer_norm")
+    for M, shift in ((0, 0.0), (5, -1e6)):
+        with torch.no_grad():
+            sae.b_enc.fill_(shift)
+        x = torch.randn(M, 48, device="cuda", requires_grad=True)
+        x_hat, csr = forward_train(sae, x, hold=torch.float8_e4m3fn)
+        assert x_hat.shape == (M, 48) and csr[1].numel() == 0
+        x_hat.sum().backward()
+        g = grads_of(sae)
+        assert all((g[n] == 0).all() for n in ("W_enc", "b_enc", "W_dec")) and x.grad.shape == (M, 48)
+        assert sae(x.detach()).shape == (M, 48)
+
+
+def test_two_streams_at_once():
+    """Backward passes side by side on two streams, each with its own workspaces."""
+    def inputs(seed):
+        x, W_enc, b_enc, W_dec, b_dec, csr, f, G, H = problem(800, 768, 512, torch.bfloat16, seed=seed, hot=2)
+        return cuda(x, W_enc, b_enc, W_dec, b_dec, *csr, G, H, torch.randn(768).bfloat16(), torch.randn(768).bfloat16())
+
+    def work(x, We, be, Wd, bd, ip, ix, va, G, H, w, b):
+        y, held, mean, rstd = kernels.layer_norm_held(x, w, b)
+        a = kernels.layer_norm_backward(G, held, None, rstd, w, b)
+        c = sparse_backward(quantize_rows(y, shift=bd), We, be, Wd, bd, (ip, ix, va), G, H)
+        return y, a.x, a.weight, a.bias, c.W_enc, c.W_dec, c.b_enc, c.b_dec, c.x
+
+    sets = [inputs(1), inputs(2)]
+    want = [work(*s) for s in sets]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    got = [None, None]
+    for _ in range(5):
+        for i in (0, 1):
+            with torch.cuda.stream(streams[i]):
+                got[i] = work(*sets[i])
+    torch.cuda.synchronize()
+    for i in (0, 1):
+        assert all(torch.equal(a, c) for a, c in zip(want[i], got[i]))
