@@ -401,6 +401,14 @@ SF_API int sf_column_sums(const void* A, int64_t M, int64_t D, int64_t sa, int d
 SF_API int sf_matvec(const void* W, int64_t R, int64_t C, int64_t swr, int64_t swc, int w_dt, const float* v,
               float sign, int accumulate, float* out, float* workspace, int64_t workspace_floats, void* stream);
 
+/* The biases' gradients of the sparse path in three launches: d_bdec [D] = sum_m g[m] - W d_benc for g [M, D] (rows sg apart,
+ * unit column stride) and W = W_enc [D, N] (any strides), summed as sf_column_sums and sf_matvec sum and rounded once
+ * to bdec_dt; out_benc [N] (or NULL) = d_benc (fp32 [N]) rounded to benc_dt. workspace: fp32 of at least (min(256,
+ * max(M, 1)) + min(256, max(N, 1))) * D floats. */
+SF_API int sf_backward_biases(const void* g, int64_t M, int64_t D, int64_t sg, int g_dt, const void* W, int64_t N,
+                              int64_t swr, int64_t swc, int w_dt, const float* d_benc, void* out_benc, int benc_dt,
+                              void* out_bdec, int bdec_dt, float* workspace, int64_t workspace_floats, void* stream);
+
 /*
  * Rows in 8 bits (no reference counterpart): e4m3 codes with one power-of-two scale for each block of
  * 128 elements along a row. Row r of a store of R rows over K elements: codes q + r * sq (sq bytes

@@ -68,6 +68,8 @@ SIGNATURES = {
     "sf_transpose": (_I32, [_P, _I64, _I64, _I64, _I32, _P, _P, _P]),
     "sf_column_sums": (_I32, [_P, _I64, _I64, _I64, _I32, ctypes.c_float, _I32, _P, _P, _I64, _P]),
     "sf_matvec": (_I32, [_P, _I64, _I64, _I64, _I64, _I32, _P, ctypes.c_float, _I32, _P, _P, _I64, _P]),
+    "sf_backward_biases": (_I32, [_P, _I64, _I64, _I64, _I32, _P, _I64, _I64, _I64, _I32, _P, _P, _I32, _P, _I32, _P, _I64,
+                                  _P]),
     "sf_quantize_rows": (_I32, [_P, _I64, _I64, _I32, _P, _I32, _I64, _I64, _P, _I64, _P, _I64, _I64, _I64, _P]),
     "sf_dequantize_rows": (_I32, [_P, _I64, _P, _I64, _I64, _P, _I64, _P, _I32, _I64, _I64, _P, _I64, _I32, _P]),
     "sf_encode_fp8_rows": (_I32, [_P, _I64, _P, _I64, _P, _I64, _P, _I64, _P, _I32, _P, _I32, _P, _I64, _I32, _P, _I64,
@@ -174,6 +176,16 @@ def fp8_workspace_bytes(M, K):
     nbytes = ctypes.c_int64()
     check(load().sf_encode_fp8_workspace_size(M, K, ctypes.byref(nbytes)))
     return nbytes.value
+
+
+@functools.lru_cache(maxsize=256)
+def backward_sizes(M, N, nnz, D, code):
+    """sf_csr_transpose_workspace_size and sf_backward_bounds, functions of their arguments alone: (bytes, work
+    items, partial slots, floats)."""
+    nbytes, items, slots, floats = (ctypes.c_int64() for _ in range(4))
+    check(load().sf_csr_transpose_workspace_size(M, N, nnz, ctypes.byref(nbytes)))
+    check(load().sf_backward_bounds(N, nnz, D, code, ctypes.byref(items), ctypes.byref(slots), ctypes.byref(floats)))
+    return nbytes.value, items.value, slots.value, floats.value
 
 
 @functools.lru_cache(maxsize=256)

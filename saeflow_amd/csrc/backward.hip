@@ -235,6 +235,8 @@ constexpr int CSC_MAX_LB = 11;    // pass 4 keeps 4 x 2^LB counters in LDS (32 K
 constexpr int CSC_MAX_NB = 4096;  // passes 1 and 3 keep 4 x nb counters in LDS (64 KB)
 constexpr int CSC_MAX_RW = 32;    // a wave's row offsets sit in its lanes
 constexpr int CSC_U = 4;          // 64-entry chunks whose loads are in flight together
+constexpr int CSC_SHORT_RW = 16;
+constexpr int64_t CSC_ONE_SCAN = 4096;
 
 struct CscPlan {
   int LB, nb, nb_bits;
@@ -253,6 +255,12 @@ CscPlan csc_plan(int64_t M, int64_t N) {
   p.nb = (int)std::max<int64_t>(1, (N + (1LL << p.LB) - 1) >> p.LB);
   p.nb_bits = bits_for(p.nb);
   p.RW = std::min<int64_t>(CSC_MAX_RW, std::max<int64_t>(1, (M + CSC_WAVES - 1) / CSC_WAVES));
+  // Few tokens: as few waves as leave 4096 counters, which sf_scan_counts takes in one round of one small block, as long as
+  // a wave walks no more than CSC_SHORT_RW rows (the order of the result is the same). Scan, us: 128 tokens of 24576 features 17
+  // -> 5; up to 32768 counters, which would still be one launch in place of three, 20 against 10 for more tokens.
+  int64_t rw = p.RW;
+  while (rw <= CSC_SHORT_RW && (M + rw - 1) / rw * p.nb > CSC_ONE_SCAN) ++rw;
+  if (rw <= CSC_SHORT_RW) p.RW = rw;
   p.S = std::max<int64_t>(1, (M + p.RW - 1) / p.RW);
   return p;
 }
@@ -1486,6 +1494,49 @@ __global__ __launch_bounds__(256) void col_sums_final_kernel(const float* part, 
   }
 }
 
+// The biases' gradients from the partial sums, each in its parameter's type: db_dec[d] = (column sums of g_xhat) - (W_enc
+// db_enc)[d], added up as col_sums_final_kernel and, for a row-contiguous W_enc (V_ROWS), matvec_final_kernel add, and
+// db_enc rounded on the way (blocks behind the first ceil(D / 64)).
+__global__ __launch_bounds__(256) void biases_kernel(const float* part_g, int64_t nparts_g, const float* part_w,
+                                                     int64_t nparts_w, int v_rows, int64_t D, void* d_bdec, int bdec_dt,
+                                                     const float* d_benc, int64_t N, void* out_benc, int benc_dt) {
+  const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6;
+  const int64_t nd = (D + 63) / 64;
+  if ((int64_t)blockIdx.x >= nd) {
+    const int64_t i = ((int64_t)blockIdx.x - nd) * 256 + threadIdx.x;
+    if (i < N) {
+      if (benc_dt == SF_F32) ((float*)out_benc)[i] = d_benc[i];
+      else ((u16*)out_benc)[i] = (u16)f32_to_bits(d_benc[i], benc_dt);
+    }
+    return;
+  }
+  __shared__ float s_g[3][64], s_v[3][64];
+  const int64_t d = (int64_t)blockIdx.x * 64 + lane, dc = min(d, D - 1);
+  float s = 0.f, v = 0.f;
+#pragma unroll 8
+  for (int64_t p = wv; p < nparts_g; p += 4) s += part_g[p * D + dc];
+  if (v_rows) {
+    if (wv == 0) {
+#pragma unroll 8
+      for (int64_t p = 0; p < nparts_w; ++p) v += part_w[dc * nparts_w + p];
+    }
+  } else {
+#pragma unroll 8
+    for (int64_t p = wv; p < nparts_w; p += 4) v += part_w[p * D + dc];
+  }
+  if (wv > 0) {
+    s_g[wv - 1][lane] = s;
+    s_v[wv - 1][lane] = v;
+  }
+  __syncthreads();
+  if (wv != 0 || d >= D) return;
+  s = ((s + s_g[0][lane]) + s_g[1][lane]) + s_g[2][lane];
+  if (!v_rows) v = ((v + s_v[0][lane]) + s_v[1][lane]) + s_v[2][lane];
+  s -= v;
+  if (bdec_dt == SF_F32) ((float*)d_bdec)[d] = s;
+  else ((u16*)d_bdec)[d] = (u16)f32_to_bits(s, bdec_dt);
+}
+
 bool aligned16(const void* p, int64_t stride_elems, int es) {
   return ((uintptr_t)p % 16) == 0 && ((stride_elems * es) % 16) == 0;
 }
@@ -1886,27 +1937,35 @@ extern "C" int sf_transpose(const void* src, int64_t R, int64_t C, int64_t ss, i
   return SF_OK;
 }
 
+// Partial sums [nparts, D] of the columns of A [M, D] (row stride sa, unit column stride), M > 0, rows weighted by w if given.
+static int column_parts(const void* A, int64_t M, int64_t D, int64_t sa, int dt, const float* w, int64_t nparts,
+                        float* workspace, hipStream_t s) {
+  const int es = sf_dtype_size(dt), epc = 16 / es;
+  const bool vec = D % epc == 0 && aligned16(A, sa, es);
+  const int64_t rows_per = (M + nparts - 1) / nparts;
+  const dim3 grid((unsigned)((D + 64 * epc - 1) / (64 * epc)), (unsigned)nparts);
+  const char* a = (const char*)A;
+#define SF_CS(DTV, VECV) hipLaunchKernelGGL((col_sums_kernel<DTV, VECV>), grid, dim3(256), 0, s, a, M, D, sa, w, rows_per, workspace)
+  switch (dt) {
+    case SF_BF16: if (vec) SF_CS(SF_BF16, true); else SF_CS(SF_BF16, false); break;
+    case SF_F16: if (vec) SF_CS(SF_F16, true); else SF_CS(SF_F16, false); break;
+    default: if (vec) SF_CS(SF_F32, true); else SF_CS(SF_F32, false); break;
+  }
+#undef SF_CS
+  SF_LAUNCH_CHECK("col_sums_kernel");
+  return SF_OK;
+}
+static int64_t column_nparts(int64_t M) { return std::max<int64_t>(1, std::min<int64_t>(256, M)); }
+
 // Weighted or plain column sums of A [M, D] (row stride sa, unit column stride) into out.
 static int column_sums(const void* A, int64_t M, int64_t D, int64_t sa, int dt, const float* w, float sign,
                        int accumulate, float* out, float* workspace, int64_t workspace_floats, hipStream_t s,
                        const char* who) {
-  const int64_t nparts = std::max<int64_t>(1, std::min<int64_t>(256, M));
+  const int64_t nparts = column_nparts(M);
   SF_REQUIRE(workspace_floats >= nparts * D, "%s: workspace of %lld floats, need %lld", who,
              (long long)workspace_floats, (long long)(nparts * D));
-  const int es = sf_dtype_size(dt), epc = 16 / es;
   if (M > 0) {
-    const bool vec = D % epc == 0 && aligned16(A, sa, es);
-    const int64_t rows_per = (M + nparts - 1) / nparts;
-    const dim3 grid((unsigned)((D + 64 * epc - 1) / (64 * epc)), (unsigned)nparts);
-    const char* a = (const char*)A;
-#define SF_CS(DTV, VECV) hipLaunchKernelGGL((col_sums_kernel<DTV, VECV>), grid, dim3(256), 0, s, a, M, D, sa, w, rows_per, workspace)
-    switch (dt) {
-      case SF_BF16: if (vec) SF_CS(SF_BF16, true); else SF_CS(SF_BF16, false); break;
-      case SF_F16: if (vec) SF_CS(SF_F16, true); else SF_CS(SF_F16, false); break;
-      default: if (vec) SF_CS(SF_F32, true); else SF_CS(SF_F32, false); break;
-    }
-#undef SF_CS
-    SF_LAUNCH_CHECK("col_sums_kernel");
+    if (const int rc = column_parts(A, M, D, sa, dt, w, nparts, workspace, s)) return rc;
   } else {
     hipLaunchKernelGGL(fill_i32_kernel, dim3((unsigned)((D + 255) / 256)), dim3(256), 0, s, (int32_t*)workspace, D,
                        0);
@@ -1915,6 +1974,28 @@ static int column_sums(const void* A, int64_t M, int64_t D, int64_t sa, int dt, 
   hipLaunchKernelGGL(col_sums_final_kernel, dim3((unsigned)((D + 63) / 64)), dim3(256), 0, s, workspace,
                      M > 0 ? nparts : 1, D, sign, out, accumulate);
   SF_LAUNCH_CHECK("col_sums_final_kernel");
+  return SF_OK;
+}
+
+// Partial sums [R, nparts] of W v for a row-contiguous W.
+static int64_t matvec_nparts(int64_t C) { return std::max<int64_t>(1, std::min<int64_t>(64, (C + 8191) / 8192)); }
+static int matvec_parts(const void* W, int64_t R, int64_t C, int64_t swr, int64_t swc, int w_dt, const float* v,
+                        int64_t nparts, float* workspace, hipStream_t s) {
+  const int es = sf_dtype_size(w_dt), epc = 16 / es;
+  const bool vec = swc == 1 && C % epc == 0 && aligned16(W, swr, es) && ((uintptr_t)v % 16) == 0;
+  const int64_t cols_per = ((C + nparts - 1) / nparts + epc - 1) / epc * epc;
+  const char* w = (const char*)W;
+  const int64_t blocks = (R + MV_RB - 1) / MV_RB * nparts;
+  SF_REQUIRE(blocks < (1LL << 24), "sf_matvec: %lld rows is too many", (long long)R);
+  const dim3 grid((unsigned)blocks);
+#define SF_MV(DTV, VECV) hipLaunchKernelGGL((matvec_kernel<DTV, VECV>), grid, dim3(256), 0, s, w, R, C, swr, swc, v, cols_per, nparts, workspace)
+  switch (w_dt) {
+    case SF_BF16: if (vec) SF_MV(SF_BF16, true); else SF_MV(SF_BF16, false); break;
+    case SF_F16: if (vec) SF_MV(SF_F16, true); else SF_MV(SF_F16, false); break;
+    default: if (vec) SF_MV(SF_F32, true); else SF_MV(SF_F32, false); break;
+  }
+#undef SF_MV
+  SF_LAUNCH_CHECK("matvec_kernel");
   return SF_OK;
 }
 
@@ -1939,26 +2020,45 @@ extern "C" int sf_matvec(const void* W, int64_t R, int64_t C, int64_t swr, int64
   hipStream_t s = (hipStream_t)stream;
   if (swc != 1 && swr == 1 && C > 0)  // column-contiguous W: the v-weighted column sums of W^T [C, R]
     return column_sums(W, C, R, swc, w_dt, v, sign, accumulate, out, workspace, workspace_floats, s, "sf_matvec");
-  const int64_t nparts = std::max<int64_t>(1, std::min<int64_t>(64, (C + 8191) / 8192));
+  const int64_t nparts = matvec_nparts(C);
   SF_REQUIRE(workspace_floats >= R * nparts, "sf_matvec: workspace of %lld floats, need %lld",
              (long long)workspace_floats, (long long)(R * nparts));
-  const int es = sf_dtype_size(w_dt), epc = 16 / es;
-  const bool vec = swc == 1 && C % epc == 0 && aligned16(W, swr, es) && ((uintptr_t)v % 16) == 0;
-  const int64_t cols_per = ((C + nparts - 1) / nparts + epc - 1) / epc * epc;
-  const char* w = (const char*)W;
-  const int64_t blocks = (R + MV_RB - 1) / MV_RB * nparts;
-  SF_REQUIRE(blocks < (1LL << 24), "sf_matvec: %lld rows is too many", (long long)R);
-  const dim3 grid((unsigned)blocks);
-#define SF_MV(DTV, VECV) hipLaunchKernelGGL((matvec_kernel<DTV, VECV>), grid, dim3(256), 0, s, w, R, C, swr, swc, v, cols_per, nparts, workspace)
-  switch (w_dt) {
-    case SF_BF16: if (vec) SF_MV(SF_BF16, true); else SF_MV(SF_BF16, false); break;
-    case SF_F16: if (vec) SF_MV(SF_F16, true); else SF_MV(SF_F16, false); break;
-    default: if (vec) SF_MV(SF_F32, true); else SF_MV(SF_F32, false); break;
-  }
-#undef SF_MV
-  SF_LAUNCH_CHECK("matvec_kernel");
+  if (const int rc = matvec_parts(W, R, C, swr, swc, w_dt, v, nparts, workspace, s)) return rc;
   hipLaunchKernelGGL(matvec_final_kernel, dim3((unsigned)((R + 255) / 256)), dim3(256), 0, s, workspace, R, nparts,
                      sign, accumulate, out);
   SF_LAUNCH_CHECK("matvec_final_kernel");
+  return SF_OK;
+}
+
+extern "C" int sf_backward_biases(const void* g, int64_t M, int64_t D, int64_t sg, int g_dt, const void* W, int64_t N,
+                                  int64_t swr, int64_t swc, int w_dt, const float* d_benc, void* out_benc, int benc_dt,
+                                  void* out_bdec, int bdec_dt, float* workspace, int64_t workspace_floats, void* stream) {
+  sf_clear_error();
+  SF_REQUIRE(M >= 0 && N >= 0 && D >= 0 && D < (1LL << 24), "sf_backward_biases: bad size");
+  SF_REQUIRE(sf_valid_dtype(g_dt) && sf_valid_dtype(w_dt) && sf_valid_dtype(bdec_dt) && (!out_benc || sf_valid_dtype(benc_dt)),
+             "sf_backward_biases: bad dtype");
+  SF_REQUIRE((D == 0 || out_bdec) && (M == 0 || D == 0 || g) && (N == 0 || (d_benc && (D == 0 || W))),
+             "sf_backward_biases: NULL buffer");
+  const int64_t need = (column_nparts(M) + column_nparts(N)) * D;
+  SF_REQUIRE(need == 0 || (workspace && workspace_floats >= need), "sf_backward_biases: workspace of %lld floats, need %lld",
+             (long long)workspace_floats, (long long)need);
+  hipStream_t s = (hipStream_t)stream;
+  const int v_rows = !(swc != 1 && swr == 1);  // (a column-contiguous W_enc: the weighted column sums of its transpose)
+  const int64_t ng = M > 0 && D > 0 ? column_nparts(M) : 0, nw = N > 0 && D > 0 ? (v_rows ? matvec_nparts(N) : column_nparts(N)) : 0;
+  float* part_w = workspace + ng * D;
+  if (ng) {
+    if (const int rc = column_parts(g, M, D, sg, g_dt, nullptr, ng, workspace, s)) return rc;
+  }
+  if (nw) {
+    if (const int rc = v_rows ? matvec_parts(W, D, N, swr, swc, w_dt, d_benc, nw, part_w, s)
+                              : column_parts(W, N, D, swc, w_dt, d_benc, nw, part_w, s))
+      return rc;
+  }
+  const int64_t blocks = (D + 63) / 64 + (out_benc ? (N + 255) / 256 : 0);
+  if (blocks == 0) return SF_OK;
+  SF_REQUIRE(blocks < (1LL << 31), "sf_backward_biases: too many features");
+  hipLaunchKernelGGL(biases_kernel, dim3((unsigned)blocks), dim3(256), 0, s, workspace, ng, part_w, nw, v_rows, D, out_bdec,
+                     bdec_dt, d_benc, N, out_benc, benc_dt);
+  SF_LAUNCH_CHECK("biases_kernel");
   return SF_OK;
 }

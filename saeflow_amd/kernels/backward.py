@@ -75,6 +75,7 @@ def sparse_backward(x, W_enc, b_enc, W_dec, b_dec, csr, grad_x_hat=None, grad_va
         raise ValueError(f"indptr has {indptr.numel()} entries for {M} rows")
     dt = W_dec.dtype
     code = _lib.dtype_code(W_dec, "W_dec")
+    es = W_dec.element_size()
     nnz = indices.numel()
     lib = _lib.load()
     with _lib.device(dev):
@@ -87,48 +88,48 @@ def sparse_backward(x, W_enc, b_enc, W_dec, b_dec, csr, grad_x_hat=None, grad_va
         gv = None if grad_values is None else grad_values.reshape(-1).contiguous()
         if gv is not None and gv.numel() != nnz:
             raise ValueError(f"grad_values has {gv.numel()} entries for nnz={nnz}")
+        csc_bytes, max_items, max_slots, work_floats = _lib.backward_sizes(M, N, nnz, D, code)
+        bias_floats = (min(256, max(M, 1)) + min(256, max(N, 1))) * D
+        benc_code, bdec_code = _lib.DTYPE.get(b_enc.dtype), _lib.DTYPE.get(b_dec.dtype)
+        own_benc = benc_code != 0 and benc_code is not None  # fp32 db_enc is needed, and rounded at the end
+        # all scratch is one tensor (a tensor made is 1.4 us on the host, a pass over few tokens 25 launches)
+        at, total = [], 0
+        for nbytes in (8 * (N + 1), 4 * nnz, 4 * nnz, csc_bytes, 24 * (N + 1), 4 * max_items, 4 * N, 4 * max_slots,
+                       4 * max_slots * (2 * D + 1), 4 * work_floats, 4 * bias_floats, 4 * N if own_benc else 0,
+                       0 if held else M * D * es):
+            at.append(total)
+            total += (nbytes + 255) // 256 * 256
+        scratch = torch.empty(total, dtype=torch.uint8, device=dev)
+        base = scratch.data_ptr()
+        (colptr, rows, pos, csc_ws, plan, item_col, multi_col, slot_item, partials, work, bias_ws, benc32,
+         xs) = (base + o for o in at)
+        ip, ix = indptr.data_ptr(), indices.data_ptr()
         # per-feature sums over the CSC
-        colptr, rows, pos = csr_transpose(indptr, indices, N)
+        _lib.check(lib.sf_csr_transpose(ip, ix, M, N, nnz, colptr, rows, pos, csc_ws, csc_bytes, s))
         if held:  # gathered as they lie
             columns, x_args = lib.sf_backward_columns_held, x._args()
         else:
-            xs = torch.empty(M, D, dtype=dt, device=dev)
             _lib.check(lib.sf_shifted_input(_lib.ptr(x), x.stride(0), x.stride(1), _lib.dtype_code(x, "x"),
-                                            _lib.ptr(b_dec), _lib.dtype_code(b_dec, "b_dec"), M, D, code, _lib.ptr(xs), s))
-            columns, x_args = lib.sf_backward_columns, (_lib.ptr(xs), D)
-        plan_i64 = torch.empty(3 * (N + 1), dtype=torch.int64, device=dev)
-        max_items, max_slots, work_floats = ctypes.c_int64(), ctypes.c_int64(), ctypes.c_int64()
-        _lib.check(lib.sf_backward_bounds(N, nnz, D, code, ctypes.byref(max_items), ctypes.byref(max_slots),
-                                          ctypes.byref(work_floats)))
-        item_col = torch.empty(max_items.value, dtype=torch.int32, device=dev)
-        multi_col = torch.empty(N, dtype=torch.int32, device=dev)
-        slot_item = torch.empty(max_slots.value, dtype=torch.int32, device=dev)
-        _lib.check(lib.sf_backward_plan(_lib.ptr(colptr), N, nnz, _lib.ptr(plan_i64), _lib.ptr(item_col),
-                                        _lib.ptr(multi_col), _lib.ptr(slot_item), s))
+                                            _lib.ptr(b_dec), _lib.dtype_code(b_dec, "b_dec"), M, D, code, xs, s))
+            columns, x_args = lib.sf_backward_columns, (xs, D)
+        _lib.check(lib.sf_backward_plan(colptr, N, nnz, plan, item_col, multi_col, slot_item, s))
         g_pre = torch.empty(nnz, dtype=torch.float32, device=dev)  # dL/dpre on the nonzeros
-        d_wdec = torch.empty(N, D, dtype=dt, device=dev)
-        d_wenc = torch.empty(D, N, dtype=dt, device=dev)
-        d_benc = torch.empty(N, dtype=torch.float32, device=dev)
-        partials = torch.empty(max_slots.value * (2 * D + 1), dtype=torch.float32, device=dev)
-        work = torch.empty(work_floats.value, dtype=torch.float32, device=dev)
+        d_wdec = torch.empty((N, D), dtype=dt, device=dev)
+        d_wenc = torch.empty((D, N), dtype=dt, device=dev)
+        d_benc = torch.empty(N, dtype=b_enc.dtype if own_benc else torch.float32, device=dev)
+        benc = benc32 if own_benc else d_benc.data_ptr()
         # the grid is sized by the bound of the work-item count (surplus waves return at once), so
         # nothing here waits for the GPU
-        _lib.check(columns(_lib.ptr(colptr), _lib.ptr(rows), _lib.ptr(pos), _lib.ptr(plan_i64), _lib.ptr(item_col),
-                           _lib.ptr(multi_col), _lib.ptr(slot_item), max_items.value, max_slots.value, _lib.ptr(values),
-                           _lib.dtype_code(values, "values"), _lib.ptr(gv),
-                           0 if gv is None else _lib.dtype_code(gv, "grad_values"), _lib.ptr(Wd), Wd.stride(0), *x_args,
-                           _lib.ptr(g), g.stride(0), code, N, M, D, nnz, _lib.ptr(g_pre), _lib.ptr(d_wdec),
-                           _lib.ptr(d_wenc), _lib.ptr(d_benc), _lib.ptr(partials), _lib.ptr(work), work.numel(), s))
-        del partials, work
-        xs = None  # (its memory is free for what follows)
+        _lib.check(columns(colptr, rows, pos, plan, item_col, multi_col, slot_item, max_items, max_slots,
+                           values.data_ptr(), _lib.dtype_code(values, "values"), _lib.ptr(gv),
+                           0 if gv is None else _lib.dtype_code(gv, "grad_values"), Wd.data_ptr(), Wd.stride(0), *x_args,
+                           g.data_ptr(), g.stride(0), code, N, M, D, nnz, g_pre.data_ptr(), d_wdec.data_ptr(),
+                           d_wenc.data_ptr(), benc, partials, work, work_floats, s))
         # db_dec = sum_m g_xhat[m] - sum_m dx'[m], and sum_m dx'[m] = W_enc db_enc
-        d_bdec = torch.empty(D, dtype=torch.float32, device=dev)
-        ws = torch.empty(min(256, max(M, 1)) * D, dtype=torch.float32, device=dev)
-        _lib.check(lib.sf_column_sums(_lib.ptr(g), M, D, g.stride(0), code, 1.0, 0, _lib.ptr(d_bdec), _lib.ptr(ws),
-                                      ws.numel(), s))
-        mv_ws = torch.empty(D * min(256, max(N, 1)), dtype=torch.float32, device=dev)
-        _lib.check(lib.sf_matvec(_lib.ptr(W_enc), D, N, W_enc.stride(0), W_enc.stride(1), code, _lib.ptr(d_benc),
-                                 -1.0, 1, _lib.ptr(d_bdec), _lib.ptr(mv_ws), mv_ws.numel(), s))
+        d_bdec = torch.empty(D, dtype=torch.float32 if bdec_code is None else b_dec.dtype, device=dev)
+        _lib.check(lib.sf_backward_biases(g.data_ptr(), M, D, g.stride(0), code, W_enc.data_ptr(), N, W_enc.stride(0),
+                                          W_enc.stride(1), code, benc, d_benc.data_ptr() if own_benc else None,
+                                          benc_code or 0, d_bdec.data_ptr(), bdec_code or 0, bias_ws, bias_floats, s))
         dxs = None
         if need_grad_x:  # dx' = g_pre W_enc^T: the forward decode over the rows of W_enc^T
             if W_enc.stride(0) == 1:  # W_enc is the transpose of a row-major [d_sae, d_in]
@@ -138,8 +139,8 @@ def sparse_backward(x, W_enc, b_enc, W_dec, b_dec, csr, grad_x_hat=None, grad_va
                 We = _rows(W_enc, dt)
                 _lib.check(lib.sf_transpose(_lib.ptr(We), D, N, We.stride(0), code, None, _lib.ptr(W_encT), s))
             dxs = torch.empty(M, D, dtype=torch.float32, device=dev)
-            _lib.check(lib.sf_decode(_lib.ptr(indptr), _lib.ptr(indices), _lib.ptr(g_pre), _lib.DTYPE[torch.float32],
+            _lib.check(lib.sf_decode(ip, ix, g_pre.data_ptr(), _lib.DTYPE[torch.float32],
                                      nnz, _lib.ptr(W_encT), W_encT.stride(0), W_encT.stride(1), code, N, None, 0,
                                      _lib.ptr(dxs), D, 1, _lib.DTYPE[torch.float32], M, D, None, s))
-    return SimpleNamespace(W_enc=d_wenc.to(W_enc.dtype), b_enc=d_benc.to(b_enc.dtype), W_dec=d_wdec,
+    return SimpleNamespace(W_enc=d_wenc, b_enc=d_benc.to(b_enc.dtype), W_dec=d_wdec,
                            b_dec=d_bdec.to(b_dec.dtype), x=dxs if dxs is None or held else dxs.to(x.dtype), pre=g_pre)

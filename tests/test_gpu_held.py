@@ -12,7 +12,7 @@ import torch
 import saeflow_amd
 from cache_model import TinyHooked
 from oracle import norm as onorm
-from saeflow_amd import SAE, Fp8Encoder, denormalize, forward_train, kernels, layer_norm
+from saeflow_amd import SAE, Fp8Encoder, _lib, denormalize, forward_train, kernels, layer_norm
 from saeflow_amd.cache import ActivationReader, cache_activations
 from saeflow_amd.kernels import csr_to_dense, dequantize_rows, quantize_rows, sparse_backward
 from test_gpu_norm import U, cuda, half, held_values, tiny, within
@@ -441,3 +441,42 @@ def test_two_streams_at_once():
     torch.cuda.synchronize()
     for i in (0, 1):
         assert all(torch.equal(a, c) for a, c in zip(want[i], got[i]))
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("M,D,N", [(1, 64, 256), (300, 1003, 777), (0, 40, 50), (17, 40, 0), (900, 513, 20000)])
+@pytest.mark.parametrize("transposed", [False, True])
+def test_biases_are_the_sums_of_their_parts(M, D, N, dtype, transposed):
+    """sf_backward_biases against sf_column_sums and sf_matvec, bit for bit, and rounded."""
+    lib, dev = _lib.load(), torch.device("cuda", torch.cuda.current_device())
+    g = torch.randn(M, D + 3, device="cuda").to(dtype)[:, :D]
+    W = torch.randn(N, D, device="cuda").to(dtype).T if transposed else torch.randn(D, N, device="cuda").to(dtype)
+    v = torch.randn(N, device="cuda")
+    code, s = _lib.DTYPE[dtype], _lib.stream(dev)
+    ws = torch.empty((min(256, max(M, 1)) + min(256, max(N, 1))) * D, device="cuda")
+    want = torch.empty(D, device="cuda")
+    _lib.check(lib.sf_column_sums(g.data_ptr(), M, D, D + 3, code, 1.0, 0, want.data_ptr(), ws.data_ptr(), ws.numel(), s))
+    _lib.check(lib.sf_matvec(W.data_ptr(), D, N, W.stride(0), W.stride(1), code, v.data_ptr(), -1.0, 1, want.data_ptr(),
+                             ws.data_ptr(), ws.numel(), s))
+    for out in DTYPES:
+        d_bdec, d_benc = torch.empty(D, dtype=out, device="cuda"), torch.empty(N, dtype=out, device="cuda")
+        _lib.check(lib.sf_backward_biases(g.data_ptr(), M, D, D + 3, code, W.data_ptr(), N, W.stride(0), W.stride(1), code,
+                                          v.data_ptr(), d_benc.data_ptr(), _lib.DTYPE[out], d_bdec.data_ptr(), _lib.DTYPE[out],
+                                          ws.data_ptr(), ws.numel(), s))
+        assert torch.equal(d_bdec, want.to(out)) and torch.equal(d_benc, v.to(out))
+
+
+def test_transposes_of_few_tokens_are_those_of_many():
+    """The plan of the counting sort changes with the number of tokens; its result does not."""
+    from saeflow_amd.kernels import csr_transpose
+
+    g = torch.Generator().manual_seed(9)
+    for M in (1, 16, 85, 86, 340, 341, 342, 700):
+        counts = torch.randint(0, 90, (M,), generator=g)
+        indptr = torch.cat([torch.zeros(1, dtype=torch.int64), counts.cumsum(0)])
+        indices = torch.randint(0, 24576, (int(indptr[-1]),), generator=g).int()
+        colptr, rows, pos = csr_transpose(indptr.cuda(), indices.cuda(), 24576)
+        order = torch.sort(indices, stable=True).indices
+        assert torch.equal(pos.cpu().long(), order)
+        assert torch.equal(rows.cpu().long(), torch.arange(M).repeat_interleave(counts)[order])
+        assert torch.equal(colptr.cpu(), torch.cat([torch.zeros(1, dtype=torch.int64), torch.bincount(indices.long(), minlength=24576).cumsum(0)]))

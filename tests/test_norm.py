@@ -171,3 +171,17 @@ def test_c_abi_refuses_bad_arguments_without_touching_the_gpu():
     refused(lib.sf_denormalize(16, 8, 3, 16, 16, 4, 8, 16, 8, 1, None), b"dtype")
     refused(lib.sf_denormalize_backward(16, 8, 1, None, 8, 1, 16, 4, 8, 16, 8, 1, 16, 16, None), b"h must not be NULL")
     refused(lib.sf_denormalize_backward(16, 8, 1, 16, 8, 1, None, 4, 8, 16, 8, 1, None, None, None), b"rstd")
+    P = 16
+    refused(lib.sf_backward_biases(P, 4, 8, 8, 5, P, 4, 4, 1, 1, P, None, 0, P, 0, P, 64, None), b"dtype")
+    refused(lib.sf_backward_biases(P, 4, 8, 8, 1, P, 4, 4, 1, 1, None, None, 0, P, 0, P, 64, None), b"NULL")
+    refused(lib.sf_backward_biases(P, 4, 8, 8, 1, P, 4, 4, 1, 1, P, None, 0, P, 0, P, 63, None), b"workspace")
+    refused(lib.sf_backward_biases(P, -4, 8, 8, 1, P, 4, 4, 1, 1, P, None, 0, P, 0, P, 64, None), b"size")
+
+    def held(q=P, sq=128, scale=P, ss=4):
+        return lib.sf_backward_columns_held(P, P, P, P, P, P, P, 1, 1, P, 1, None, 0, P, 8, q, sq, scale, ss, P, 8, 1, 4, 4, 8,
+                                            4, P, P, P, P, P, P, 64, None)
+
+    refused(held(q=None), b"NULL codes")
+    refused(held(q=24), b"16-B")
+    refused(held(sq=64), b"too short")
+    refused(held(ss=2), b"4-B")
