@@ -20,18 +20,30 @@ __device__ __forceinline__ float wave_sum(float v) {
   return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), 63));
 }
 
+// What v_permlane32_swap_b32 and v_permlane16_swap_b32 leave of a and b, added: of a in the lower 32 lanes (the even rows of
+// 16 lanes) each lane's value plus that of the lane 32 (16) above, of b the same in the others.
+template <int LANES>
+__device__ __forceinline__ float swap_add(float a, float b) {
+  static_assert(LANES == 32 || LANES == 16, "");
+  const auto r = LANES == 32 ? __builtin_amdgcn_permlane32_swap(__float_as_uint(a), __float_as_uint(b), false, false)
+                             : __builtin_amdgcn_permlane16_swap(__float_as_uint(a), __float_as_uint(b), false, false);
+  return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
+
 // Wave sums of 8 values at once: afterwards every lane l holds the total of v[(l >> 3) & 7].
 // A reduce-scatter: each of three exchanges (lanes 32, 16 and 8 apart) keeps half of the values
 // a lane still carries and adds its partner's copy of that half, then DPP moves sum the 8-lane
-// groups (quads, then the half-row mirror). 7 permutes and 10 adds instead of 8 full reductions.
+// groups (quads, then the half-row mirror). The first two are swaps of register halves, so no value is
+// selected and none goes through LDS.
 __device__ __forceinline__ float wave_sum8(const float (&v)[8], int lane) {
-  const bool b5 = lane & 32, b4 = lane & 16, b3 = lane & 8;
   float w[4], x[2];
 #pragma unroll
-  for (int k = 0; k < 4; ++k) w[k] = (b5 ? v[k + 4] : v[k]) + __shfl_xor(b5 ? v[k] : v[k + 4], 32);
+  for (int k = 0; k < 4; ++k) w[k] = swap_add<32>(v[k], v[k + 4]);
 #pragma unroll
-  for (int k = 0; k < 2; ++k) x[k] = (b4 ? w[k + 2] : w[k]) + __shfl_xor(b4 ? w[k] : w[k + 2], 16);
-  float y = (b3 ? x[1] : x[0]) + __shfl_xor(b3 ? x[0] : x[1], 8);
+  for (int k = 0; k < 2; ++k) x[k] = swap_add<16>(w[k], w[k + 2]);
+  const bool b3 = lane & 8;
+  float y = b3 ? x[1] : x[0];
+  y += __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(b3 ? x[0] : x[1]), 0x128, 0xF, 0xF, false));  // row_ror:8
   y = dpp_add<0xB1, 0xF>(y);   // quad_perm [1,0,3,2]
   y = dpp_add<0x4E, 0xF>(y);   // quad_perm [2,3,0,1]
   return dpp_add<0x141, 0xF>(y);  // row_half_mirror: the other quad of the 8-lane group
