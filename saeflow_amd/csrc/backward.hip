@@ -620,7 +620,7 @@ struct HeldChunk {
     else q = __builtin_bit_cast(sff8::u32x2, __builtin_amdgcn_raw_buffer_load_b64(rs, (int)k, at, 0));
   }
   // What the walk over a wave's 64 entries reads of each with readlane: where its row lies, its scale word and its
-  // scalar. Lanes without an entry take the last one's row with a scalar of zero, so the walk needs no bounds.
+  // scalar (zero in lanes without an entry, which take the last one's row).
   template <int HELD>
   static __device__ __forceinline__ void entries(const ColArgs& a, int slab, int kn, int lane, int& my_row, uint32_t& my_word) {
     my_row = lane < kn ? my_row : __builtin_amdgcn_readlane(my_row, max(kn - 1, 0));
@@ -821,15 +821,19 @@ __global__ __launch_bounds__(256) void backward_units_kernel(ColArgs a, int nsla
     int my_row = ok ? r : 0;
     my_s = ok ? my_s : 0.f;
     uint32_t my_word = 0;
+    // lanes without an entry take the last one's row with a scalar of zero, so the walk needs no bounds, and a row is
+    // its byte offset (phase A, us, against bounds and an offset for each entry: fp32 2048 tokens x 768 x 24576 features
+    // 73 -> 71, fp16 1000 x 1000 x 10007 38 -> 33, bf16 16384 x 2304 x 65536 654 -> 649: there L2 misses decide)
     if constexpr (HELD) HeldChunk<DT>::template entries<HELD>(a, (int)slab, kn, lane, my_row, my_word);
+    else if constexpr (VEC) my_row = (int)((uint32_t)(lane < kn ? my_row : __builtin_amdgcn_readlane(my_row, kn - 1)) * (uint32_t)st_bytes);
     for (int kk = 0; kk < kn; kk += U) {
       int rows[U];
       float sv[U];
 #pragma unroll
       for (int u = 0; u < U; ++u) {
-        const int sl = HELD ? kk + u : min(kk + u, kn - 1);
+        const int sl = VEC ? kk + u : min(kk + u, kn - 1);
         rows[u] = __builtin_amdgcn_readlane(my_row, sl);
-        sv[u] = HELD || kk + u < kn ? __int_as_float(__builtin_amdgcn_readlane(__float_as_int(my_s), sl)) : 0.f;
+        sv[u] = VEC || kk + u < kn ? __int_as_float(__builtin_amdgcn_readlane(__float_as_int(my_s), sl)) : 0.f;
       }
       u32x4 r[U];       // VEC: raw chunks
       float v[U][EPC];  // otherwise: elements
@@ -839,8 +843,7 @@ __global__ __launch_bounds__(256) void backward_units_kernel(ColArgs a, int nsla
         if constexpr (HELD) {
           h[u].template load<HELD>(a, rs, rows[u], coff / 16 * EPC);
         } else if constexpr (VEC) {
-          r[u] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(
-                                               rs, (int)coff, (int)((uint32_t)rows[u] * (uint32_t)st_bytes), 0));
+          r[u] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(rs, (int)coff, rows[u], 0));
         } else if (cin) {
           load_chunk<DT, false>(src + (int64_t)rows[u] * st_bytes, c, a.D, v[u]);
         } else {
