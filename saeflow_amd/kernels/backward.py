@@ -130,6 +130,7 @@ def sparse_backward(x, W_enc, b_enc, W_dec, b_dec, csr, grad_x_hat=None, grad_va
         _lib.check(lib.sf_backward_biases(g.data_ptr(), M, D, g.stride(0), code, W_enc.data_ptr(), N, W_enc.stride(0),
                                           W_enc.stride(1), code, benc, d_benc.data_ptr() if own_benc else None,
                                           benc_code or 0, d_bdec.data_ptr(), bdec_code or 0, bias_ws, bias_floats, s))
+        del scratch
         dxs = None
         if need_grad_x:  # dx' = g_pre W_enc^T: the forward decode over the rows of W_enc^T
             if W_enc.stride(0) == 1:  # W_enc is the transpose of a row-major [d_sae, d_in]

@@ -480,3 +480,24 @@ def test_transposes_of_few_tokens_are_those_of_many():
         assert torch.equal(pos.cpu().long(), order)
         assert torch.equal(rows.cpu().long(), torch.arange(M).repeat_interleave(counts)[order])
         assert torch.equal(colptr.cpu(), torch.cat([torch.zeros(1, dtype=torch.int64), torch.bincount(indices.long(), minlength=24576).cumsum(0)]))
+
+
+def test_scratch_is_given_back_before_the_gradient_of_the_tokens():
+    """W_enc's transpose and dx do not lie beside the scratch of the sums over the features."""
+    M, D, N = 2048, 512, 8192
+    x, W_enc, b_enc, W_dec, b_dec, csr, _, G, _ = problem(M, D, N, torch.float32, l0=32)
+    args = cuda(x, W_enc, b_enc, W_dec, b_dec)
+    csr, G = cuda(*csr), G.cuda()
+
+    def peak(need_grad_x):
+        torch.cuda.synchronize()
+        before = torch.cuda.memory_allocated()
+        torch.cuda.reset_peak_memory_stats()
+        got = sparse_backward(*args, csr, G, need_grad_x=need_grad_x)
+        return torch.cuda.max_memory_allocated() - before, torch.cuda.memory_allocated() - before, got
+
+    sums, kept, got = peak(False)
+    del got
+    transposed, dx = 4 * N * D, 4 * M * D
+    assert sums - kept > 4 << 20  # there is scratch to speak of
+    assert peak(True)[0] <= max(sums, kept + transposed + dx) + (1 << 20)
