@@ -152,11 +152,8 @@ def prepare(case, seed):
     # features of log-normal frequencies; a token has up to twice the mean number of them, one in sixteen has none
     k = torch.randint(0, 2 * case["l0"], (M,), generator=g, device=DEVICE)
     k[torch.rand(M, generator=g, device=DEVICE) < 1 / 16] = 0
-    # drawn through whole numbers: sums of fractions (torch.multinomial's too) vary with their order on the GPU, and
-    # a few features with them
-    upto = (torch.exp(1.5 * normal(N)) * 2.0 ** 20).long().clamp(min=1).cumsum(0)
-    at = torch.rand(M, 2 * case["l0"], generator=g, device=DEVICE, dtype=torch.float64) * upto[-1]
-    picks = torch.searchsorted(upto, at.long(), right=True).clamp(max=N - 1)
+    p = torch.exp(1.5 * normal(N))
+    picks = torch.multinomial(p, M * 2 * case["l0"], replacement=True, generator=g).view(M, -1)
     live = torch.arange(2 * case["l0"], device=DEVICE) < k[:, None]
     picks = torch.where(live, picks, N).sort(dim=1).values
     live = picks < N
