@@ -209,6 +209,17 @@ class _Writer(threading.Thread):
             raise self.failure
 
 
+def _encoder_dtype(sae, dtype):
+    """The type in which rows of `dtype` go to sae's encoder: its weights'. With an input norm the rows keep their own
+    (float32 if the norm does not take it): a rounding ahead of the norm would take rows far from zero apart, and the
+    features have to be those of encode_sparse on the same rows."""
+    from .ops import input_norm
+
+    if input_norm(sae) is None:
+        return sae.W_enc.dtype
+    return dtype if dtype in _DTYPE_NAMES else torch.float32
+
+
 @torch.inference_mode()
 def cache_activations(model, tokens, hook_names, out_dir, *, batch_size=8, batches_per_shard=32,
                       dtype=torch.float32, encoders=None):
@@ -283,7 +294,7 @@ def cache_activations(model, tokens, hook_names, out_dir, *, batch_size=8, batch
                         if isinstance(sae, Fp8Encoder):
                             csr, widths[h] = sae.encode_sparse(rows.to(sae.W.device)), len(sae.W)
                         else:
-                            csr = encode_sparse(sae, rows.to(sae.W_enc.device, sae.W_enc.dtype))
+                            csr = encode_sparse(sae, rows.to(sae.W_enc.device, _encoder_dtype(sae, rows.dtype)))
                             widths[h] = int(sae.W_enc.shape[1])
                         held[h].append((staging.to_host(csr[0]), staging.to_host(csr[1]),
                                         staging.to_host(csr[2].to(value_dtype))))
