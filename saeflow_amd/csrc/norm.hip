@@ -195,6 +195,18 @@ __device__ __forceinline__ double over_d(double sum, int64_t D, double per_d) {
   return fabs(rest) < __builtin_inf() ? fma(rest, per_d, q) : q;
 }
 __device__ __forceinline__ float inverse_std(float sum_sq, float D, float eps) { return 1.0f / sqrtf(sum_sq / D + eps); }
+// Whether 32 bits did not hold a row's sum of squares: deviations of about 1e19 overflow it (NaN and infinities in the row come
+// out here too), and squares under 2^-126 lose their bits, which matters to sums under 1e-30 where eps is as small. Such a
+// row's squares are summed again, of deviations times 2^-80 or 2^80, which hold all that counts of either sum. The look at the
+// sum costs 1 to 2% (16384 x 2304 bf16 25.8 -> 26.2 us, 4096 x 5120 21.4 -> 22.2); squares in 64 bits from the start cost 2 to
+// 9, and lost rows done again behind all others 1 to 7, by registers.
+__device__ __forceinline__ bool squares_lost(float sum_sq, float eps) {
+  return !(sum_sq < __builtin_inff()) || (sum_sq < 1e-30f && eps < 1e-30f);
+}
+__device__ __forceinline__ float squares_scale(float sum_sq) { return sum_sq < 1e-30f ? 0x1p80f : 0x1p-80f; }
+__device__ __forceinline__ float inverse_std_scaled(float sum_sq, float D, float eps, float c) {
+  return c * (1.0f / sqrtf(sum_sq / D + eps * c * c));
+}
 
 // ------------------------------------------------------------------ forward
 struct FwdArgs {
@@ -280,8 +292,10 @@ __device__ __forceinline__ void put_codes(const FwdArgs& a, int64_t m, int64_t k
 // A token alone takes 3.6 us, 5.2 before.
 // W: waves of a row, one up to 4096 elements and a block's four up to 8192, which then exchange their sums through LDS
 // (4096 rows of 5120 in bf16: 22.5 us, 52 by norm_any_kernel; of 8192 31 and 58).
+// Up to seven chunks of 16-bit types (five of fp32) without codes keep 128 registers, for the four waves a SIMD that the grid
+// gives (8192 x 3500 fp16 20.2 us, 23.2 at 132 registers).
 template <int DT, int U, bool HOLD, int W>
-__global__ __launch_bounds__(256) void norm_kernel(FwdArgs a) {
+__global__ __launch_bounds__(256, W == 1 && !HOLD && U <= (DT == SF_F32 ? 5 : 7) ? 4 : 1) void norm_kernel(FwdArgs a) {
   constexpr int ES = DT == SF_F32 ? 4 : 2, CH = W * U * 64, ROWS = 4 / W;
   constexpr bool bf = DT == SF_BF16;
   __shared__ u32x4 s_par[4 * CH];  // weight's lower and upper halves, then bias's
@@ -356,7 +370,23 @@ __global__ __launch_bounds__(256) void norm_kernel(FwdArgs a) {
       __syncthreads();
       sq = (s_sq[buf][0] + s_sq[buf][1]) + (s_sq[buf][2] + s_sq[buf][3]);
     }
-    const float rstd = inverse_std(sq, (float)D, a.eps);
+    float rstd = inverse_std(sq, (float)D, a.eps);
+    if (__builtin_expect(squares_lost(sq, a.eps), 0)) {  // wave-uniform, and with W > 1 the same in the whole block
+      const float c = squares_scale(sq);
+      sq = 0.f;
+#pragma unroll
+      for (int i = 0; i < U; ++i)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) sq = fmaf(v[i][e] * c, v[i][e] * c, sq);
+      sq = wave_sum(sq);
+      if constexpr (W > 1) {
+        if (lane == 0) s_sum[buf][wave] = (double)sq;  // (all have read the row's sum: they have met since)
+        __syncthreads();
+        sq = (float)((s_sum[buf][0] + s_sum[buf][1]) + (s_sum[buf][2] + s_sum[buf][3]));
+      }
+      rstd = inverse_std_scaled(sq, (float)D, a.eps, c);
+      sq = __builtin_inff();  // (not known to be finite)
+    }
     if constexpr (HOLD) {
       const bool finite = sq < __builtin_inff();  // so is every element: no NaN or infinity to look for
       const int words = (D + 511) / 512 * 4;
@@ -453,7 +483,21 @@ __global__ __launch_bounds__(NT == 64 ? 256 : 1024) void norm_any_kernel(FwdArgs
         sq = fmaf(d, d, sq);
       }
     }
-    const float rstd = inverse_std(row_sum<NT>(sq, s_f), (float)a.D, a.eps);
+    sq = row_sum<NT>(sq, s_f);
+    float rstd = inverse_std(sq, (float)a.D, a.eps);
+    if (squares_lost(sq, a.eps)) {  // the same in all of the row's threads
+      const float c = squares_scale(sq);
+      sq = 0.f;
+      for (int64_t k0 = t * 8; k0 < a.D; k0 += NT * 8) {
+        const Raw<ES> r = load_raw<ES>(row, k0, a.D);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const float d = k0 + e < a.D ? (raw_elem(r, e, bf) - mean) * c : 0.f;
+          sq = fmaf(d, d, sq);
+        }
+      }
+      rstd = inverse_std_scaled(row_sum<NT>(sq, s_f), (float)a.D, a.eps, c);
+    }
     if (t == 0) {
       if (a.mean) a.mean[m] = mean;
       if (a.rstd) a.rstd[m] = rstd;
