@@ -992,7 +992,13 @@ struct UndoArgs {
 __device__ __forceinline__ void inverse_pair(float rstd, float& r, float& e) {
   r = 1.0f / rstd;
   e = fmaf(-rstd, r, 1.0f) * r;
-  if (!(fabsf(e) < 1e30f)) e = 0.f;  // rstd of zero or infinity
+  if (!(fabsf(e) < __builtin_inff())) e = 0.f;  // rstd of zero or infinity
+}
+// v r + (v e + rest): v / rstd + rest. A lower part that is infinite or no number (v is, or v r is far past the largest
+// number) would undo the upper one and is left out.
+__device__ __forceinline__ float times_pair(float v, float r, float e, float rest) {
+  const float low = fmaf(v, e, rest);
+  return fmaf(v, r, fabsf(low) < __builtin_inff() ? low : rest);
 }
 
 // out = h / rstd + mean, a wave a row. Bound by memory: 24 us for 16384 x 2304 in bf16 (6.3 TB/s).
@@ -1010,7 +1016,7 @@ __global__ __launch_bounds__(256) void undo_kernel(UndoArgs a) {
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
         const float v = raw_elem(h, e, HT == SF_BF16);
-        o[e] = fmaf(v, r, fmaf(v, c, mean));
+        o[e] = times_pair(v, r, c, mean);
       }
       store8_any(a.out + m * a.som, a.out_dt, k0, a.D, o);
     }
@@ -1040,7 +1046,7 @@ __global__ __launch_bounds__(256) void undo_backward_kernel(UndoArgs a) {
       for (int e = 0; e < 8; ++e) {
         const float ge = raw_elem(g, e, GT == SF_BF16);
         s1 += ge;
-        o[e] = fmaf(ge, r, ge * c);
+        o[e] = times_pair(ge, r, c, 0.f);
       }
       if (a.out) store8_any(a.out + m * a.som, a.out_dt, k0, a.D, o);
     }
