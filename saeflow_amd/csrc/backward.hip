@@ -1550,11 +1550,15 @@ constexpr int64_t GRID_BLOCKS = 2048;  // blocks of the grid-stride backward ker
 // entries per feature (d_sae 65536, 16384 tokens, L0 64) one item per wave is fastest (four:
 // phase A 0.74 -> 0.88 ms, phase B 0.69 -> 0.77: the queue's registers cost occupancy); at 0.5
 // (d_sae 2^20, 4096 tokens, L0 128) four are (phase A 1.27 -> 0.77 ms, phase B 0.84 -> 0.55).
-// With few waves one item each is faster all the same, as a long column's items, which follow each other, then run side by
-// side (us, one item a wave -> four: fp16 d_in 1000, d_sae 10007, 1000 tokens, 20 K waves of one item 41 -> 63, 100
-// tokens, 7 K 9.7 -> 11.5; bf16 2304, 32768, 200 tokens, 58 K 37 -> 31; 65536, 1000 tokens, 184 K 80 -> 57; fp32 768,
-// 24576, 500 tokens, 74 K 31 -> 34).
-int units_per_wave(int64_t nnz, int64_t N, int64_t waves) { return nnz < 4 * N && waves >= 40000 ? 4 : 1; }
+// Four lose where features are used unevenly, as a long column's items, which follow each other, then share a wave; with few
+// waves that loss decides, with many the gain. Whole backward passes, us, one item a wave -> four, 60 (fp16: 37) entries a
+// token, features of log-normal frequencies | all alike: fp16 d_in 1000, d_sae 10007, 7.4 K waves of one item 97 -> 102 | 89 ->
+// 89, 15 K 96 -> 101 | 95 -> 93, 20 K 136 -> 152 | 106 -> 105; fp32 768, 24576, 18 K 105 -> 106 | 106 -> 104, 36 K 120 -> 124 |
+// 122 -> 118, 74 K 171 -> 178 | 150 -> 142; fp16 1000, 40000, 15 K 116 -> 116 | 118 -> 115, 30 K 139 -> 140 | 131 -> 126; bf16
+// 512, 131072, 26 K 208 -> 213 | 198 -> 192; bf16 4096, 16384, 26 K 168 -> 167 | 172 -> 166; bf16 2304, 32768, 30 K 185 -> 182 |
+// 189 -> 182, 60 K 202 -> 198 | 209 -> 198, 165 K 263 -> 255 | 260 -> 229. From about 24 K waves on four win more than they lose,
+// but at d_in 768 and 1000 with uneven features up to 80 K (up to 234 -> 298), which the host cannot tell.
+int units_per_wave(int64_t nnz, int64_t N, int64_t waves) { return nnz < 4 * N && waves >= 24000 ? 4 : 1; }
 
 bool held_near(const ColArgs& a) { return a.M * a.sxq < (1LL << 32); }
 
