@@ -353,11 +353,13 @@ class ActivationReader:
                 _as_tensor(indices[lo:hi], torch.int32),
                 _as_tensor(values[lo:hi], torch.bfloat16 if self.dtype == _FP8 else self.dtype))
 
-    def iter_batches(self, hook, batch_size):
+    def iter_batches(self, hook, batch_size, *, normed=False):
         """Yield `batch_size`-row batches in cache order (the last may be short). Dense hooks
         yield [rows, d] tensors; encoded hooks yield CSR (indptr, indices, values) tuples, which
         decode_sparse takes once they are on the GPU; dense hooks in 8 bits yield kernels.Fp8Rows,
-        which dequantize_rows and Fp8Encoder take once they are there (rows.to("cuda"))."""
+        which dequantize_rows and Fp8Encoder take once they are there (rows.to("cuda")).
+
+        normed: whether the hook lies behind a dictionary's input norm; 8-bit rows say so to an Fp8Encoder."""
         total, opened = self.n_rows(), {}
         for start in range(0, total, batch_size):
             stop = min(start + batch_size, total)
@@ -376,6 +378,6 @@ class ActivationReader:
                 from .kernels import Fp8Rows
 
                 codes, scale = (torch.cat(part) for part in zip(*pieces))
-                yield Fp8Rows(codes.view(_FP8), scale, self.manifest["hooks"][hook]["d"])
+                yield Fp8Rows(codes.view(_FP8), scale, self.manifest["hooks"][hook]["d"], normed=bool(normed))
             else:
                 yield torch.cat(pieces)

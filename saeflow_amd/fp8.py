@@ -28,14 +28,15 @@ class ActivationBuffer:
 
     center: optional [d] (a dictionary's b_dec, or the activations' mean); the buffer holds x - center,
     which spends the codes on what differs between tokens, and adds it back on reading.
+    normed: whether what is written has been through a dictionary's input norm; its rows say so to an Fp8Encoder.
     len(buffer) is the number of rows written so far, at most `rows`.
     """
 
-    def __init__(self, rows, d, *, center=None, device="cuda"):
+    def __init__(self, rows, d, *, center=None, device="cuda", normed=False):
         if rows < 1 or d < 1:
             raise ValueError(f"a buffer needs rows and a width, got {rows} x {d}")
         self.center = None if center is None else _vector(center.detach(), d, "center").clone()
-        self.store = Fp8Rows.empty(rows, d, device)
+        self.store = Fp8Rows.empty(rows, d, device, normed=bool(normed))
         self._device = _lib.require_gpu(("the buffer", self.store.q), ("center", self.center))
         self._next, self._filled = 0, 0
 
@@ -93,7 +94,8 @@ class Fp8Encoder:
 
     Tokens are quantised minus b_dec, in blocks of 128, on the way into the product. 8-bit rows (an
     ActivationBuffer's) are taken as they are: they hold x - center, `center` by default b_dec.
-    input_norm="layer_norm": tokens are normed first, as the SAE's are; 8-bit rows hold normed tokens then.
+    input_norm="layer_norm": tokens are normed first, as the SAE's are. 8-bit rows hold normed tokens then: those of a buffer or
+    a cache that were not normed are refused.
     """
 
     def __init__(self, W_enc, b_enc, b_dec, threshold=None, activation="relu", k=None, *, center=None, input_norm=None,
@@ -140,6 +142,9 @@ class Fp8Encoder:
 
     def _features(self, x, activation, row_nnz=None, out_dtype=None):
         if isinstance(x, Fp8Rows):
+            if self.input_norm is not None and x.normed is False:
+                raise ValueError("the encoder norms its tokens, and these 8-bit rows hold tokens that were not normed: pass them "
+                                 "read back, or, if they were, say normed=True to the ActivationBuffer or iter_batches")
             return fused_encode_fp8(x, self.W, self.rows_bias, self.threshold, activation, out_dtype=out_dtype,
                                     row_nnz=row_nnz)
         if self.input_norm is not None:

@@ -20,18 +20,21 @@ def _up(n, m):
     return -(-n // m) * m
 
 
-def _rows_of_bytes(q, scale, d):
-    return Fp8Rows(q.view(torch.float8_e4m3fn), scale, d)
+def _rows_of_bytes(q, scale, d, normed=None):
+    return Fp8Rows(q.view(torch.float8_e4m3fn), scale, d, normed=normed)
 
 
 class Fp8Rows:
     """R rows of d elements in 8 bits: `q` [R, d rounded up to 128] float8_e4m3fn, zeros behind d, and
     `scale` [R, ceil(d / 128) rounded up to 4] uint8. Slicing rows gives a view. The three belong together, so
-    they are not assigned to; copies and pickles are made of them alone."""
+    they are not assigned to; copies and pickles are made of them alone.
 
-    __slots__ = ("q", "scale", "d", "_strides")
+    normed: whether the rows hold tokens behind a dictionary's input norm, for an encoder that norms its tokens: None where
+    it is not known (quantize_rows), what an ActivationBuffer or a cache was told; views and copies keep it."""
 
-    def __init__(self, q, scale, d):
+    __slots__ = ("q", "scale", "d", "normed", "_strides")
+
+    def __init__(self, q, scale, d, *, normed=None):
         if q.dtype != torch.float8_e4m3fn or scale.dtype != torch.uint8:
             raise ValueError(f"8-bit rows are float8_e4m3fn codes and uint8 scales, got {q.dtype} and {scale.dtype}")
         if d < 1 or q.dim() != 2 or scale.dim() != 2 or q.shape[0] != scale.shape[0]:
@@ -45,7 +48,7 @@ class Fp8Rows:
             raise ValueError(f"codes are on {q.device}, scales on {scale.device}")
         # a lone row's stride is not used and may be anything
         strides = (q.stride(0), scale.stride(0)) if q.shape[0] > 1 else (q.shape[1], scale.shape[1])
-        for name, value in (("q", q), ("scale", scale), ("d", d), ("_strides", strides)):
+        for name, value in (("q", q), ("scale", scale), ("d", d), ("normed", normed), ("_strides", strides)):
             object.__setattr__(self, name, value)
 
     def __setattr__(self, name, value):
@@ -53,7 +56,7 @@ class Fp8Rows:
 
     def __reduce__(self):
         # (the codes as bytes: torch has no plain pickles of float8 tensors)
-        return _rows_of_bytes, (self.q.view(torch.uint8), self.scale, self.d)
+        return _rows_of_bytes, (self.q.view(torch.uint8), self.scale, self.d, self.normed)
 
     def _args(self):
         """The C ABI's (codes, their stride, scales, their stride)."""
@@ -61,7 +64,7 @@ class Fp8Rows:
         return self.q.data_ptr(), sq, self.scale.data_ptr(), ss
 
     @classmethod
-    def empty(cls, rows, d, device="cuda"):
+    def empty(cls, rows, d, device="cuda", *, normed=None):
         """Room for `rows` rows, uninitialised."""
         if rows < 0 or d < 1:
             raise ValueError(f"no room to be made for {rows} rows of {d}")
@@ -70,7 +73,7 @@ class Fp8Rows:
         q = torch.empty((rows, kp), dtype=torch.float8_e4m3fn, device=device)
         made = object.__new__(cls)  # (of the right shapes: __init__'s checks would cost 1 us)
         for name, value in (("q", q), ("scale", torch.empty((rows, sp), dtype=torch.uint8, device=q.device)), ("d", d),
-                            ("_strides", (kp, sp))):
+                            ("normed", normed), ("_strides", (kp, sp))):
             object.__setattr__(made, name, value)
         return made
 
@@ -110,10 +113,11 @@ class Fp8Rows:
     def __getitem__(self, rows):
         if not isinstance(rows, slice):
             raise TypeError("8-bit rows are sliced; dequantize_rows takes row ids")
-        return Fp8Rows(self.q[rows], self.scale[rows], self.d)
+        return Fp8Rows(self.q[rows], self.scale[rows], self.d, normed=self.normed)
 
     def to(self, device, non_blocking=False):
-        return Fp8Rows(self.q.to(device, non_blocking=non_blocking), self.scale.to(device, non_blocking=non_blocking), self.d)
+        return Fp8Rows(self.q.to(device, non_blocking=non_blocking), self.scale.to(device, non_blocking=non_blocking), self.d,
+                       normed=self.normed)
 
     def __repr__(self):
         return f"Fp8Rows({len(self)} x {self.d}, {self.device})"

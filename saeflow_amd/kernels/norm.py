@@ -104,7 +104,7 @@ def _forward(x, weight, bias, eps, out_dtype, stats, hold):
         rstd = mean + 4 * M
     held, q = None, (None, 0, None, 0)
     if hold:
-        held = Fp8Rows.empty(M, D, x.device)
+        held = Fp8Rows.empty(M, D, x.device, normed=False)
         q = held._args()
     if M:
         _run(_lib.load().sf_layer_norm, at, x.data_ptr(), row, x_code, w_ptr, w_code, b_ptr, b_code, eps, M, D,

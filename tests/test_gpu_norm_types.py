@@ -1,12 +1,15 @@
 """GPU: dictionaries with an input norm where the activations' type is not the dictionary's, and where their 8-bit rows
 were not normed."""
 
+import copy
+
 import pytest
 import torch
 
 import saeflow_amd
-from saeflow_amd import SAE
+from saeflow_amd import SAE, ActivationBuffer, Fp8Encoder, kernels
 from saeflow_amd.cache import ActivationReader, cache_activations
+from saeflow_amd.kernels import quantize_rows
 
 pytestmark = pytest.mark.gpu
 
@@ -63,3 +66,37 @@ def test_cached_features_of_a_model_in_64_bits(tmp_path):
     want = saeflow_amd.encode_sparse(sae, model.rows.detach()[tokens.cuda()].flatten(0, 1).float())
     (got,) = ActivationReader(out).iter_batches(HOOK, 20)
     assert torch.equal(got[1], want[1].cpu()) and torch.equal(got[2], want[2].float().cpu())
+
+
+# ----------------------------------------------------------------------------- 8-bit rows and an encoder that norms
+def test_rows_that_were_not_normed_are_refused_by_an_encoder_that_norms(tmp_path):
+    sae = normed_sae(96, 256, "relu", torch.bfloat16)
+    bare = SAE(96, 256, "relu", dtype=torch.bfloat16).cuda()
+    bare.load_state_dict(sae.state_dict())
+    enc, plain = Fp8Encoder.from_sae(sae), Fp8Encoder.from_sae(bare)
+    torch.manual_seed(0)
+    x = (torch.randn(40, 96, device="cuda") * 2 + 3).bfloat16()
+    z = saeflow_amd.layer_norm(x)
+    raw, normed = ActivationBuffer(64, 96, center=sae.b_dec), ActivationBuffer(64, 96, center=sae.b_dec, normed=True)
+    raw.write(x)
+    normed.write(z)
+    for call in (enc.encode, enc.encode_sparse):
+        for rows in (raw.rows(0, 40), raw.rows(3, 20)[2:5], copy.copy(raw.rows(0, 40)), kernels.layer_norm_held(x)[1]):
+            with pytest.raises(ValueError, match="normed"):
+                call(rows)
+    want = plain.encode(quantize_rows(z, shift=sae.b_dec))
+    assert torch.equal(enc.encode(normed.rows(0, 40)), want)
+    assert torch.equal(enc.encode(quantize_rows(z, shift=sae.b_dec)), want)  # rows that nobody said anything about
+    assert torch.equal(plain.encode(raw.rows(0, 40)), plain.encode(quantize_rows(x, shift=sae.b_dec)))
+    assert torch.equal(plain.encode(normed.rows(0, 40)), want)
+    assert enc.encode(raw.read()).shape == (40, 256)
+
+    tokens = torch.arange(40).view(4, 10)
+    out = cache_activations(Table(x), tokens, [HOOK], tmp_path / "c", dtype=torch.float8_e4m3fn)
+    behind = cache_activations(Table(z), tokens, [HOOK], tmp_path / "z", dtype=torch.float8_e4m3fn)
+    zeros = Fp8Encoder.from_sae(sae, center=torch.zeros(96, device="cuda"))
+    for rows in ActivationReader(out).iter_batches(HOOK, 20):
+        with pytest.raises(ValueError, match="normed"):
+            zeros.encode(rows.to("cuda"))
+    (rows,) = ActivationReader(behind).iter_batches(HOOK, 40, normed=True)
+    assert torch.equal(zeros.encode(rows.to("cuda")), zeros.encode(quantize_rows(z)))
