@@ -16,6 +16,7 @@ from types import SimpleNamespace
 import torch
 
 from .. import _lib
+from .decode import _csr_parts
 from .fp8 import Fp8Rows
 
 
@@ -30,10 +31,10 @@ def csr_transpose(indptr, indices, n_cols):
     """CSR [M, n_cols] -> (colptr int64 [n_cols+1], rows int32 [nnz], positions int32 [nnz]):
     per column, its entries' rows in increasing order and their positions in the CSR arrays.
     Deterministic. Entries whose index is outside [0, n_cols) are left out."""
+    indptr, indices, _ = _csr_parts(indptr, indices, indices)
     M = indptr.numel() - 1
     nnz = indices.numel()
     dev = _lib.require_gpu(("indptr", indptr), ("indices", indices))
-    indptr, indices = indptr.contiguous(), indices.contiguous()
     lib = _lib.load()
     colptr = torch.empty(n_cols + 1, dtype=torch.int64, device=dev)
     rows = torch.empty(nnz, dtype=torch.int32, device=dev)
@@ -68,6 +69,11 @@ def sparse_backward(x, W_enc, b_enc, W_dec, b_dec, csr, grad_x_hat=None, grad_va
     N = W_enc.shape[1]
     if W_enc.dtype != W_dec.dtype:
         raise ValueError(f"W_enc ({W_enc.dtype}) and W_dec ({W_dec.dtype}) must share a dtype")
+    if b_enc.numel() != N or b_dec.numel() != D:
+        raise ValueError(f"shape mismatch: b_enc {tuple(b_enc.shape)} and b_dec {tuple(b_dec.shape)} for W_enc {tuple(W_enc.shape)}")
+    if grad_x_hat is not None and grad_x_hat.shape != (M, D):
+        raise ValueError(f"shape mismatch: grad_x_hat {tuple(grad_x_hat.shape)}, x {tuple(x.shape)}")
+    indptr, indices, values = _csr_parts(indptr, indices, values)
     dev = _lib.require_gpu(("x", x.q if held else x), ("W_enc", W_enc), ("b_enc", b_enc), ("W_dec", W_dec), ("b_dec", b_dec),
                            ("indptr", indptr), ("indices", indices), ("values", values),
                            ("grad_x_hat", grad_x_hat), ("grad_values", grad_values))
@@ -82,9 +88,9 @@ def sparse_backward(x, W_enc, b_enc, W_dec, b_dec, csr, grad_x_hat=None, grad_va
         s = _lib.stream(dev)
         g = torch.zeros(M, D, dtype=dt, device=dev) if grad_x_hat is None else _rows(grad_x_hat, dt)
         Wd = _rows(W_dec, dt)
-        # the kernels read these as dense arrays; the gradient of a sum arrives as a view that
+        # the kernels read these as dense arrays (the CSR is one); the gradient of a sum arrives as a view that
         # expands one element (stride 0)
-        indptr, indices, values, b_dec = (t.contiguous() for t in (indptr, indices, values, b_dec))
+        b_dec = b_dec.contiguous()
         gv = None if grad_values is None else grad_values.reshape(-1).contiguous()
         if gv is not None and gv.numel() != nnz:
             raise ValueError(f"grad_values has {gv.numel()} entries for nnz={nnz}")
