@@ -459,8 +459,9 @@ SF_API int sf_encode_fp8(const void* x, int64_t sxm, int64_t sxk, int x_dt, cons
 
 /*
  * Layer norm (no reference counterpart). Rows of D elements, 1 <= D <= 2^24, unit column stride and row
- * strides in elements; any element-aligned addresses. Per row m: mean = sum x / D (summed in 64 bits), rstd =
- * 1 / sqrt(sum (x - mean)^2 / D + eps), xh = (x - mean) rstd.
+ * strides in elements; any element-aligned addresses. Per row m: mean = sum x / D (summed and divided in 64 bits), rstd =
+ * 1 / sqrt(sum (x - mean)^2 / D + eps), xh = (x - mean) rstd. Squares may pass the range of fp32, x - mean and rstd may not: such
+ * rows, and those that hold NaN or infinities, become NaN (infinite for an infinite rstd) and leave the others alone.
  *
  * sf_layer_norm: y = xh w + b, formed in fp32 and rounded once to y_dt. w, b [D] contiguous, either NULL; eps >= 0;
  *   mean, rstd fp32 [M], either NULL. With q (16-B aligned) and scale also row m of an 8-bit store of x - mean
@@ -471,7 +472,7 @@ SF_API int sf_encode_fp8(const void* x, int64_t sxm, int64_t sxk, int x_dt, cons
  *   g_mean, g_rstd fp32 [M]: gradients of mean and rstd, either NULL. dx [M, D], dw, db [D]: any of them NULL.
  *   Sums in fp32 in a fixed order. workspace: caller-owned, 4-B aligned, at least
  *   sf_layer_norm_backward_workspace_size bytes; calls in flight at the same time must not share one.
- * sf_denormalize: out = h / rstd + mean, rounded once to out_dt.
+ * sf_denormalize: out = h / rstd + mean, rounded once to out_dt; infinities stay infinite.
  * sf_denormalize_backward: dh = g / rstd, dmean[m] = sum g, drstd[m] = -sum g h / rstd^2; any of the three NULL, and
  *   h is read only for drstd.
  */

@@ -205,7 +205,8 @@ __device__ __forceinline__ bool squares_lost(float sum_sq, float eps) {
 }
 __device__ __forceinline__ float squares_scale(float sum_sq) { return sum_sq < 1e-30f ? 0x1p80f : 0x1p-80f; }
 __device__ __forceinline__ float inverse_std_scaled(float sum_sq, float D, float eps, float c) {
-  return c * (1.0f / sqrtf(sum_sq / D + eps * c * c));
+  // (infinite: a deviation itself is, or an element; NaN, as zero would leave the row's other elements at the bias)
+  return sum_sq < __builtin_inff() ? c * (1.0f / sqrtf(sum_sq / D + eps * c * c)) : __builtin_nanf("");
 }
 
 // ------------------------------------------------------------------ forward

@@ -50,6 +50,24 @@ def test_rows_up_to_the_largest_number(D):
     check_held(x, held)
 
 
+@pytest.mark.parametrize("D", [7, 96, 1000, 5000, 9000])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_rows_whose_deviations_are_infinite_are_not_numbers(dtype, D):
+    """All of the row, not the element whose deviation is; gradients too."""
+    x, w, b, g = make(5, D, dtype, seed=D)
+    x[1], x[3] = -3e38, 3e38
+    x[1, D - 1], x[3, 0] = 3e38, -3e38
+    xg, wg, bg, gg = cuda(x, w, b, g)
+    y, held, mean, rstd = kernels.layer_norm_held(xg, wg, bg)
+    y32, _, _ = kernels.layer_norm(xg, wg, bg, out_dtype=torch.float32)
+    clean = [0, 2, 4]
+    assert torch.isnan(y[[1, 3]]).all() and torch.isnan(y32[[1, 3]]).all() and torch.isfinite(mean).all()
+    check_forward(x[clean], w, b, y[clean], mean[clean], rstd[clean])
+    for source in (xg, held):
+        gr = kernels.layer_norm_backward(gg, source, mean, rstd, wg, bg)
+        assert torch.isnan(gr.x[[1, 3]]).all() and torch.isfinite(gr.x[clean]).all()
+
+
 def test_a_dictionary_over_rows_whose_squares_leave_fp32():
     """The reconstruction in the rows' own space goes with their size."""
     torch.manual_seed(0)
