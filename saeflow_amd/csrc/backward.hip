@@ -596,6 +596,7 @@ __device__ __forceinline__ float chunk_dot(const u32x4& x, const u32x4& y) {
   return d;
 }
 
+// HELD_FAR, for 4 GB of codes and more, spills four registers (20 B a lane) in the 16-bit enc_tile_kernel, bounded to 64.
 enum Held { HELD_NO = 0, HELD_NEAR = 1, HELD_FAR = 2 };
 
 // x' held in 8 bits: a lane's EPC codes of a row, and the word with the scale bytes of the row's slab (a slab of 64
@@ -1917,8 +1918,10 @@ extern "C" int sf_backward_columns_held(const int64_t* colptr, const int32_t* cs
     SF_REQUIRE(sxq >= sff8::code_bytes(D) && sxs >= sff8::scale_bytes(D),
                "sf_backward_columns_held: rows of 8 bits are too short for %lld elements", (long long)D);
   }
+  // rows of nothing are not gathered: their codes and scales, which were not looked at above, are not read either
+  const Input in = M > 0 && D > 0 ? Input{nullptr, 0, xq, sxq, xscale, sxs} : Input{nullptr, 0, nullptr, 0, nullptr, 0};
   return backward_columns(colptr, csc_row, csc_pos, plan_i64, item_col, multi_col, slot_item, max_items, max_slots, values,
-                          val_dt, g_val, gval_dt, w_dec, sw, Input{nullptr, 0, xq, sxq, xscale, sxs}, g_xhat, sg, dt, N, M, D,
+                          val_dt, g_val, gval_dt, w_dec, sw, in, g_xhat, sg, dt, N, M, D,
                           nnz, g_pre, d_wdec, d_wenc, d_benc, partials, work, work_floats, stream);
 }
 
