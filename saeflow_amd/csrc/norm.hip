@@ -7,10 +7,11 @@
 // Gradients gm and gr of mean and rstd themselves add gm / D - gr rstd^2 xh / D to dx.
 //
 // All of it is bound by HBM: a row is read once and held in registers between the sums and the result. Measured for
-// 16384 rows of 2304 in bf16 (75.5 MB; a large copy reads and writes 5.2 TB/s on this card), the data partly in the
-// last-level cache: forward 25.5 us (5.9 TB/s), with 8-bit rows 38 (33 where x was just read; 5.7), backward 43 (5.3), from
-// 8-bit rows 41 (4.6), undone 24 (6.3), its backward pass 35 to 39 (5.8 to 6.5). In fp32 58, 68, 90, 69, 56 and 88 us
-// (4.9 to 5.4 TB/s). Rows of 2303 begin anywhere and take 3 to 10% longer.
+// 16384 rows of 2304 in bf16 (75.5 MB; a large copy reads and writes 4.9 TB/s on this card), calls one after the other, the
+// data partly in the last-level cache: forward 26.2 us (5.8 TB/s), with 8-bit rows 32.9 (5.7; 38 where x was not just read),
+// backward with its parameters' sums 43 (5.2), from 8-bit rows 40 (4.7), undone 24.4 (6.2), its backward pass 35 (6.4; 38
+// behind other kernels). In fp32 62, 71, 92, 71, 65 and 90 us (4.6 to 5.3 TB/s). Rows of 2303 begin anywhere and take 3 to
+// 18% longer.
 #include <algorithm>
 #include <type_traits>
 
@@ -456,8 +457,9 @@ template <>
 __device__ __forceinline__ float row_sum<1024>(float v, float* s) { return block_sum_1024(v, s); }
 
 // Everything else, in three passes over the row, the last two out of the caches: a wave a row where y is of another type
-// than x or rows have less than eight elements, a block of 1024 a row where no block holds it (2048 rows of 12288 in bf16
-// 40 us, 2.5 TB/s).
+// than x or rows have less than eight elements (16384 x 2304 bf16 to fp32 57 us, 4.0 TB/s), a block of 1024 a row where no
+// block holds it (2048 rows of 12288 in bf16 40 us, 2.5 TB/s of the bytes that it cannot do without, fp32 48, 4.2; 512 of
+// 32768 bf16 25, 2.7): each pass waits for the row's sum before the next one's loads begin.
 template <int DT, bool HOLD, int NT>
 __global__ __launch_bounds__(NT == 64 ? 256 : 1024) void norm_any_kernel(FwdArgs a) {
   constexpr int ES = DT == SF_F32 ? 4 : 2, ROWS = NT == 64 ? 4 : 1;
@@ -619,8 +621,9 @@ __device__ __forceinline__ void put_sums(const BwdArgs& a, int64_t k0, const flo
 // The general form: types that mix, up to 8192 elements. R rows at a time by a team of T <= 8 waves, a lane holding the same U chunks of eight columns of every row, so
 // that the columns' sums stay in its registers over all rows of the block. A row's two sums go over the team
 // through LDS, those of R rows together (one barrier a batch, two buffers), while the next batch's loads are under
-// way. Teams of one or two waves share a block, which adds up its teams' column sums at the end. (16384 x 2304, x in bf16 and
-// g in fp32: 74 us, 4.1 TB/s.)
+// way. Teams of one or two waves share a block, which adds up its teams' column sums at the end. (With the parameters'
+// sums: 16384 x 2304, x in bf16 and g in fp32, 75 us, 4.0 TB/s; all bf16 4096 x 5120 43 us, 2.9 TB/s, from 8-bit rows 43, 4096 x
+// 8192 51, 3.9, and 49: two chunks a lane take 173 registers, two waves a SIMD.)
 constexpr int MAX_T = 8;
 template <int XT, int GT, int U>
 __global__ __launch_bounds__(64 * MAX_T) void norm_backward_kernel(BwdArgs a) {
@@ -772,9 +775,11 @@ __global__ __launch_bounds__(64 * MAX_T) void norm_backward_kernel(BwdArgs a) {
 // the row's last whole chunk and rows past the last without a branch, so that waiting for the next row's loads does not
 // wait for the last row's stores. Elements are unpacked once, into the registers that both halves use, and g xh is formed
 // once for both sums it is in: thirteen vector instructions an element (16384 x 2304 bf16: 67 us by the general form). One row
-// at a time keeps the registers at 80 (96 in fp32), for two blocks of up to ten waves a CU: 41 us, two rows and 128
-// registers 46; from 8-bit rows 43 with 80 registers, 58 with 96. A single block for few rows, which would save the launch
-// of norm_params_kernel, was slower from 16 rows on (32 rows 21 us against 14).
+// at a time keeps the registers at 80 (96 in fp32), for two blocks of up to ten waves a CU: 5 us less than two rows at 128
+// registers, from 8-bit rows 15 less than at 96. A single block for few rows, which would save the launch
+// of norm_params_kernel, was slower from 16 rows on (32 rows 21 us against 14). The row's sums are multiplied by a rounded
+// 1 / D, half a unit more of error than a division's. A team of one row each makes a part for every few rows: 2048 x 768 fp32
+// takes 10 us and another 5.8 to add 410 parts up, four times what its bytes need.
 constexpr int FAST_WAVES = 10;
 template <int XT, int GT>
 __global__ __launch_bounds__(64 * FAST_WAVES, GT == SF_F32 ? 5 : 6) void norm_backward_fast_kernel(BwdArgs a) {
@@ -906,7 +911,9 @@ __global__ __launch_bounds__(1024) void norm_params_kernel(const float* part, in
   }
 }
 
-// Rows longer than a team holds, or shorter than eight elements: dx by a block a row in two passes ...
+// Rows longer than a team holds, or shorter than eight elements: dx by a block a row in two passes ... (With the
+// parameters' sums, which read x and g a third time: 2048 x 12288 bf16 62 us, 2.4 TB/s of the bytes that it cannot do without,
+// fp32 97, 3.1; 512 x 32768 bf16 48, 2.1. Rows under eight elements keep one lane of a block's 1024 busy: 65536 x 4 1.3 ms.)
 template <int XT, int GT>
 __global__ __launch_bounds__(1024) void norm_backward_long_kernel(BwdArgs a) {
   constexpr int GES = GT == SF_F32 ? 4 : 2;
