@@ -73,7 +73,8 @@ def sparse_backward(x, W_enc, b_enc, W_dec, b_dec, csr, grad_x_hat=None, grad_va
         raise ValueError(f"shape mismatch: b_enc {tuple(b_enc.shape)} and b_dec {tuple(b_dec.shape)} for W_enc {tuple(W_enc.shape)}")
     if grad_x_hat is not None and grad_x_hat.shape != (M, D):
         raise ValueError(f"shape mismatch: grad_x_hat {tuple(grad_x_hat.shape)}, x {tuple(x.shape)}")
-    indptr, indices, values = _csr_parts(indptr, indices, values)
+    if indices.dtype != torch.int32 or indptr.dtype != torch.int64 or values.numel() != indices.numel():
+        indptr, indices, values = _csr_parts(indptr, indices, values)  # (3 us on the host, so not where all fits)
     dev = _lib.require_gpu(("x", x.q if held else x), ("W_enc", W_enc), ("b_enc", b_enc), ("W_dec", W_dec), ("b_dec", b_dec),
                            ("indptr", indptr), ("indices", indices), ("values", values),
                            ("grad_x_hat", grad_x_hat), ("grad_values", grad_values))
@@ -88,9 +89,9 @@ def sparse_backward(x, W_enc, b_enc, W_dec, b_dec, csr, grad_x_hat=None, grad_va
         s = _lib.stream(dev)
         g = torch.zeros(M, D, dtype=dt, device=dev) if grad_x_hat is None else _rows(grad_x_hat, dt)
         Wd = _rows(W_dec, dt)
-        # the kernels read these as dense arrays (the CSR is one); the gradient of a sum arrives as a view that
+        # the kernels read these as dense arrays; the gradient of a sum arrives as a view that
         # expands one element (stride 0)
-        b_dec = b_dec.contiguous()
+        indptr, indices, values, b_dec = (t.contiguous() for t in (indptr, indices, values, b_dec))
         gv = None if grad_values is None else grad_values.reshape(-1).contiguous()
         if gv is not None and gv.numel() != nnz:
             raise ValueError(f"grad_values has {gv.numel()} entries for nnz={nnz}")
